@@ -11,7 +11,7 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SCALAR = {"int": "c_int", "float": "f32", "size_t": "usize", "long long": "c_longlong", "uint64_t": "u64",
-          "uint32_t": "u32", "unsigned char": "u8", "int8_t": "i8", "char": "c_char", "void": "c_void",
+          "uint32_t": "u32", "uint8_t": "u8", "unsigned char": "u8", "int8_t": "i8", "char": "c_char", "void": "c_void",
           "unsigned int": "c_uint", "double": "f64", "uint16_t": "u16", "int32_t": "i32", "int64_t": "i64"}
 OPAQUE = {"mx230_handle": "Mx230Handle", "mx230_kv_pool": "Mx230KvPool", "mx230_sched": "Mx230Sched",
           "mx230_splitkv_comm": "Mx230SplitKvComm"}

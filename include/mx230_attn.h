@@ -98,7 +98,28 @@ enum {
     MX230_K_GEMV = 12,
     MX230_K_BWD_FUSED = 13,
     MX230_K_ZERO = 14, /* dQ cleared in front of the fused backward, where no staging launch does so on the way */
-    MX230_K_COUNT = 15
+    MX230_K_ROTARY = 15,
+    MX230_K_GEMV_INT4 = 16,
+    MX230_K_PACK_INT4 = 17,
+    MX230_K_COUNT = 18
+};
+
+/* element types, where an entry point takes several */
+enum {
+    MX230_F32 = 0,
+    MX230_F16 = 1,
+    MX230_BF16 = 2
+};
+
+/* how mx230_rotary_table stretches the angles for contexts longer than the trained one */
+enum {
+    MX230_ROTARY_PLAIN = 0,
+    MX230_ROTARY_LINEAR = 1,     /* every frequency / factor */
+    MX230_ROTARY_NTK = 2,        /* base * factor^(rot_dim / (rot_dim - 2)) */
+    MX230_ROTARY_WAVELENGTH = 3, /* by the turns a pair makes over `length`: at least `high` as it is, at most `low` / factor,
+                                    linear in the turns between */
+    MX230_ROTARY_YARN = 4        /* linear in the pair's index between those that make `high` and `low` turns over `length`
+                                    (rounded outwards): as it is below, / factor above; outputs times 0.1 ln(factor) + 1 */
 };
 
 typedef struct mx230_handle mx230_handle;
@@ -200,6 +221,22 @@ int mx230_rope_batch(mx230_handle *h, void *stream, float *qkv, int pos0, int n_
                      int n_kv_head, int head_dim, int stride, float theta);
 int mx230_rope_seqpos(mx230_handle *h, void *stream, float *qkv, const int *pos, int n_seq,
                       int n_head, int n_kv_head, int head_dim, int stride, float theta);
+
+/* Rotary positions in the forms that the reference's kernels do not have (beside mx230_rope*, whose bits they do not share: the
+ * angles are exact here at any position).  x [n_rows][n_head][head_dim] of `dtype` with any strides between rows and heads (in
+ * elements; a token-major qkv row, or [n_head][n_rows][head_dim] as mx230_attn_flash takes it), out likewise, or x itself with
+ * the same strides; otherwise the two do not overlap.  The first rot_dim values of a head are rotated, the rest goes over as it
+ * is.  Pair i is (i, i + rot_dim / 2), or (2i, 2i + 1) if interleaved; row r is at position pos[r], or pos0 + r without `pos`
+ * (negative ones too):
+ *     a' = (a cos - b sin) factor, b' = (a sin + b cos) factor, angle = position * frequency i
+ * inverse != 0: -angle; this is also the gradient of the forward call.  Computed in fp32, rounded once to `dtype`.
+ * `turns` [rot_dim / 2]: the frequencies in units of 2^-64 turns per position, in device memory.  mx230_rotary_table computes
+ * them on the host for frequencies theta^(-2i / rot_dim), stretched as MX230_ROTARY_* says, and the factor that goes with them. */
+int mx230_rotary_table(uint64_t *turns_host, float *factor_host, int rot_dim, double theta, int scaling, double factor,
+                       double low, double high, int length);
+int mx230_rotary(mx230_handle *h, void *stream, void *out, const void *x, int dtype, const int *pos, int pos0,
+                 const uint64_t *turns, float factor, int n_rows, int n_head, int head_dim, int rot_dim, int interleaved,
+                 int inverse, long long x_row, long long x_head, long long out_row, long long out_head);
 
 /* fp32 KV write: copy_kv_dyn / copy_kv_paged_dyn (llm.cu:965-986), copy_kv_batch /
  * copy_kv_batch_paged (llm.cu:3635-3655), copy_kv_seqpos (llm.cu:1491-1501);
@@ -484,6 +521,20 @@ int mx230_gemm(mx230_handle *h, void *stream, float *C, const float *A, const vo
  * nearest even; integer dots by dp4a; y[o] (+)= (sum_g dot_g * xs_g) * scales[o] + b[o].  n_in % 8 == 0. */
 int mx230_gemv_int8(mx230_handle *h, void *stream, float *y, const float *x, const void *w_packed,
                     const float *scales, const float *b, int n_in, int n_out, int accum, int act_group);
+/* The same for up to a few rows over 4-bit weights with group scales (decode tokens of several sequences):
+ *     y[r][o] = sum_i x[r][i] scale[i / group][o] (code[i][o] - zero[i / group][o]) + bias[o] + add[r][o]
+ * x, y, bias, add fp32, rows x_stride, y_stride, add_stride elements apart; bias and add may be null, add may be y (with its
+ * stride).  Any n_in, n_out and number of rows; built for 1 to 16 rows, more go in turns over the weights.  A row's bits do not depend on the
+ * rows computed with it.  `packed` (mx230_int4_bytes, 16-byte aligned) is made once by mx230_pack_int4 from codes [n_in][n_out] (the
+ * low four bits of a byte), fp16 scales and zeros [ceil(n_in / group)][n_out] (zeros null: 8); group 32 or a multiple of 64.
+ * Weights and both parts of x (22 bits of it, relative to the largest of 64) are exact on the tensor cores; sums are fp32.
+ * No workspace. */
+size_t mx230_int4_bytes(int n_in, int n_out, int group);
+int mx230_pack_int4(mx230_handle *h, void *stream, void *packed, const uint8_t *codes, const void *scales_fp16,
+                    const uint8_t *zeros, int n_in, int n_out, int group);
+int mx230_gemv_int4(mx230_handle *h, void *stream, float *y, const float *x, const void *packed, const float *bias,
+                    const float *add, int n_rows, int n_in, int n_out, int group, long long x_stride, long long y_stride,
+                    long long add_stride);
 /* The qkv step in one launch: qkv = x W + b (W [n_in][(n_head + 2 n_kv_head) * 64]; w_kind 0 fp32, 1 fp16,
  * 2 int8 packed with w_scales and act_group as for mx230_gemv_int8), RoPE at `pos` (or *pos_ptr when
  * non-null: the graph-captured decode) on the Q and K heads, K and V rows written to cache row pos

@@ -78,6 +78,16 @@ extern "C" {
         h: *mut Mx230Handle, stream: *mut c_void, qkv: *mut f32, pos: *const c_int, n_seq: c_int, n_head: c_int,
         n_kv_head: c_int, head_dim: c_int, stride: c_int, theta: f32,
     ) -> c_int;
+    pub fn mx230_rotary_table(
+        turns_host: *mut u64, factor_host: *mut f32, rot_dim: c_int, theta: f64, scaling: c_int, factor: f64,
+        low: f64, high: f64, length: c_int,
+    ) -> c_int;
+    pub fn mx230_rotary(
+        h: *mut Mx230Handle, stream: *mut c_void, out: *mut c_void, x: *const c_void, dtype: c_int,
+        pos: *const c_int, pos0: c_int, turns: *const u64, factor: f32, n_rows: c_int, n_head: c_int,
+        head_dim: c_int, rot_dim: c_int, interleaved: c_int, inverse: c_int, x_row: c_longlong, x_head: c_longlong,
+        out_row: c_longlong, out_head: c_longlong,
+    ) -> c_int;
     pub fn mx230_copy_kv(
         h: *mut Mx230Handle, stream: *mut c_void, kcache: *mut f32, vcache: *mut f32, qkv: *const f32, pos: c_int,
         q_dim: c_int, kv_dim: c_int,
@@ -300,6 +310,16 @@ extern "C" {
     pub fn mx230_gemv_int8(
         h: *mut Mx230Handle, stream: *mut c_void, y: *mut f32, x: *const f32, w_packed: *const c_void,
         scales: *const f32, b: *const f32, n_in: c_int, n_out: c_int, accum: c_int, act_group: c_int,
+    ) -> c_int;
+    pub fn mx230_int4_bytes(n_in: c_int, n_out: c_int, group: c_int) -> usize;
+    pub fn mx230_pack_int4(
+        h: *mut Mx230Handle, stream: *mut c_void, packed: *mut c_void, codes: *const u8, scales_fp16: *const c_void,
+        zeros: *const u8, n_in: c_int, n_out: c_int, group: c_int,
+    ) -> c_int;
+    pub fn mx230_gemv_int4(
+        h: *mut Mx230Handle, stream: *mut c_void, y: *mut f32, x: *const f32, packed: *const c_void,
+        bias: *const f32, add: *const f32, n_rows: c_int, n_in: c_int, n_out: c_int, group: c_int,
+        x_stride: c_longlong, y_stride: c_longlong, add_stride: c_longlong,
     ) -> c_int;
     pub fn mx230_qkv_rope_kvwrite(
         h: *mut Mx230Handle, stream: *mut c_void, qkv: *mut f32, x: *const f32, w: *const c_void, w_kind: c_int,

@@ -19,7 +19,8 @@ ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_CUDA, ERR_DEVICE_STATUS, ER
 Q8_SCORE_REF, Q8_SCORE_EXACT = 0, 1
 OPT_Q8_SCORE_MODE, OPT_DECODE_CHUNK, OPT_DECODE_TENSOR, OPT_BWD_TWO_PASS = 1, 2, 3, 4
 OPT_BWD_REUSE_STAGED, OPT_WAIT_LIMIT, OPT_TEST_DROP_TILE = 5, 6, 7
-K_COUNT = 15
+F32, F16, BF16 = 0, 1, 2
+K_COUNT = 18
 
 
 class Mx230Error(RuntimeError):
@@ -29,7 +30,7 @@ class Mx230Error(RuntimeError):
 
 
 _CTYPE = {
-    "int": C.c_int, "float": C.c_float, "size_t": C.c_size_t, "long long": C.c_longlong, "void": None, "uint32_t": C.c_uint32,
+    "int": C.c_int, "float": C.c_float, "double": C.c_double, "size_t": C.c_size_t, "long long": C.c_longlong, "void": None, "uint32_t": C.c_uint32,
     "uint64_t": C.c_uint64,
 }
 
@@ -87,6 +88,12 @@ def lib() -> C.CDLL:
 def check(code: int) -> None:
     if code != OK:
         raise Mx230Error(code, lib().mx230_last_error().decode())
+
+
+def require(cond, msg: str) -> None:
+    """The bindings' own checks, for what no pointer shows (shapes, types, devices): the error that the library would raise."""
+    if not cond:
+        raise Mx230Error(ERR_INVALID_ARG, msg)
 
 
 def ptr(t) -> C.c_void_p | None:

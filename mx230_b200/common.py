@@ -67,16 +67,16 @@ def _stream_getter():
     import torch
     raw, device = (getattr(torch._C, n, None) for n in ("_cuda_getCurrentRawStream", "_cuda_getDevice"))
     if raw is None or device is None:
-        return lambda: torch.cuda.current_stream().cuda_stream
+        return lambda d: torch.cuda.current_stream(d).cuda_stream
     torch.cuda.current_stream()   # (initialises CUDA, which the calls above take for granted)
-    return lambda: raw(device())
+    return lambda d: raw(device() if d is None else d)
 
 
 _current_raw_stream = None
 
 
-def stream_ptr(stream=None):
-    """Raw CUstream of a torch stream (None = torch's current stream)."""
+def stream_ptr(stream=None, device=None):
+    """Raw CUstream of a torch stream (None = torch's current stream, of the current device or of `device`)."""
     if isinstance(stream, int):
         return C.c_void_p(stream)
     if stream is not None:
@@ -84,7 +84,7 @@ def stream_ptr(stream=None):
     global _current_raw_stream
     if _current_raw_stream is None:
         _current_raw_stream = _stream_getter()
-    return C.c_void_p(_current_raw_stream())
+    return C.c_void_p(_current_raw_stream(device))
 
 
 def time_median_ms(stream, warmup: int, iters: int, f) -> float:

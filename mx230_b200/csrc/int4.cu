@@ -1,0 +1,408 @@
+// Products of a few rows with a matrix of 4-bit weights (the projections of a decode step, beside mx230_gemv and mx230_gemv_int8):
+//   y[r][o] = sum_i x[r][i] s[g][o] (q[i][o] - z[g][o]) + bias[o] + add[r][o],   g = i / group
+//
+// Bounded by HBM on the weights: half a byte each, read once, and 4 bytes of scale and zero point per group.  At that rate an SM
+// takes 46 weights a cycle, so a weight may cost about two instructions of a lane; multiply-adds on CUDA cores, with the
+// conversion from 4 bits in front, would take more for a single row and that many times more for several.  Hence warp-level
+// tensor-core tiles (m16n8k16) with the weights as A: 16 outputs x 16 inputs, q - z formed exactly in fp16 (two instructions for
+// two weights: the four bits or'ed into the mantissa of 1024, or of 64 + z in sixteenths, and the offset taken off), and the rows as
+// the eight columns of B, two columns a row:
+//   x 2^e = hi + lo, both fp16, e such that the largest of the 64 values of a tile lies in [2^14, 2^15):
+// |x 2^e - hi - lo| <= 2^-24 |x 2^e|, as exact as x itself (but for values 2^-15 times the tile's largest and less, which keep an
+// absolute error of 2^-40 of that).  Products are then exact in fp32; sums are fp32, per tile of 64 inputs (32, if groups are of
+// 32), and are multiplied by s 2^-e into the row's fp32 total.
+//
+// Layout, made once by mx230_pack_int4: tiles of 16 outputs x 64 inputs, 512 bytes, of which lane (g = lane / 4, j = lane % 4) has 16:
+// words [row g: inputs 8j .. 8j+7][row g: inputs 32 + 8j ..][row g + 8: 8j ..][row g + 8: 32 + 8j ..], input 2p of eight at bits
+// 4p, input 2p + 1 at bits 16 + 4p.  (Which input a k index of the MMA stands for is free, as long as A and B agree.)  Tiles of an
+// output row follow one another along the inputs; behind all tiles, per (16 outputs, group), 16 words (s, 1024 + z) of fp16.
+//
+// Order of the sums: the inputs are cut into S slices (a power of two that depends on n_in and n_out alone), each summed by one warp
+// in index order, and the slices are added pairwise.  So a row has the same bits whatever rows are computed with it.
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace {
+
+constexpr int W4_K = 64;          // inputs of a tile
+constexpr int W4_N = 16;          // outputs of a tile
+constexpr int W4_WARPS = 8;
+constexpr int W4_THREADS = W4_WARPS * 32;
+constexpr int W4_CLUSTER = 8;     // most CTAs whose sums are added through shared memory
+constexpr int W4_X_BYTES = 64 * 1024;   // of shared memory for rows, about
+
+struct Int4Params {
+    float *y;
+    const float *x;
+    const uint4 *codes;      // [n_tiles][k_tiles][32]
+    const uint32_t *sz;      // [n_tiles][groups][16]
+    const float *bias, *add;
+    int n_rows, n_in, n_out, group, groups;
+    int n_tiles, k_tiles;
+    int kw, ctas_k;          // warps of a CTA along the inputs, CTAs of a cluster; kw * ctas_k slices
+    int xq;                  // tiles of a slice whose rows are in shared memory at a time
+    int x_vec;               // rows are 16-byte aligned
+    long long x_stride, y_stride, add_stride;
+};
+
+// (s, 1024 + z) and codes of one output tile and input tile; padding: s = 0
+__global__ void pack_int4_kernel(uint4 *codes_out, uint32_t *sz_out, const uint8_t *codes, const __half *scales, const uint8_t *zeros,
+                                 int n_in, int n_out, int group, int n_tiles, int k_tiles, int groups) {
+    const long long n_codes = (long long)n_tiles * k_tiles * 32, n_sz = (long long)n_tiles * groups * 16;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n_codes + n_sz; i += (long long)gridDim.x * blockDim.x) {
+        if (i < n_codes) {
+            const int lane = (int)(i & 31), g = lane >> 2, j = lane & 3;
+            const long long t = i >> 5;
+            const int nt = (int)(t / k_tiles), kt = (int)(t - (long long)nt * k_tiles);
+            uint32_t w[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int o = nt * W4_N + g + (q >> 1) * 8, k0 = kt * W4_K + (q & 1) * 32 + 8 * j;
+                uint32_t v = 0;
+                for (int e = 0; e < 8; ++e)
+                    if (o < n_out && k0 + e < n_in) v |= (uint32_t)(codes[(size_t)(k0 + e) * n_out + o] & 15) << (4 * (e >> 1) + 16 * (e & 1));
+                w[q] = v;
+            }
+            codes_out[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            const long long s = i - n_codes;
+            const long long t = s >> 4;
+            const int nt = (int)(t / groups), gr = (int)(t - (long long)nt * groups), o = nt * W4_N + (int)(s & 15);
+            __half sc = __float2half(0.0f), z = __float2half(1024.0f + 8.0f);
+            if (o < n_out) {
+                sc = scales[(size_t)gr * n_out + o];
+                if (zeros) z = __float2half(1024.0f + (float)zeros[(size_t)gr * n_out + o]);
+            }
+            sz_out[s] = (uint32_t)__half_as_ushort(sc) | (uint32_t)__half_as_ushort(z) << 16;
+        }
+    }
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {   // (a & b) | c in one instruction
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t h2_u(__half2 v) { return *(uint32_t *)&v; }
+__device__ __forceinline__ __half2 u_h2(uint32_t v) { return *(__half2 *)&v; }
+
+// eight codes -> four pairs (inputs 2p, 2p + 1) of q - z; z1024 = (1024 + z) twice, z64 = -(64 + z) twice
+__device__ __forceinline__ void dequant8(uint32_t w, __half2 z1024, __half2 z64, uint32_t (&a)[4]) {
+    const __half2 sixteenth = __float2half2_rn(0.0625f);
+    const uint32_t v = w >> 8;
+    a[0] = h2_u(__hsub2(u_h2(and_or(w, 0x000F000Fu, 0x64006400u)), z1024));
+    a[1] = h2_u(__hfma2(u_h2(and_or(w, 0x00F000F0u, 0x64006400u)), sixteenth, z64));   // (1024 + 16 q) / 16 - 64 - z
+    a[2] = h2_u(__hsub2(u_h2(and_or(v, 0x000F000Fu, 0x64006400u)), z1024));
+    a[3] = h2_u(__hfma2(u_h2(and_or(v, 0x00F000F0u, 0x64006400u)), sixteenth, z64));
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// pairwise sum of n (a power of two, at most 8) values `step` apart
+__device__ __forceinline__ float tree_sum(const float *p, int n, int step) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i * step] : 0.0f;
+    if (n > 1) v[0] += v[1], v[2] += v[3], v[4] += v[5], v[6] += v[7];
+    if (n > 2) v[0] += v[2], v[4] += v[6];
+    return n > 4 ? v[0] + v[4] : v[0];
+}
+
+// NT: column tiles of four rows.  T: output tiles of a warp.  G32: groups of 32 inputs (else a multiple of 64).
+// Shared memory: rows [kw][xq][NT][lanes][8 words], their scales [kw][xq][NT * 4], ring [8 warps][STAGES][T][512 + 64 or 128],
+// sums [8 warps][T * NT * 64]; in the first CTA of a cluster also the other CTAs' sums.
+constexpr int STAGES = 6;
+template <int NT, int T, bool G32>
+struct Int4Smem {
+    static constexpr int SZ = G32 ? 128 : 64;               // bytes of (s, z) of a tile
+    static constexpr int STAGE = T * (512 + SZ);
+    static constexpr int RING = W4_WARPS * STAGES * STAGE;
+    static constexpr int SUMS = T * NT * 64;                // floats of a warp
+};
+
+template <int NT, int T, bool G32>
+__global__ void __launch_bounds__(W4_THREADS) gemv_int4_kernel(const Int4Params P) {
+    using S = Int4Smem<NT, T, G32>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
+    const int kw = P.kw, tg = W4_WARPS / kw, C = P.ctas_k;
+    const int rank = blockIdx.x % C, grp = blockIdx.x / C;
+    const int row0 = blockIdx.y * (4 * NT), rows = min(4 * NT, P.n_rows - row0);
+    const int rt = min(4, rows);                            // rows of a column tile that are there at all
+    const int x_lanes = NT == 1 ? 8 * rt : 32;
+    unsigned char *ring = smem + warp * (STAGES * S::STAGE);
+    float *sums = (float *)(smem + S::RING);                // [8][SUMS]
+    float *parts = sums + W4_WARPS * S::SUMS;               // [C][tg][SUMS], first CTA
+    float *xscale = parts + (C > 1 ? C * tg * S::SUMS : 0); // [kw][xq][NT * 4]
+    uint32_t *xf = (uint32_t *)(xscale + kw * P.xq * NT * 4);   // [kw][xq][NT][x_lanes][8]
+
+    mx::pdl_trigger();
+    if (C > 1) mx::cluster_arrive_relaxed();   // waited for before the first store to another CTA's memory
+    mx::pdl_wait();
+
+    // this warp's slice and output tiles
+    const int ws = warp % kw, slice = rank * kw + ws, n_slices = C * kw;
+    const int t_first = (grp * tg + warp / kw) * T;
+    const int k0 = (int)((long long)P.k_tiles * slice / n_slices), k1 = (int)((long long)P.k_tiles * (slice + 1) / n_slices);
+    const int per_group = G32 ? 1 : P.group / W4_K;
+    auto request = [&](int kt, int stage) {
+        if (kt < k1 && t_first < P.n_tiles) {
+            unsigned char *dst = ring + stage * S::STAGE;
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                const int nt = min(t_first + t, P.n_tiles - 1);
+                cp_async16(mx::smem_u32(dst + t * 512 + lane * 16), P.codes + ((size_t)nt * P.k_tiles + kt) * 32 + lane);
+            }
+            constexpr int LPT = S::SZ / 16;                 // lanes that fetch (s, z) of a tile
+            if (lane < T * LPT) {
+                const int nt = min(t_first + lane / LPT, P.n_tiles - 1);
+                // (a second group of 32 behind the last one: the padding of the inputs, whatever it is multiplied by is 0)
+                const int gr = G32 ? min(2 * kt + (lane % LPT) / 4, P.groups - 1) : kt / per_group;
+                cp_async16(mx::smem_u32(dst + T * 512 + lane * 16), P.sz + ((size_t)nt * P.groups + gr) * 16 + (lane & 3) * 4);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) request(k0 + s, s);
+
+    float total[T][NT][2];
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) total[t][n][0] = total[t][n][1] = 0.0f;
+
+    const int most = (P.k_tiles + n_slices - 1) / n_slices;   // tiles of the longest slice
+    int stage = 0;
+    for (int c0 = 0; c0 < most; c0 += P.xq) {
+        if (c0) __syncthreads();
+        // ---- rows of the next xq tiles of every slice: scaled, split, in the order of B's fragments ----
+        // a thread takes the 16 inputs (8j .. , 32 + 8j ..) of a (slice, tile, row); the four of a row follow one another
+        const int n_x = kw * P.xq * NT * 4 * 4;
+        for (int i0 = tid & ~31; i0 < n_x; i0 += W4_THREADS) {   // (whole warps, for the shuffles)
+            const int i = min(i0 + lane, n_x - 1);
+            const int jj = i & 3, r = (i >> 2) & (NT * 4 - 1), q = (i >> 2) / (NT * 4), sl = q / P.xq, kk = q - sl * P.xq;
+            const int s_ = rank * kw + sl;
+            const int kt = (int)((long long)P.k_tiles * s_ / n_slices) + c0 + kk;
+            const bool in = i0 + lane < n_x && r < rows && c0 + kk < most && kt < P.k_tiles;
+            float v[16];
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const int k = kt * W4_K + hf * 32 + 8 * jj;
+                const float *src = P.x + (long long)(row0 + r) * P.x_stride + k;
+                if (in && P.x_vec && k + 8 <= P.n_in) {
+                    *(float4 *)&v[8 * hf] = *(const float4 *)src, *(float4 *)&v[8 * hf + 4] = *(const float4 *)(src + 4);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[8 * hf + e] = in && k + e < P.n_in ? src[e] : 0.0f;
+                }
+            }
+            float amax = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(v[e]));
+            amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
+            // 2^(14 - exponent of amax) and its inverse, by their bits
+            const int eb = max((int)(__float_as_uint(amax) >> 23), 15);
+            const float up = __uint_as_float((uint32_t)(268 - eb) << 23);
+            if (i0 + lane >= n_x) continue;
+            if (jj == 0) xscale[q * (NT * 4) + r] = __uint_as_float((uint32_t)(eb - 14) << 23);
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float a = v[2 * e] * up, b = v[2 * e + 1] * up;
+                const __half ha = __float2half_rn(a), hb = __float2half_rn(b);
+                const float fa = __half2float(ha), fb = __half2float(hb);
+                hi[e] = h2_u(__halves2half2(ha, hb));
+                // (an infinite value has no second part)
+                lo[e] = h2_u(__halves2half2(__float2half_rn(isinf(fa) ? 0.0f : a - fa), __float2half_rn(isinf(fb) ? 0.0f : b - fb)));
+            }
+            const int n = r >> 2, l = (r & 3) * 8 + jj;     // lanes of columns 2 (r % 4) and 2 (r % 4) + 1
+            if (l < x_lanes) {
+                // pairs 0 .. 3 of each half of the tile: MMA steps 2 hf, 2 hf + 1 take two each
+                uint4 *dst = (uint4 *)(xf + ((size_t)(q * NT + n) * x_lanes + l) * 8);
+                dst[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]), dst[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+                dst += 8;
+                dst[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]), dst[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+            }
+        }
+        __syncthreads();
+        // ---- this warp's tiles ----
+        const int end = min(k1 - k0, c0 + P.xq);
+        for (int kk = c0; kk < end; ++kk) {
+            cp_async_wait<STAGES - 2>();
+            __syncwarp();
+            const unsigned char *st = ring + stage * S::STAGE;
+            const int q = ws * P.xq + kk - c0;
+            uint4 b[NT][2];
+            float xs[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const uint4 *src = (const uint4 *)(xf + ((size_t)(q * NT + n) * x_lanes + lane) * 8);
+                b[n][0] = b[n][1] = make_uint4(0, 0, 0, 0);
+                if (lane < x_lanes) b[n][0] = src[0], b[n][1] = src[1];
+                xs[n] = xscale[q * (NT * 4) + n * 4 + j];   // of the row whose sums this lane gets
+            }
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                const uint4 w = *(const uint4 *)(st + t * 512 + lane * 16);
+                float acc[NT][4];
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const uint32_t *sz = (const uint32_t *)(st + T * 512 + t * S::SZ + (G32 ? hf * 64 : 0));
+                    const __half2 s0 = u_h2(sz[g]), s1 = u_h2(sz[g + 8]);
+                    const __half2 sub = __float2half2_rn(960.0f);
+                    const __half2 z0 = __high2half2(s0), z1 = __high2half2(s1);
+                    uint32_t a0[4], a1[4];
+                    dequant8(hf ? w.y : w.x, z0, __hsub2(sub, z0), a0);   // 960 - (1024 + z) = -(64 + z)
+                    dequant8(hf ? w.w : w.z, z1, __hsub2(sub, z1), a1);
+                    if (G32 || hf == 0)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma_f16(acc[n], a0[0], a1[0], a0[1], a1[1], b[n][hf].x, b[n][hf].y);
+                        mma_f16(acc[n], a0[2], a1[2], a0[3], a1[3], b[n][hf].z, b[n][hf].w);
+                    }
+                    if (G32 || hf == 1)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            total[t][n][0] = fmaf(__low2float(s0) * xs[n], acc[n][0] + acc[n][1], total[t][n][0]);
+                            total[t][n][1] = fmaf(__low2float(s1) * xs[n], acc[n][2] + acc[n][3], total[t][n][1]);
+                        }
+                }
+            }
+            __syncwarp();
+            request(k0 + kk + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
+        }
+    }
+    // ---- slices of the CTA, then of the cluster, pairwise ----
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) sums[warp * S::SUMS + ((t * NT + n) * 2 + e) * 32 + lane] = total[t][n][e];
+    __syncthreads();
+    if (C > 1) {
+        mx::cluster_wait();
+        for (int i = tid; i < tg * S::SUMS; i += W4_THREADS) {
+            const int gi = i / S::SUMS, e = i - gi * S::SUMS;
+            const float v = tree_sum(sums + gi * kw * S::SUMS + e, kw, S::SUMS);
+            const uint32_t dst = mx::cluster_map(mx::smem_u32(parts + rank * tg * S::SUMS + i), 0);
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(v) : "memory");
+        }
+        mx::cluster_sync();
+        if (rank != 0) return;
+    }
+    for (int i = tid; i < tg * S::SUMS; i += W4_THREADS) {
+        const int gi = i / S::SUMS, e = i - gi * S::SUMS, l = e & 31, hf = (e >> 5) & 1, n = (e >> 6) % NT, t = (e >> 6) / NT;
+        const float v = C > 1 ? tree_sum(parts + i, C, tg * S::SUMS) : tree_sum(sums + gi * kw * S::SUMS + e, kw, S::SUMS);
+        const int o = ((grp * tg + gi) * T + t) * W4_N + (l >> 2) + 8 * hf, r = n * 4 + (l & 3);
+        if (o < P.n_out && r < rows) {
+            float out = P.bias ? v + P.bias[o] : v;
+            if (P.add) out = P.add[(long long)(row0 + r) * P.add_stride + o] + out;
+            P.y[(long long)(row0 + r) * P.y_stride + o] = out;
+        }
+    }
+}
+
+template <int NT, int T, bool G32>
+int launch_int4(mx230_handle *h, cudaStream_t st, Int4Params P) {
+    using S = Int4Smem<NT, T, G32>;
+    const int tg = W4_WARPS / P.kw, C = P.ctas_k, n_slices = P.kw * C;
+    const int most = (P.k_tiles + n_slices - 1) / n_slices;
+    const int per_tile = P.kw * NT * (32 * (NT == 1 ? 8 * (P.n_rows < 4 ? P.n_rows : 4) : 32) + 16);
+    P.xq = W4_X_BYTES / per_tile;
+    if (P.xq > most) P.xq = most;
+    if (P.xq < 1) P.xq = 1;
+    const size_t sm = (size_t)S::RING + (size_t)(W4_WARPS + (C > 1 ? C * tg : 0)) * S::SUMS * 4 + (size_t)P.xq * per_tile;
+    MX_SMEM_ATTR_ONCE(h->device, (gemv_int4_kernel<NT, T, G32>), 227 * 1024);
+    const long long groups_n = (P.n_tiles + (long long)tg * T - 1) / ((long long)tg * T);
+    const dim3 grid((unsigned)(groups_n * C), (unsigned)((P.n_rows + 4 * NT - 1) / (4 * NT)));
+    MX_LAUNCH(h, st, MX230_K_GEMV_INT4, mx_launch(gemv_int4_kernel<NT, T, G32>, grid, W4_THREADS, sm, st, C, true, P));
+    return MX230_OK;
+}
+
+int check_shape(const char *who, int n_in, int n_out, int group) {
+    MX_REQUIRE(n_in > 0 && n_out > 0, MX230_ERR_INVALID_ARG, "%s: n_in %d, n_out %d", who, n_in, n_out);
+    MX_REQUIRE(group == 32 || (group > 0 && group % 64 == 0), MX230_ERR_UNSUPPORTED, "%s: groups of %d inputs (32, or a multiple of 64)", who, group);
+    return MX230_OK;
+}
+
+size_t codes_bytes(int n_in, int n_out) {
+    return (size_t)((n_out + (long long)W4_N - 1) / W4_N) * (size_t)((n_in + (long long)W4_K - 1) / W4_K) * 512;
+}
+
+}  // namespace
+
+extern "C" size_t mx230_int4_bytes(int n_in, int n_out, int group) {
+    if (n_in <= 0 || n_out <= 0 || group <= 0) return 0;
+    return codes_bytes(n_in, n_out) + (size_t)((n_out + (long long)W4_N - 1) / W4_N) * (size_t)((n_in + (long long)group - 1) / group) * 64;
+}
+
+extern "C" int mx230_pack_int4(mx230_handle *h, void *stream, void *packed, const uint8_t *codes, const void *scales,
+                               const uint8_t *zeros, int n_in, int n_out, int group) {
+    MX_REQUIRE(h && packed && codes && scales, MX230_ERR_INVALID_ARG, "pack_int4: null argument");
+    int rc = check_shape("pack_int4", n_in, n_out, group);
+    if (rc) return rc;
+    MX_REQUIRE(((uintptr_t)packed & 15) == 0 && ((uintptr_t)scales & 1) == 0, MX230_ERR_INVALID_ARG, "pack_int4: misaligned pointer");
+    mx230_device_guard guard(h->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    const int n_tiles = (int)((n_out + (long long)W4_N - 1) / W4_N), k_tiles = (int)((n_in + (long long)W4_K - 1) / W4_K);
+    const int groups = (int)((n_in + (long long)group - 1) / group);
+    const long long work = (long long)n_tiles * k_tiles * 32 + (long long)n_tiles * groups * 16;
+    const long long blocks = (work + 255) / 256, most = 64ll * h->sm_count;
+    MX_LAUNCH(h, st, MX230_K_PACK_INT4, (pack_int4_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(
+        (uint4 *)packed, (uint32_t *)((char *)packed + codes_bytes(n_in, n_out)), codes, (const __half *)scales, zeros, n_in, n_out, group,
+        n_tiles, k_tiles, groups)));
+    return MX230_OK;
+}
+
+extern "C" int mx230_gemv_int4(mx230_handle *h, void *stream, float *y, const float *x, const void *packed, const float *bias,
+                               const float *add, int n_rows, int n_in, int n_out, int group, long long x_stride,
+                               long long y_stride, long long add_stride) {
+    MX_REQUIRE(h, MX230_ERR_INVALID_ARG, "gemv_int4: null handle");
+    int rc = check_shape("gemv_int4", n_in, n_out, group);
+    if (rc) return rc;
+    MX_REQUIRE(n_rows >= 0, MX230_ERR_INVALID_ARG, "gemv_int4: %d rows", n_rows);
+    if (n_rows == 0) return MX230_OK;
+    MX_REQUIRE(y && x && packed, MX230_ERR_INVALID_ARG, "gemv_int4: null argument");
+    MX_REQUIRE(n_rows < 2 || (x_stride >= 0 && y_stride >= n_out && (add == nullptr || add_stride >= 0)), MX230_ERR_INVALID_ARG,
+               "gemv_int4: rows of y share memory, or a stride is negative (x %lld, y %lld, add %lld)", x_stride, y_stride, add_stride);
+    MX_REQUIRE(((uintptr_t)packed & 15) == 0 && (((uintptr_t)x | (uintptr_t)y | (uintptr_t)bias | (uintptr_t)add) & 3) == 0, MX230_ERR_INVALID_ARG,
+               "gemv_int4: misaligned pointer");
+    MX_REQUIRE(add != y || n_rows < 2 || add_stride == y_stride, MX230_ERR_INVALID_ARG, "gemv_int4: add is y, with another stride");
+    MX_REQUIRE(n_rows <= 65535 * 4, MX230_ERR_UNSUPPORTED, "gemv_int4: %d rows", n_rows);
+    Int4Params P{};
+    P.y = y, P.x = x, P.bias = bias, P.add = add;
+    P.codes = (const uint4 *)packed, P.sz = (const uint32_t *)((const char *)packed + codes_bytes(n_in, n_out));
+    P.n_rows = n_rows, P.n_in = n_in, P.n_out = n_out, P.group = group;
+    P.groups = (int)((n_in + (long long)group - 1) / group);
+    P.n_tiles = (int)((n_out + (long long)W4_N - 1) / W4_N), P.k_tiles = (int)((n_in + (long long)W4_K - 1) / W4_K);
+    P.x_stride = x_stride, P.y_stride = y_stride, P.add_stride = add_stride;
+    P.x_vec = ((uintptr_t)x & 15) == 0 && (n_rows < 2 || x_stride % 4 == 0);
+    // Slices of the inputs: enough warps for eight per SM, as far as there are tiles.  This fixes the order of the sums.
+    int n_slices = 1;
+    while (n_slices < W4_WARPS * W4_CLUSTER && 2 * n_slices <= P.k_tiles && (long long)P.n_tiles * n_slices < 8ll * h->sm_count) n_slices *= 2;
+    P.kw = n_slices < W4_WARPS ? n_slices : W4_WARPS;
+    P.ctas_k = n_slices / P.kw;
+    mx230_device_guard guard(h->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool g32 = group == 32;
+    if (n_rows <= 4) return g32 ? launch_int4<1, 1, true>(h, st, P) : launch_int4<1, 1, false>(h, st, P);
+    return g32 ? launch_int4<2, 1, true>(h, st, P) : launch_int4<2, 1, false>(h, st, P);
+}

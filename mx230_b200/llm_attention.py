@@ -7,9 +7,12 @@ Tensors are torch CUDA tensors; nothing here synchronises or allocates on the st
 """
 from __future__ import annotations
 
+import ctypes as C
+
 import torch
 
-from ._lib import addr, check, lib, ptr
+from . import _lib
+from ._lib import addr, check, lib, ptr, require
 from .common import Handle, stream_ptr
 
 KV_BLOCK = 16  # 03-llm-engine/src/gpu.rs:209
@@ -79,6 +82,54 @@ def rope_batch(h: Handle, qkv, pos0, n_tok, n_head, n_kv_head, head_dim, stride,
 def rope_seqpos(h: Handle, qkv, pos, n_seq, n_head, n_kv_head, head_dim, stride, theta, stream=None):
     check(lib().mx230_rope_seqpos(h._h, stream_ptr(stream), addr(qkv), addr(pos), n_seq, n_head,
                                   n_kv_head, head_dim, stride, theta))
+
+
+# ---------------------------------------------------------------- rotary positions beyond the reference's forms
+_DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_SCALINGS = {"linear": (1, ()), "ntk": (2, ()), "wavelength": (3, ("low", "high", "length")), "yarn": (4, ("slow", "fast", "length"))}
+
+
+def on_device(h: Handle, what: str, t, dtype=None):
+    """A CUDA tensor of the handle's device, and of `dtype`."""
+    require(isinstance(t, torch.Tensor) and t.is_cuda and t.device.index == h.device, f"{what}: not a tensor of device {h.device}")
+    require(dtype is None or t.dtype == dtype, f"{what}: {t.dtype}, not {dtype}")
+
+
+class Rotary:
+    """The frequencies of `rotary`, made once: theta^(-2i / rot_dim) for pair i of the first `rot_dim` values of a head.
+    `scaling`: None, or how they are stretched for contexts longer than the trained one, as a dict with "kind" and "factor":
+    "linear", "ntk", "wavelength" (with "low", "high", "length") or "yarn" (with "slow", "fast", "length"); the formulas stand
+    in include/mx230_attn.h at MX230_ROTARY_*.  `interleaved`: pairs (2i, 2i + 1) instead of (i, i + rot_dim / 2)."""
+
+    def __init__(self, rot_dim: int, theta: float, scaling: dict | None = None, interleaved: bool = False, device="cuda"):
+        kind, names = (0, ()) if scaling is None else _SCALINGS.get(scaling.get("kind"), (None, ()))
+        require(kind is not None, f"Rotary: scaling {scaling!r}")
+        given = {} if scaling is None else {k: v for k, v in scaling.items() if k != "kind"}
+        require(set(given) == ({"factor", *names} if kind else set()), f"Rotary: scaling {scaling!r} needs factor {' '.join(names)}")
+        low, high, length = [given[n] for n in names] or (0.0, 0.0, 0)
+        table, factor = (C.c_uint64 * max(1, rot_dim // 2))(), C.c_float()
+        check(lib().mx230_rotary_table(table, C.byref(factor), rot_dim, theta, kind, given.get("factor", 1.0), low, high, length))
+        self.rot_dim, self.interleaved, self.factor = rot_dim, interleaved, factor.value
+        # (torch has no arithmetic on unsigned 64-bit words; only the bits matter)
+        self.turns = torch.frombuffer(table, dtype=torch.int64).to(device)
+
+
+def rotary(h: Handle, out, x, pos, plan: Rotary, inverse=False, stream=None):
+    """Rotates the first plan.rot_dim values of every head of x [n_rows][n_head][head_dim] (fp32, fp16 or bf16; any strides between
+    rows and heads) into `out` of the same shape, which may be x.  `pos`: an int32 tensor [n_rows], or the first row's position.
+    `inverse` turns back; it takes the gradient of `out` to that of x."""
+    require(x.dim() == 3 and out.shape == x.shape, f"rotary: x {tuple(x.shape)}, out {tuple(out.shape)}")
+    require(x.dtype in _DTYPES, f"rotary: {x.dtype}")
+    on_device(h, "rotary: x", x), on_device(h, "rotary: out", out, x.dtype), on_device(h, "rotary: plan", plan.turns)
+    n, heads, dim = x.shape
+    require(dim == 1 or (x.stride(2) == 1 and out.stride(2) == 1), "rotary: the values of a head must be contiguous")
+    dyn = isinstance(pos, torch.Tensor)
+    if dyn:
+        on_device(h, "rotary: pos", pos, torch.int32)
+        require(pos.shape == (n,) and (n < 2 or pos.stride(0) == 1), f"rotary: positions {tuple(pos.shape)} for {n} rows")
+    check(lib().mx230_rotary(h._h, stream_ptr(stream, h.device), addr(out), addr(x), _DTYPES[x.dtype], addr(pos) if dyn else None,
+                             0 if dyn else pos, addr(plan.turns), plan.factor, n, heads, dim, plan.rot_dim, int(plan.interleaved),
+                             int(inverse), x.stride(0), x.stride(1), out.stride(0), out.stride(1)))
 
 
 # ---------------------------------------------------------------- fp32 KV write
@@ -384,6 +435,57 @@ def gemv_int8(h: Handle, y, x, w_packed, scales, b=None, accum=False, act_group=
     n_in, n_out = w_packed.shape[0] * 4, w_packed.shape[1]
     check(lib().mx230_gemv_int8(h._h, stream_ptr(stream), addr(y), addr(x), addr(w_packed), addr(scales), addr(b),
                                 n_in, n_out, int(accum), act_group))
+
+
+class Int4Weights:
+    """A matrix [n_in][n_out] of 4-bit weights in the layout of `gemv_int4` (made by `pack_int4`)."""
+
+    def __init__(self, packed, n_in: int, n_out: int, group: int):
+        self.packed, self.n_in, self.n_out, self.group = packed, n_in, n_out, group
+
+    def nbytes(self) -> int:
+        return self.packed.numel()
+
+
+def pack_int4(h: Handle, codes, scales, zeros=None, group: int | None = None, stream=None) -> Int4Weights:
+    """Lays out weights scale * (code - zero) once for `gemv_int4`: `codes` uint8 [n_in][n_out] (low four bits), `scales` fp16 and
+    `zeros` uint8 [groups][n_out] (None: 8).  A group is 32 inputs or a multiple of 64; `group` may be left out where the
+    number of groups determines it among the powers of two.  Allocates the result: not for the step path."""
+    require(codes.dim() == 2 and scales.dim() == 2 and scales.shape[1] == codes.shape[1], "pack_int4: codes [n_in][n_out], scales [groups][n_out]")
+    n_in, n_out = codes.shape
+    groups = scales.shape[0]
+    if group is None:
+        fits = [g for g in (32, 64, 128, 256, 512, 1024) if -(-n_in // g) == groups]
+        require(len(fits) == 1, f"pack_int4: {groups} groups of {n_in} inputs: give the group")
+        group = fits[0]
+    require(group > 0 and -(-n_in // group) == groups, f"pack_int4: {groups} groups of {group} for {n_in} inputs")
+    on_device(h, "pack_int4: codes", codes, torch.uint8), on_device(h, "pack_int4: scales", scales, torch.float16)
+    require(codes.is_contiguous() and scales.is_contiguous(), "pack_int4: codes and scales must be contiguous")
+    if zeros is not None:
+        on_device(h, "pack_int4: zeros", zeros, torch.uint8)
+        require(zeros.shape == scales.shape and zeros.is_contiguous(), "pack_int4: zeros must be contiguous, of the scales' shape")
+    packed = torch.empty(lib().mx230_int4_bytes(n_in, n_out, group), dtype=torch.uint8, device=codes.device)
+    check(lib().mx230_pack_int4(h._h, stream_ptr(stream, h.device), addr(packed), addr(codes), addr(scales), addr(zeros), n_in, n_out, group))
+    return Int4Weights(packed, n_in, n_out, group)
+
+
+def gemv_int4(h: Handle, y, x, w: Int4Weights, b=None, add=None, stream=None):
+    """y = x W + b + add over 4-bit weights: x [n_in] or [n_rows][n_in], y and add (which may be y: the residual row) with n_out.
+    A row's bits do not depend on the rows beside it."""
+    x2, y2 = (x, y) if x.dim() == 2 else (x[None], y[None])
+    a2 = add if add is None or add.dim() == 2 else add[None]
+    n = x2.shape[0]
+    require(x.dim() in (1, 2) and y.dim() == x.dim() and x2.shape[1] == w.n_in and y2.shape == (n, w.n_out),
+            f"gemv_int4: x {tuple(x.shape)}, y {tuple(y.shape)}, weights [{w.n_in}][{w.n_out}]")
+    require(a2 is None or a2.shape == y2.shape, "gemv_int4: add must have the shape of y")
+    for what, t in (("x", x2), ("y", y2), ("add", a2), ("bias", b)):
+        if t is not None:
+            on_device(h, "gemv_int4: " + what, t, torch.float32)
+            require(t.shape[-1] < 2 or t.stride(-1) == 1, f"gemv_int4: the values of a row of {what} must be contiguous")
+    on_device(h, "gemv_int4: weights", w.packed)
+    require(b is None or b.shape == (w.n_out,), "gemv_int4: bias must be [n_out]")
+    check(lib().mx230_gemv_int4(h._h, stream_ptr(stream, h.device), addr(y2), addr(x2), addr(w.packed), addr(b), addr(a2), n, w.n_in, w.n_out,
+                                w.group, x2.stride(0), y2.stride(0), 0 if a2 is None else a2.stride(0)))
 
 
 def qkv_rope_kvwrite(h: Handle, qkv, x, w, b, pos, c: KvCache, n_head, n_kv_head, theta, pg: Paging | None = None,

@@ -1,0 +1,206 @@
+"""Products with 4-bit weights against the same sums in 64 bits.
+
+Tolerance, against the sum of the products' magnitudes M = sum |x s (q - z)|.  Weights and both parts of x are exact in fp16; x is
+off by 2^-24 |x| (or 2^-40 of the largest of its 64).  The tensor core adds the 16 products of a step with at most 17 truncations
+of 2^-24 M: 2^-20 M with the steps of a tile.  A tile's sum times its scale rounds and is added: 2^-23 M a tile, for at most
+the tiles of a slice, and six pairwise sums.  Then the bias and what is added, half a step each.
+"""
+import math
+
+import pytest
+import torch
+
+from mx230_b200 import _lib
+from mx230_b200 import llm_attention as la
+
+pytestmark = pytest.mark.gpu
+
+
+def weights(n_in, n_out, group, zeros, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    groups = -(-n_in // group)
+    codes = torch.randint(0, 16, (n_in, n_out), device="cuda", generator=g, dtype=torch.uint8)
+    scales = ((0.5 + torch.rand(groups, n_out, device="cuda", generator=g)) * 0.01).half()
+    z = torch.randint(0, 16, (groups, n_out), device="cuda", generator=g, dtype=torch.uint8) if zeros else None
+    return codes, scales, z
+
+
+def dense(codes, scales, z, group):
+    at = torch.arange(codes.shape[0], device="cuda") // group
+    return (codes.double() - (8.0 if z is None else z.double()[at])) * scales.double()[at]
+
+
+def limit(x, w, want, *more):
+    m = x.double().abs() @ w.abs()
+    tiles = -(-w.shape[0] // 64)
+    # (2^-40 of the largest x of a tile against the tile's M: covered where the tile's largest product is in M; 1e-12 for the rest)
+    out = m * (2.0 ** -20 + (tiles + 8) * 2.0 ** -23) + want.abs() * 2.0 ** -23 + 1e-30
+    for t in more:
+        out = out + t.double().abs() * 2.0 ** -23
+    return out + x.double().abs().amax(1, keepdim=True) * w.abs().amax(0) * w.shape[0] * 2.0 ** -40
+
+
+def check(got, want, lim, what):
+    err = (got.double() - want).abs()
+    assert (err <= lim).all(), (what, float((err / lim).max()))
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128, 192])
+@pytest.mark.parametrize("n_in,n_out,rows", [(1, 1, 1), (33, 17, 3), (64, 16, 1), (896, 1152, 1), (896, 1152, 5), (1000, 77, 2), (4864, 896, 8),
+                                             (2047, 130, 4), (4160, 513, 11), (130, 40001, 7), (9000, 24, 16), (64, 5000, 33)])
+def test_matches_the_sums(handle, n_in, n_out, rows, group, zeros):
+    codes, scales, z = weights(n_in, n_out, group, zeros, n_in + n_out)
+    w = la.pack_int4(handle, codes, scales, z, group=group)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x, b, old = (torch.randn(*s, device="cuda", generator=g) for s in ((rows, n_in), (n_out,), (rows, n_out)))
+    d = dense(codes, scales, z, group)
+    want = x.double() @ d
+    y = torch.full((rows, n_out), math.nan, device="cuda")
+    la.gemv_int4(handle, y, x, w)
+    check(y, want, limit(x, d, want), "plain")
+    la.gemv_int4(handle, y, x, w, b, add=old)
+    want = want + b.double() + old.double()
+    check(y, want, limit(x, d, want, b, old), "bias and add")
+    acc = old.clone()
+    la.gemv_int4(handle, acc, x, w, b, add=acc)
+    assert torch.equal(acc, y), "added in place"
+
+
+@pytest.mark.parametrize("n_in,n_out,group", [(896, 1152, 32), (4864, 896, 64), (14336, 96, 128), (300, 3000, 64), (4096, 6000, 128)])
+def test_a_row_does_not_depend_on_the_others(handle, n_in, n_out, group):
+    codes, scales, z = weights(n_in, n_out, group, True, 5)
+    w = la.pack_int4(handle, codes, scales, z, group=group)
+    x = torch.randn(37, n_in, device="cuda", generator=torch.Generator(device="cuda").manual_seed(6))
+    alone = torch.empty(37, n_out, device="cuda")
+    for r in range(37):
+        la.gemv_int4(handle, alone[r], x[r], w)
+    for n in (2, 3, 4, 5, 7, 8, 9, 12, 16, 17, 37):
+        y = torch.empty(n, n_out, device="cuda")
+        la.gemv_int4(handle, y, x[:n], w)
+        assert torch.equal(y, alone[:n]), n
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1.0, 1e20])
+def test_ranges_of_x(handle, scale):
+    """Very small, very large and mixed rows: x is split relative to the largest of 64 values."""
+    n_in, n_out = 640, 200
+    codes, scales, z = weights(n_in, n_out, 64, True, 9)
+    w = la.pack_int4(handle, codes, scales, z)
+    d = dense(codes, scales, z, 64)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(6, n_in, device="cuda", generator=g) * scale
+    x[1] = 0.0
+    x[2, ::64] *= 1e6
+    x[3, 64:128] = 0.0
+    x[4] *= torch.exp2(torch.randint(-12, 12, (n_in,), device="cuda", generator=g).float())
+    x[5, 1:] = 0.0
+    y = torch.empty(6, n_out, device="cuda")
+    la.gemv_int4(handle, y, x, w)
+    want = x.double() @ d
+    check(y, want, limit(x, d, want), scale)
+    assert (y[1] == 0).all()
+
+
+def test_infinities_and_nan_stay_in_their_row(handle):
+    codes, scales, _ = weights(256, 64, 64, False, 2)
+    w = la.pack_int4(handle, codes, scales)
+    d = dense(codes, scales, None, 64)
+    x = torch.randn(7, 256, device="cuda")
+    clean = torch.empty(7, 64, device="cuda")
+    la.gemv_int4(handle, clean, x, w)
+    x[2, 70], x[4, 3], x[5, 255] = math.nan, math.inf, -math.inf
+    y = torch.empty(7, 64, device="cuda")
+    la.gemv_int4(handle, y, x, w)
+    assert torch.equal(y[[0, 1, 3, 6]], clean[[0, 1, 3, 6]])
+    assert torch.isnan(y[2]).all()
+    for r, k, v in ((4, 3, math.inf), (5, 255, -math.inf)):
+        want = v * d[k]   # NaN where the weight is 0
+        assert torch.equal(torch.isnan(want), torch.isnan(y[r])) and torch.equal(want[~torch.isnan(want)], y[r].double()[~torch.isnan(want)])
+
+
+def test_strides_and_what_lies_beside(handle):
+    n_in, n_out, rows = 200, 50, 6
+    codes, scales, z = weights(n_in, n_out, 64, True, 3)
+    w = la.pack_int4(handle, codes, scales, z)
+    d = dense(codes, scales, z, 64)
+    for off, wide in ((0, 208), (1, 203), (3, 211)):
+        store = torch.randn(rows * wide + 8, device="cuda")
+        x = store[off:off + rows * wide].view(rows, wide)[:, :n_in]
+        whole = torch.full((rows + 2, n_out + 7), 5.0, device="cuda")
+        y = whole[1:rows + 1, 3:3 + n_out]
+        add = torch.randn(rows, n_out + 1, device="cuda")[:, 1:]
+        la.gemv_int4(handle, y, x, w, add=add)
+        want = x.double() @ d + add.double()
+        check(y, want, limit(x, d, want, add), off)
+        inside = torch.zeros_like(whole, dtype=torch.bool)
+        inside[1:rows + 1, 3:3 + n_out] = True
+        assert (whole[~inside] == 5).all()
+    one = torch.randn(1, n_in, device="cuda")
+    y = torch.empty(4, n_out, device="cuda")
+    la.gemv_int4(handle, y, one.expand(4, n_in), w)
+    single = torch.empty(n_out, device="cuda")
+    la.gemv_int4(handle, single, one[0], w)
+    assert torch.equal(y, single.expand(4, n_out))
+
+
+def test_high_bits_of_codes_and_large_zeros(handle):
+    codes, scales, _ = weights(128, 32, 64, False, 4)
+    z = torch.full((2, 32), 255, dtype=torch.uint8, device="cuda")
+    x = torch.randn(2, 128, device="cuda")
+    a, b = torch.empty(2, 32, device="cuda"), torch.empty(2, 32, device="cuda")
+    la.gemv_int4(handle, a, x, la.pack_int4(handle, codes, scales, z))
+    la.gemv_int4(handle, b, x, la.pack_int4(handle, codes + 240, scales, z))
+    assert torch.equal(a, b)
+    d = dense(codes, scales, z, 64)
+    want = x.double() @ d
+    check(a, want, limit(x, d, want), "zeros of 255")
+
+
+def test_captured_replayed_and_on_another_stream(handle):
+    n_in, n_out = 4864, 896
+    codes, scales, z = weights(n_in, n_out, 64, True, 7)
+    w = la.pack_int4(handle, codes, scales, z)
+    x, y = torch.randn(3, n_in, device="cuda"), torch.zeros(3, n_out, device="cuda")
+    side = torch.cuda.Stream()
+    la.gemv_int4(handle, y, x, w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        la.gemv_int4(handle, y, x, w)
+        la.gemv_int4(handle, y, x, w, add=y)
+    for seed in (1, 2):
+        x.copy_(torch.randn(3, n_in, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = torch.empty_like(y)
+        la.gemv_int4(handle, want, x, w)
+        la.gemv_int4(handle, want, x, w, add=want)
+        assert torch.equal(want, y)
+    got = torch.zeros_like(y)
+    torch.cuda.synchronize()
+    la.gemv_int4(handle, got, x, w, stream=side)   # two at once
+    la.gemv_int4(handle, want, x, w)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_refusals(handle):
+    codes, scales, z = weights(256, 48, 64, True, 1)
+    w = la.pack_int4(handle, codes, scales, z)
+    x, y = torch.zeros(2, 256, device="cuda"), torch.zeros(2, 48, device="cuda")
+    la.gemv_int4(handle, y[:0], x[:0], w)
+    bad = [lambda: la.gemv_int4(handle, y, x[:, :255], w), lambda: la.gemv_int4(handle, y[:1], x, w), lambda: la.gemv_int4(handle, y, x.half(), w),
+           lambda: la.gemv_int4(handle, y.cpu(), x, w), lambda: la.gemv_int4(handle, y, x, w, torch.zeros(47, device="cuda")),
+           lambda: la.gemv_int4(handle, y, x, w, add=y[:1]), lambda: la.gemv_int4(handle, y[:1].expand(2, 48), x, w),
+           lambda: la.gemv_int4(handle, torch.zeros(48, 2, device="cuda").t(), x, w),
+           lambda: la.pack_int4(handle, codes, scales.float(), z), lambda: la.pack_int4(handle, codes, scales, z[:2]),
+           lambda: la.pack_int4(handle, codes, scales, z, group=128), lambda: la.pack_int4(handle, codes.t(), scales, z),
+           lambda: la.pack_int4(handle, codes[:60].contiguous(), scales[:1].contiguous())]   # 64 or 128 or more
+    for call in bad:
+        with pytest.raises(_lib.Mx230Error) as e:
+            call()
+        assert e.value.code == _lib.ERR_INVALID_ARG
+    with pytest.raises(_lib.Mx230Error) as e:
+        la.pack_int4(handle, codes, torch.zeros(6, 48, dtype=torch.float16, device="cuda"), group=48)
+    assert e.value.code == _lib.ERR_UNSUPPORTED

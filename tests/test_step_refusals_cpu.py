@@ -1,0 +1,70 @@
+"""What the C entry points beside the attention step refuse before they touch the device: calls with a handle that no device stands
+behind (all of these return before it is looked at), and the host-side table of rotary frequencies."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+from mx230_b200 import _lib
+
+
+@pytest.fixture(scope="module")
+def L(lib_built):
+    return _lib.lib()
+
+
+FAKE = C.create_string_buffer(1 << 16)   # a handle of zeros
+H = C.addressof(FAKE)
+P = 1 << 20                              # an address that is never used, 16-byte aligned
+
+
+def test_rotary_refuses(L):
+    ok = dict(h=H, st=None, out=P, x=P + 4096, dt=0, pos=None, pos0=0, turns=P, factor=1.0, rows=4, heads=2, dim=64, rot=64, inter=0, inv=0,
+              xr=128, xh=64, outr=128, outh=64)
+    cases = [dict(h=None), dict(out=None), dict(x=None), dict(turns=None), dict(dt=3), dict(dt=-1), dict(rows=-1), dict(heads=-1), dict(rot=63),
+             dict(rot=0), dict(rot=66), dict(dim=0), dict(xr=-1), dict(outh=-64), dict(outr=0), dict(outh=0), dict(outr=64), dict(outh=32),
+             dict(outr=100, outh=64), dict(out=P + 4096, outr=256), dict(x=P + 4097), dict(out=P + 2), dict(turns=P + 4), dict(pos=P + 2)]
+    for c in cases:
+        assert L.mx230_rotary(*{**ok, **c}.values()) == _lib.ERR_INVALID_ARG, c
+    assert L.mx230_rotary(*{**ok, "dim": 8192, "rot": 8192, "outh": 8192, "outr": 16384}.values()) == _lib.ERR_UNSUPPORTED
+    assert L.mx230_rotary(*{**ok, "rows": 0}.values()) == 0 and L.mx230_rotary(*{**ok, "heads": 0}.values()) == 0
+
+
+def test_rotary_table(L):
+    t, f = (C.c_uint64 * 32)(), C.c_float()
+    table = lambda *a: L.mx230_rotary_table(t, C.byref(f), *a)  # noqa: E731
+    for bad in [(63, 1e4, 0, 1.0, 0.0, 0.0, 0), (0, 1e4, 0, 1.0, 0.0, 0.0, 0), (64, 0.0, 0, 1.0, 0.0, 0.0, 0), (64, math.inf, 0, 1.0, 0.0, 0.0, 0),
+                (64, math.nan, 0, 1.0, 0.0, 0.0, 0), (64, 1e4, 5, 1.0, 0.0, 0.0, 0), (64, 1e4, 1, 0.0, 0.0, 0.0, 0), (64, 1e4, 2, math.nan, 0.0, 0.0, 0),
+                (64, 1e4, 3, 8.0, 4.0, 1.0, 8192), (64, 1e4, 3, 8.0, 1.0, 4.0, 0), (64, 1e4, 4, 8.0, 1.0, 1.0, 8192), (64, 1.0, 4, 8.0, 1.0, 32.0, 8192)]:
+        assert table(*bad) == _lib.ERR_INVALID_ARG, bad
+    assert L.mx230_rotary_table(None, C.byref(f), 64, 1e4, 0, 1.0, 0.0, 0.0, 0) == _lib.ERR_INVALID_ARG
+    assert table(64, 1e4, 0, 1.0, 0.0, 0.0, 0) == 0 and f.value == 1.0
+    turns = np.array(t, np.uint64).astype(np.float64) / 2.0 ** 64
+    want = 1e4 ** (-np.arange(32) / 32) / (2 * np.pi)
+    # a power and a quotient in 64 bits on either side, and half a unit of 2^-64 turns: at 2e-5 turns that is 2^-49 of the value
+    assert (np.abs(turns - want) <= 4 * 2.0 ** -53 * want + 2.0 ** -65).all()
+    assert table(64, 0.001, 0, 1.0, 0.0, 0.0, 0) == 0   # frequencies above a turn a position: the remainder
+    turns = np.array(t, np.uint64).astype(np.float64) / 2.0 ** 64
+    want = np.mod(0.001 ** (-np.arange(32) / 32) / (2 * np.pi), 1.0)
+    assert np.abs(turns - want).max() < 1e-12
+    assert table(64, 1e4, 4, 16.0, 1.0, 32.0, 4096) == 0 and abs(f.value - (0.1 * math.log(16) + 1)) < 1e-7
+
+
+def test_int4_refuses(L):
+    ok = dict(h=H, st=None, y=P, x=P, packed=P, bias=None, add=None, rows=4, n_in=256, n_out=64, group=64, xs=256, ys=64, adds=0)
+    cases = [dict(h=None), dict(y=None), dict(x=None), dict(packed=None), dict(rows=-1), dict(n_in=0), dict(n_out=0), dict(n_in=-5), dict(xs=-1),
+             dict(ys=63), dict(ys=-64), dict(add=P + 64, adds=-1), dict(add=P, adds=0), dict(packed=P + 8), dict(y=P + 2), dict(x=P + 1), dict(bias=P + 2)]
+    for c in cases:
+        assert L.mx230_gemv_int4(*{**ok, **c}.values()) == _lib.ERR_INVALID_ARG, c
+    for g in (0, -64, 16, 48, 96, 31):
+        assert L.mx230_gemv_int4(*{**ok, "group": g}.values()) == _lib.ERR_UNSUPPORTED, g
+    assert L.mx230_gemv_int4(*{**ok, "rows": 1 << 30}.values()) == _lib.ERR_UNSUPPORTED
+    assert L.mx230_gemv_int4(*{**ok, "rows": 0}.values()) == 0
+    pk = dict(h=H, st=None, packed=P, codes=P, scales=P, zeros=None, n_in=256, n_out=64, group=64)
+    for c in [dict(h=None), dict(packed=None), dict(codes=None), dict(scales=None), dict(packed=P + 4), dict(scales=P + 1), dict(n_in=0), dict(n_out=-1)]:
+        assert L.mx230_pack_int4(*{**pk, **c}.values()) == _lib.ERR_INVALID_ARG, c
+    assert L.mx230_pack_int4(*{**pk, "group": 40}.values()) == _lib.ERR_UNSUPPORTED
+    # 16 x 64 tiles of 512 bytes, 64 bytes per 16 outputs and group
+    assert L.mx230_int4_bytes(256, 64, 64) == 4 * 4 * 512 + 4 * 4 * 64 and L.mx230_int4_bytes(65, 17, 32) == 2 * 2 * 512 + 2 * 3 * 64
+    assert L.mx230_int4_bytes(0, 64, 64) == 0 and L.mx230_int4_bytes(1 << 17, 1 << 19, 64) == (1 << 15) * (1 << 11) * 576
