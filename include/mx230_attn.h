@@ -101,7 +101,8 @@ enum {
     MX230_K_ROTARY = 15,
     MX230_K_GEMV_INT4 = 16,
     MX230_K_PACK_INT4 = 17,
-    MX230_K_COUNT = 18
+    MX230_K_SAMPLE = 18,
+    MX230_K_COUNT = 19
 };
 
 /* element types, where an entry point takes several */
@@ -546,6 +547,24 @@ int mx230_qkv_rope_kvwrite(mx230_handle *h, void *stream, float *qkv, const floa
                            int pos, const int *pos_ptr, int n_head, int n_kv_head, int head_dim,
                            float theta, float *kcache, float *vcache, int8_t *kq, int8_t *vq, float *ks,
                            float *vs, float *kb, float *vb, const int *bt, int bs);
+
+/* ---- the next token of each row of logits, from given random numbers ----------------------------
+ * logits [n_rows][vocab] of `dtype` (MX230_F32, _F16, _BF16), rows row_stride elements apart; u [n_rows] in [0, 1).  Each setting is an
+ * array with a value per row, or, where that is null, one value for all.  With m the row's largest logit:
+ *   weight   w_i = exp((l_i - m) / temperature), as a whole number of 2^-40 (nearest; less than half of it is none)
+ *   order    larger logits first, of equal ones the lower index
+ *   K        the first top_k of that order (all where top_k <= 0)
+ *   P        the shortest prefix of K with at least top_p times K's weight (K where top_p >= 1 or NaN, one entry where <= 0)
+ *   M        the entries with w_i >= min_p (all where min_p <= 0 or NaN; above 1 it is 1)
+ *   token    the first of the order whose running weight, its own included, exceeds u times that of P and M together
+ *   prob     (may be null) its share of that weight
+ * temperature <= 0 or NaN: the first of the order, prob 1; above 1e30 it is 1e30.  -inf and NaN logits are masked, +inf counts as
+ * the largest finite number; a row with nothing left gets token -1, prob 0.  u below 0 or NaN is 0; at 1 and above the last kept
+ * entry is drawn.  Sums are over whole numbers: a row gives the same token in any batch.  At most 360192 logits a row.
+ * No workspace. */
+int mx230_sample(mx230_handle *h, void *stream, int *token, float *prob, const void *logits, int dtype, int n_rows, int vocab,
+                 long long row_stride, const float *u, float temperature, const float *temperatures, int top_k,
+                 const int *top_ks, float top_p, const float *top_ps, float min_p, const float *min_ps);
 
 /* ---- host side of paged attention: KV block pool with a block-granular prefix tree ----------
  * Paging and RadixCache, 03-llm-engine/src/gpu.rs:211-343,372-539; the request protocol is that

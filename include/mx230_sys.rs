@@ -328,6 +328,12 @@ extern "C" {
         kq: *mut i8, vq: *mut i8, ks: *mut f32, vs: *mut f32, kb: *mut f32, vb: *mut f32, bt: *const c_int,
         bs: c_int,
     ) -> c_int;
+    pub fn mx230_sample(
+        h: *mut Mx230Handle, stream: *mut c_void, token: *mut c_int, prob: *mut f32, logits: *const c_void,
+        dtype: c_int, n_rows: c_int, vocab: c_int, row_stride: c_longlong, u: *const f32, temperature: f32,
+        temperatures: *const f32, top_k: c_int, top_ks: *const c_int, top_p: f32, top_ps: *const f32, min_p: f32,
+        min_ps: *const f32,
+    ) -> c_int;
     pub fn mx230_kv_pool_create(
         out: *mut *mut Mx230KvPool, n_slots: c_int, block_size: c_int, prefix_cache: c_int,
     ) -> c_int;

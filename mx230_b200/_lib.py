@@ -20,7 +20,7 @@ Q8_SCORE_REF, Q8_SCORE_EXACT = 0, 1
 OPT_Q8_SCORE_MODE, OPT_DECODE_CHUNK, OPT_DECODE_TENSOR, OPT_BWD_TWO_PASS = 1, 2, 3, 4
 OPT_BWD_REUSE_STAGED, OPT_WAIT_LIMIT, OPT_TEST_DROP_TILE = 5, 6, 7
 F32, F16, BF16 = 0, 1, 2
-K_COUNT = 18
+K_COUNT = 19
 
 
 class Mx230Error(RuntimeError):

@@ -1,0 +1,584 @@
+// The next token of each row of logits, from given random numbers: temperature, top-k, top-p, min-p.
+//
+//   weight     w_i = exp((l_i - max l) / T), held as the whole number mass_i = round(2^40 w_i)   (masked: l = -inf or NaN, mass 0)
+//   order      larger logits first, among equal ones the lower index
+//   top-k      K = the first k entries of that order
+//   top-p      P = the shortest prefix of K whose mass is at least p times K's
+//   min-p      M = the entries with w_i >= m, a prefix as well
+//   token      the first entry of the order whose running mass, its own included, exceeds u times the mass of P and M's intersection
+//
+// Sums are over whole numbers, so they do not depend on their order, and the same row gives the same token on any grid.  What has
+// to be found is always "the first entry of the order whose running count or mass exceeds t"; three of them at most, each
+// target known from the one before (the intersection of two prefixes has the smaller of their masses).
+//
+// Bounded by HBM: the logits are read once.  A cluster of up to eight CTAs holds a row in its shared memory.  A histogram over 1024
+// equal intervals of max - l, as far as weights are not 0 (28.5 T), in counts and masses says which interval holds an entry that is
+// sought; the entries of that interval alone are collected, sorted and summed.  Where an interval has more entries
+// than the list, a histogram over the range of their (value, index) takes its place, as often as it takes.
+// Weights take eleven fp64 instructions an entry (a table of 256 steps of 2^(1/256) and a polynomial of degree four, below
+// 1e-15); rows with a small k take them for the entries of the list only.
+#include <cuda_fp16.h>
+#include <float.h>
+#include <math.h>
+
+#include "common.cuh"
+
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr int SM_THREADS = 512;
+constexpr int SM_WARPS = SM_THREADS / 32;
+constexpr int SM_BINS = 1024;
+constexpr int SM_LIST = 1024;        // entries that are sorted, most
+constexpr int SM_CLUSTER = 8;
+constexpr int SM_MAX_DATA = 45056;   // logits that a CTA can hold
+constexpr double SM_MASS = 1099511627776.0;   // 2^40
+
+struct SampleParams {
+    int *token;
+    float *prob;
+    const void *logits;
+    long long row_stride;
+    int vocab, ctas, idx_bits;
+    int cap;                 // logits of a CTA's share, at most
+    const float *u;
+    float temperature, top_p, min_p;
+    int top_k;
+    const float *temperatures, *top_ps, *min_ps;
+    const int *top_ks;
+};
+
+// What the first CTA tells the others (whole words, so that it can be copied as such).
+struct Window {
+    int kind;                // 0: intervals b0 .. b1 of the histogram over max - l; 1: entries lo .. hi; 2: done
+    int b0, b1;
+    int count;               // entries in it
+    u64 lo, hi;
+    u64 base_count, base_mass;   // of the entries in front of it
+};
+
+struct alignas(16) Shared {
+    unsigned cnt[SM_BINS], lo[SM_BINS], hi[SM_BINS];   // this CTA's histogram: counts, masses in two words
+    // first CTA: running counts and masses over the first histogram's intervals
+    u64 run_mass[SM_BINS];
+    unsigned run_cnt[SM_BINS];
+    // a list's entries of this CTA, and of all (first CTA); running masses of the sorted list; a later histogram's running sums
+    u64 mine[SM_LIST], all[SM_LIST];
+    double table[256];
+    u64 scan[SM_WARPS];
+    u64 slot_a[SM_CLUSTER], slot_b[SM_CLUSTER];        // a word of each CTA
+    float warp_a[SM_WARPS], warp_b[SM_WARPS];
+    Window w[2];             // the one in force and the next: a CTA may still look at one while the first CTA writes the other
+    u64 found_a, found_b, found_c;
+    unsigned n_mine, n_all;
+};
+
+__device__ __forceinline__ void cluster_sync() {   // (by whole warps)
+    __syncwarp();
+    mx::cluster_sync();
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ void st_cluster(uint32_t addr, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory"); }
+__device__ __forceinline__ uint32_t ld_cluster32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t add_cluster(uint32_t addr, uint32_t v) {
+    uint32_t old;
+    asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(v) : "memory");
+    return old;
+}
+
+template <typename T> __device__ __forceinline__ float logit(T v);
+template <> __device__ __forceinline__ float logit(float v) { return v; }
+template <> __device__ __forceinline__ float logit(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float logit(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// as it is kept: NaN is masked, infinity the largest number, -0 is 0
+__device__ __forceinline__ float kept_logit(float l) { return l == l ? fminf(l, FLT_MAX) + 0.0f : -INFINITY; }
+
+// whole numbers in the order of the floats, and back
+__device__ __forceinline__ uint32_t order_key(float l) {
+    const uint32_t b = __float_as_uint(l);
+    return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_float(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k); }
+
+// 2^(j / 256), j of a table, times the polynomial of 2^r for |r| <= 1/512
+__device__ __forceinline__ double weight(float l, float m, double log2e_t, const double *table) {
+    if (l == m) return 1.0;
+    const double x = ((double)l - (double)m) * log2e_t;
+    if (!(x > -42.0)) return 0.0;
+    const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's last bits are the rounded whole number
+    const double t = fma(x, 256.0, magic);
+    const int n = __double2loint(t);
+    const double r = fma(t - magic, -0.00390625, x);
+    // ln 2^i / i!
+    double p = fma(r, 9.618129107628477e-3, 5.550410866482158e-2);
+    p = fma(r, p, 2.402265069591007e-1);
+    p = fma(r, p, 6.931471805599453e-1);
+    p = fma(r, p, 1.0);
+    p *= table[n & 255];
+    return __hiloint2double(__double2hiint(p) + ((n >> 8) << 20), __double2loint(p));
+}
+__device__ __forceinline__ u64 to_mass(double w) {   // (ties cannot be: no weight but 1 is a binary fraction)
+    return (u64)__double_as_longlong(fma(w, SM_MASS, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+}
+
+// interval of max - l; SM_BINS and above: no weight.  Monotone in l: a difference, a product and a sum, each rounded.
+__device__ __forceinline__ int interval(float l, float m, float scale) {
+    if (l == -INFINITY) return SM_BINS;
+    return (int)(__float_as_uint(fminf((m - l) * scale, (float)SM_BINS) + 8388608.0f) & 0x7FFFFFu);
+}
+
+// inclusive sums over the block, in the order of the threads
+__device__ __forceinline__ u64 block_scan(u64 v, u64 *scratch) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 up = __shfl_up_sync(0xFFFFFFFFu, v, o);
+        if (lane >= o) v += up;
+    }
+    __syncthreads();
+    if (lane == 31) scratch[warp] = v;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) v += scratch[w];
+    return v;
+}
+
+// running sums of n values (n <= 2 * SM_THREADS), two a thread, into out
+template <typename In, typename Out>
+__device__ __forceinline__ void running_sums(const In *in, Out *out, int n, u64 *scratch) {
+    const int i = 2 * threadIdx.x;
+    const u64 a = i < n ? in[i] : 0, b = i + 1 < n ? in[i + 1] : 0;
+    const u64 s = block_scan(a + b, scratch);   // (its barriers stand between the reads and the writes)
+    if (i < n) out[i] = (Out)(s - b);
+    if (i + 1 < n) out[i + 1] = (Out)s;
+    __syncthreads();
+}
+
+// first index whose running sum exceeds t, n where none does; to be read behind the barrier
+template <typename R>
+__device__ __forceinline__ int first_over(const R *run, int n, u64 t, u64 *found) {
+    __syncthreads();
+    if (threadIdx.x == 0) *found = (u64)n;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += SM_THREADS)
+        if ((u64)run[i] > t && (i == 0 || (u64)run[i - 1] <= t)) *found = (u64)i;
+    __syncthreads();
+    return (int)*found;
+}
+
+// sorts n2 (a power of two, at least 2) entries, largest first.  A warp's pairs of strides below 64 lie in 64 entries of its own.
+__device__ __forceinline__ void sort_down(u64 *v, int n2) {
+    for (int k = 2; k <= n2; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            if (j >= 32) __syncthreads();
+            else __syncwarp();
+            for (int t = threadIdx.x; t < n2 / 2; t += SM_THREADS) {
+                const int i = 2 * (t & ~(j - 1)) | (t & (j - 1)), o = i | j;
+                const u64 a = v[i], b = v[o];
+                if ((a < b) == ((i & k) == 0)) v[i] = b, v[o] = a;
+            }
+            if (j >= 32) __syncthreads();
+        }
+    __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    Shared &S = *(Shared *)smem;
+    float *data = (float *)(smem + sizeof(Shared));
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int C = P.ctas, row = blockIdx.x / C, rank = blockIdx.x - row * C;
+    const bool first_cta = rank == 0;
+    mx::pdl_trigger();
+    if (tid < 256) S.table[tid] = exp2((double)tid / 256.0);
+    mx::pdl_wait();
+
+    float T_ = P.temperatures ? P.temperatures[row] : P.temperature;
+    int k = P.top_ks ? P.top_ks[row] : P.top_k;
+    const float p = P.top_ps ? P.top_ps[row] : P.top_p, min_p = P.min_ps ? P.min_ps[row] : P.min_p;
+    float u = P.u[row];
+    u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
+
+    // ---- this CTA's share of the row: whole 16-byte pieces ----
+    constexpr int VE = 16 / (int)sizeof(T);
+    const T *src = (const T *)P.logits + (long long)row * P.row_stride;
+    const int shift = (int)(((uintptr_t)src / sizeof(T)) % VE);   // elements between the last 16-byte boundary and the row
+    const int pieces = (P.vocab + shift + VE - 1) / VE;
+    const int v0 = (int)((long long)pieces * rank / C), v1 = (int)((long long)pieces * (rank + 1) / C);
+    const int n = (v1 - v0) * VE, idx0 = v0 * VE - shift;         // data[i] is logit idx0 + i
+    float hi = -INFINITY, lo = INFINITY;
+    for (int v = tid; v < v1 - v0; v += SM_THREADS) {
+        const int at = idx0 + v * VE;
+        float f[VE];
+        if (at >= 0 && at + VE <= P.vocab) {
+            const uint4 raw = *(const uint4 *)(src + at);
+            const T *e = (const T *)&raw;
+#pragma unroll
+            for (int i = 0; i < VE; ++i) f[i] = kept_logit(logit(e[i]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) f[i] = at + i >= 0 && at + i < P.vocab ? kept_logit(logit(src[at + i])) : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < VE; i += 4) *(float4 *)(data + v * VE + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+            hi = fmaxf(hi, f[i]);
+            if (f[i] != -INFINITY) lo = fminf(lo, f[i]);
+        }
+    }
+    hi = mx::warp_max(hi), lo = mx::warp_min(lo);
+    if (lane == 0) S.warp_a[warp] = hi, S.warp_b[warp] = lo;
+    cluster_sync();   // (every CTA of the cluster runs)
+    if (tid < C) {
+        for (int w = 0; w < SM_WARPS; ++w) hi = fmaxf(hi, S.warp_a[w]), lo = fminf(lo, S.warp_b[w]);
+        st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_a[rank]), tid), (u64)__float_as_uint(hi) << 32 | __float_as_uint(lo));
+    }
+    cluster_sync();
+    float m = -INFINITY, least = INFINITY;
+    for (int c = 0; c < C; ++c) m = fmaxf(m, __uint_as_float((uint32_t)(S.slot_a[c] >> 32))), least = fminf(least, __uint_as_float((uint32_t)S.slot_a[c]));
+    if (m == -INFINITY) {   // nothing is left to choose from
+        if (first_cta && tid == 0) {
+            P.token[row] = -1;
+            if (P.prob) P.prob[row] = 0.0f;
+        }
+        return;
+    }
+    // ---- the most likely one alone ----
+    if (!(T_ > 0.0f) || k == 1 || p <= 0.0f) {
+        if (tid == 0) S.n_mine = 0xFFFFFFFFu;
+        __syncthreads();
+        unsigned best = 0xFFFFFFFFu;
+        for (int i = tid; i < n; i += SM_THREADS)
+            if (data[i] == m) best = min(best, (unsigned)(idx0 + i));
+        if (best != 0xFFFFFFFFu) atomicMin(&S.n_mine, best);
+        __syncthreads();
+        if (tid == 0) st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_b[rank]), 0), (u64)S.n_mine);
+        cluster_sync();
+        if (first_cta && tid == 0) {
+            u64 b = 0xFFFFFFFFu;
+            for (int c = 0; c < C; ++c) b = min(b, S.slot_b[c]);
+            P.token[row] = (int)b;
+            if (P.prob) P.prob[row] = 1.0f;
+        }
+        return;
+    }
+    T_ = fminf(T_, 1e30f);   // (28.7 T stays finite)
+    if (k <= 0 || k >= P.vocab) k = 0;
+    const double log2e_t = 1.4426950408889634 / (double)T_;
+    // intervals over what has weight (2^-41 and more: 28.42 T) and what there is
+    const float range = fminf(28.7f * T_, m - least);
+    const float scale = range > 0.0f ? fminf((float)(SM_BINS - 1) / range, FLT_MAX) : 0.0f;
+    const double min_w = min_p > 0.0f ? (double)fminf(min_p, 1.0f) : 0.0;
+
+    auto entry = [&](int i) { return (u64)order_key(data[i]) << P.idx_bits | (((1u << P.idx_bits) - 1) - (unsigned)(idx0 + i)); };
+    auto entry_logit = [&](u64 e) { return key_float((uint32_t)(e >> P.idx_bits)); };
+    auto add_to = [&](int b, u64 mass) {   // a 64-bit sum by two words
+        const unsigned l = (unsigned)mass, old = atomicAdd(&S.lo[b], l);
+        const unsigned h = (unsigned)(mass >> 32) + (old + l < old);
+        if (h) atomicAdd(&S.hi[b], h);
+    };
+    auto clear = [&]() {
+        for (int b = tid; b < SM_BINS; b += SM_THREADS) S.cnt[b] = S.lo[b] = S.hi[b] = 0;
+        __syncthreads();
+    };
+    // the CTAs' histograms, added up by shares of the intervals into the first CTA's arrays, there as running sums
+    auto merge = [&](unsigned *to_cnt, u64 *to_mass) {
+        cluster_sync();
+        const int b0 = SM_BINS * rank / C, b1 = SM_BINS * (rank + 1) / C;
+        for (int b = b0 + tid; b < b1; b += SM_THREADS) {
+            unsigned c = 0;
+            u64 ms = 0;
+            for (int r = 0; r < C; ++r) {
+                c += ld_cluster32(mx::cluster_map(mx::smem_u32(&S.cnt[b]), r));
+                ms += (u64)ld_cluster32(mx::cluster_map(mx::smem_u32(&S.hi[b]), r)) << 32 | ld_cluster32(mx::cluster_map(mx::smem_u32(&S.lo[b]), r));
+            }
+            st_cluster(mx::cluster_map(mx::smem_u32(&to_cnt[b]), 0), c);
+            st_cluster(mx::cluster_map(mx::smem_u32(&to_mass[b]), 0), ms);
+        }
+        cluster_sync();
+        if (first_cta) {
+            running_sums(to_cnt, to_cnt, SM_BINS, S.scan);
+            running_sums(to_mass, to_mass, SM_BINS, S.scan);
+        }
+    };
+    // first CTA: the next window goes to all; then it is the one in force
+    int wp = 0;
+    auto tell = [&]() {
+        if (first_cta) {
+            if (tid == 0) S.n_all = 0;
+            __syncthreads();
+            constexpr int W = sizeof(Window) / 4;
+            for (int i = tid; i < (C - 1) * W; i += SM_THREADS) {
+                uint32_t *word = (uint32_t *)&S.w[wp ^ 1] + i % W;
+                st_cluster(mx::cluster_map(mx::smem_u32(word), 1 + i / W), *word);
+            }
+        }
+        cluster_sync();
+        wp ^= 1;
+    };
+    auto inside = [&](int i) {
+        const Window &w = S.w[wp];
+        if (w.kind == 0) {
+            const int b = interval(data[i], m, scale);
+            return b >= w.b0 && b <= w.b1;
+        }
+        if (data[i] == -INFINITY) return false;
+        const u64 e = entry(i);
+        return e >= w.lo && e <= w.hi;
+    };
+    // the window's entries, sorted, and their running masses (first CTA: S.all, S.mine); at most SM_LIST
+    auto collect = [&]() {
+        if (tid == 0) S.n_mine = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += SM_THREADS)
+            if (inside(i)) {
+                const unsigned at = atomicAdd(&S.n_mine, 1u);
+                if (at < SM_LIST) S.mine[at] = entry(i);
+            }
+        __syncthreads();
+        // into the first CTA's list, behind what others have put there; nobody looks at this CTA's memory any more
+        const unsigned c = min(S.n_mine, (unsigned)SM_LIST);
+        if (tid == 0 && c) S.found_a = add_cluster(mx::cluster_map(mx::smem_u32(&S.n_all), 0), c);
+        __syncthreads();
+        const unsigned base = (unsigned)S.found_a;
+        for (unsigned i = tid; i < c; i += SM_THREADS)
+            if (base + i < SM_LIST) st_cluster(mx::cluster_map(mx::smem_u32(&S.all[base + i]), 0), S.mine[i]);
+        cluster_sync();
+        int total = 0;
+        if (first_cta) {
+            total = (int)min(S.n_all, (unsigned)SM_LIST);
+            int n2 = 2;
+            while (n2 < total) n2 <<= 1;
+            for (int i = total + tid; i < n2; i += SM_THREADS) S.all[i] = 0;
+            __syncthreads();
+            sort_down(S.all, n2);
+            for (int i = tid; i < total; i += SM_THREADS) S.mine[i] = to_mass(weight(entry_logit(S.all[i]), m, log2e_t, S.table));
+            __syncthreads();
+            running_sums(S.mine, S.mine, total, S.scan);
+        }
+        return total;
+    };
+    // first entry of the order whose running count (by_mass: mass) exceeds t; in the first CTA: its number in the sorted list,
+    // the window and S.mine say what lies in front of it
+    auto search = [&](u64 t, bool by_mass) {
+        if (first_cta) {
+            int b = by_mass ? first_over(S.run_mass, SM_BINS, t, &S.found_a) : first_over(S.run_cnt, SM_BINS, t, &S.found_a);
+            b = min(b, SM_BINS - 1);
+            if (tid == 0) {
+                Window &w = S.w[wp ^ 1];
+                w.kind = 0, w.b0 = w.b1 = b;
+                w.base_count = b ? S.run_cnt[b - 1] : 0, w.base_mass = b ? S.run_mass[b - 1] : 0;
+                w.count = (int)(S.run_cnt[b] - (unsigned)w.base_count);
+            }
+        }
+        tell();
+        while (S.w[wp].count > SM_LIST) {
+            // the range of the window's entries
+            u64 e_lo = ~0ull, e_hi = 0;
+            for (int i = tid; i < n; i += SM_THREADS)
+                if (inside(i)) {
+                    const u64 e = entry(i);
+                    e_lo = min(e_lo, e), e_hi = max(e_hi, e);
+                }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                e_lo = min(e_lo, __shfl_xor_sync(0xFFFFFFFFu, e_lo, o));
+                e_hi = max(e_hi, __shfl_xor_sync(0xFFFFFFFFu, e_hi, o));
+            }
+            clear();
+            if (tid == 0) S.found_b = ~0ull, S.found_c = 0;
+            __syncthreads();
+            if (lane == 0) atomicMin(&S.found_b, e_lo), atomicMax(&S.found_c, e_hi);
+            __syncthreads();
+            if (tid < C) {
+                st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_a[rank]), tid), S.found_b);
+                st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_b[rank]), tid), S.found_c);
+            }
+            cluster_sync();
+            for (int c = 0; c < C; ++c) e_lo = min(e_lo, S.slot_a[c]), e_hi = max(e_hi, S.slot_b[c]);
+            int shr = 0;
+            while ((e_hi - e_lo) >> shr >= SM_BINS) ++shr;
+            for (int i = tid; i < n; i += SM_THREADS)
+                if (inside(i)) {
+                    const u64 e = entry(i);
+                    const int b = (int)((e_hi - e) >> shr);
+                    atomicAdd(&S.cnt[b], 1u);
+                    add_to(b, to_mass(weight(data[i], m, log2e_t, S.table)));
+                }
+            unsigned *c_run = (unsigned *)S.all;   // (no list is in use)
+            merge(c_run, S.mine);
+            if (first_cta) {
+                const Window &now = S.w[wp];
+                const u64 base = by_mass ? now.base_mass : now.base_count;
+                int b = by_mass ? first_over(S.mine, SM_BINS, t - base, &S.found_a) : first_over(c_run, SM_BINS, t - base, &S.found_a);
+                b = min(b, SM_BINS - 1);
+                __syncthreads();
+                if (tid == 0) {
+                    const u64 c_before = b ? c_run[b - 1] : 0;
+                    Window &w = S.w[wp ^ 1];
+                    w.kind = 1;
+                    w.hi = e_hi - ((u64)b << shr);
+                    w.lo = w.hi - e_lo < (1ull << shr) ? e_lo : w.hi - ((1ull << shr) - 1);
+                    w.count = (int)(c_run[b] - c_before);
+                    w.base_count = now.base_count + c_before, w.base_mass = now.base_mass + (b ? S.mine[b - 1] : 0);
+                }
+            }
+            tell();
+        }
+        const int total = collect();
+        int at = 0;
+        if (first_cta) {
+            if (by_mass) at = first_over(S.mine, total, t - S.w[wp].base_mass, &S.found_a);
+            else at = (int)(t - S.w[wp].base_count);
+            at = max(0, min(at, total - 1));
+        }
+        return at;
+    };
+    auto share = [&](double of, u64 total) { return (u64)fmin(of * (double)total, (double)total); };   // (cut off, not rounded)
+
+    bool with_mass = k == 0 || k > SM_LIST / 2;
+    u64 z = 0, z_min = 0;   // first CTA: mass of K, then of what is kept; of M
+    for (;;) {
+        // ---- histogram over max - l ----
+        clear();
+        u64 sum_min = 0;
+        for (int i = tid; i < n; i += SM_THREADS) {
+            const float l = data[i];
+            const int b = interval(l, m, scale);
+            if (b >= SM_BINS) continue;
+            atomicAdd(&S.cnt[b], 1u);
+            if (with_mass) {
+                const double w = weight(l, m, log2e_t, S.table);
+                const u64 mass = to_mass(w);
+                add_to(b, mass);
+                if (w >= min_w) sum_min += mass;
+            }
+        }
+        if (with_mass) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum_min += __shfl_xor_sync(0xFFFFFFFFu, sum_min, o);
+            if (lane == 0) S.scan[warp] = sum_min;
+            __syncthreads();
+            if (tid == 0) {
+                for (int w = 1; w < SM_WARPS; ++w) sum_min += S.scan[w];
+                st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_b[rank]), 0), sum_min);
+            }
+        }
+        merge(S.run_cnt, S.run_mass);
+        // ---- everything that can be kept, if that is one list ----
+        if (first_cta) {
+            int b = SM_BINS - 1;
+            if (k) b = min(b, first_over(S.run_cnt, SM_BINS, (u64)(k - 1), &S.found_a));
+            else if (p < 1.0f) {
+                z = S.run_mass[SM_BINS - 1];
+                b = min(b, first_over(S.run_mass, SM_BINS, (u64)ceil((double)p * (double)z) - 1, &S.found_a));
+            }
+            if (with_mass) {
+                z = S.run_mass[SM_BINS - 1];
+                z_min = 0;
+                for (int c = 0; c < C; ++c) z_min += S.slot_b[c];
+            }
+            __syncthreads();
+            if (tid == 0) {
+                Window &w = S.w[wp ^ 1];
+                w.kind = 0, w.b0 = 0, w.b1 = b, w.base_count = w.base_mass = 0;
+                w.count = (int)S.run_cnt[b];
+            }
+        }
+        tell();
+        if (S.w[wp].count <= SM_LIST || with_mass) break;
+        with_mass = true;   // (many equal logits, or many close to the k-th)
+    }
+    int at;
+    if (S.w[wp].count <= SM_LIST) {
+        const int total = collect();
+        if (!first_cta) return;
+        if (k) z = S.mine[min(k, total) - 1];
+        u64 keep = z;
+        if (p < 1.0f) keep = S.mine[min(first_over(S.mine, total, (u64)ceil((double)p * (double)z) - 1, &S.found_a), total - 1)];
+        if (min_w > 0.0) {
+            // the last entry of M among the list's; M beyond the list keeps all that P keeps
+            if (tid == 0) S.found_b = 0;
+            __syncthreads();
+            for (int i = tid; i < total; i += SM_THREADS)
+                if (weight(entry_logit(S.all[i]), m, log2e_t, S.table) >= min_w) atomicMax(&S.found_b, S.mine[i]);
+            __syncthreads();
+            keep = min(keep, S.found_b);
+        }
+        z = keep;
+        const u64 t = min(share((double)u, z), z - 1);
+        at = min(first_over(S.mine, total, t, &S.found_a), total - 1);
+    } else {
+        if (k) {
+            const int i = search(first_cta ? (u64)min((unsigned)k, S.run_cnt[SM_BINS - 1]) - 1 : 0, false);
+            if (first_cta) z = S.w[wp].base_mass + S.mine[i];
+        }
+        if (p < 1.0f) {
+            const int i = search(first_cta ? (u64)ceil((double)p * (double)z) - 1 : 0, true);
+            if (first_cta) z = S.w[wp].base_mass + S.mine[i];
+        }
+        if (first_cta) z = min(z, z_min);
+        at = search(first_cta ? min(share((double)u, z), z - 1) : 0, true);
+        if (!first_cta) return;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        const u64 e = S.all[at];
+        P.token[row] = (int)(((1u << P.idx_bits) - 1) - (unsigned)(e & ((1ull << P.idx_bits) - 1)));
+        if (P.prob) P.prob[row] = (float)((double)(S.mine[at] - (at ? S.mine[at - 1] : 0)) / (double)z);
+    }
+}
+
+template <typename T>
+int launch_sample(mx230_handle *h, cudaStream_t st, SampleParams P, int n_rows) {
+    constexpr int VE = 16 / (int)sizeof(T);
+    const int pieces = P.vocab / VE + 2;
+    // Smallest cluster whose CTAs can hold the row; more CTAs while SMs have none and each still has a few thousand logits.
+    int c = 1;
+    auto share_of = [&](int n) { return ((pieces + n - 1) / n + 1) * VE; };
+    while (c < SM_CLUSTER && share_of(c) > SM_MAX_DATA) c *= 2;
+    while (c < SM_CLUSTER && (long long)n_rows * c < 2ll * h->sm_count && P.vocab / c > 4096) c *= 2;
+    P.ctas = c, P.cap = share_of(c);
+    const size_t sm = sizeof(Shared) + (size_t)P.cap * sizeof(float);
+    MX_SMEM_ATTR_ONCE(h->device, sample_kernel<T>, 227 * 1024);
+    MX_LAUNCH(h, st, MX230_K_SAMPLE, mx_launch(sample_kernel<T>, dim3((unsigned)(n_rows * c)), SM_THREADS, sm, st, c, true, P));
+    return MX230_OK;
+}
+
+}  // namespace
+
+extern "C" int mx230_sample(mx230_handle *h, void *stream, int *token, float *prob, const void *logits, int dtype, int n_rows,
+                            int vocab, long long row_stride, const float *u, float temperature, const float *temperatures,
+                            int top_k, const int *top_ks, float top_p, const float *top_ps, float min_p, const float *min_ps) {
+    MX_REQUIRE(h, MX230_ERR_INVALID_ARG, "sample: null handle");
+    MX_REQUIRE(dtype == MX230_F32 || dtype == MX230_F16 || dtype == MX230_BF16, MX230_ERR_INVALID_ARG, "sample: element type %d", dtype);
+    MX_REQUIRE(n_rows >= 0 && vocab > 0, MX230_ERR_INVALID_ARG, "sample: %d rows of %d logits", n_rows, vocab);
+    MX_REQUIRE(vocab <= SM_CLUSTER * (SM_MAX_DATA - 32), MX230_ERR_UNSUPPORTED, "sample: %d logits a row (at most %d)", vocab,
+               SM_CLUSTER * (SM_MAX_DATA - 32));
+    MX_REQUIRE(n_rows <= (1 << 27), MX230_ERR_UNSUPPORTED, "sample: %d rows", n_rows);
+    if (n_rows == 0) return MX230_OK;
+    MX_REQUIRE(token && logits && u, MX230_ERR_INVALID_ARG, "sample: null argument");
+    MX_REQUIRE(row_stride >= 0, MX230_ERR_INVALID_ARG, "sample: row stride %lld", row_stride);
+    const size_t size = dtype == MX230_F32 ? 4 : 2;
+    MX_REQUIRE((uintptr_t)logits % size == 0 &&
+                   (((uintptr_t)token | (uintptr_t)prob | (uintptr_t)u | (uintptr_t)temperatures | (uintptr_t)top_ks | (uintptr_t)top_ps |
+                     (uintptr_t)min_ps) & 3) == 0, MX230_ERR_INVALID_ARG, "sample: misaligned pointer");
+    SampleParams P{};
+    P.token = token, P.prob = prob, P.logits = logits, P.row_stride = row_stride, P.vocab = vocab, P.u = u;
+    P.temperature = temperature, P.top_k = top_k, P.top_p = top_p, P.min_p = min_p;
+    P.temperatures = temperatures, P.top_ks = top_ks, P.top_ps = top_ps, P.min_ps = min_ps;
+    while ((1 << P.idx_bits) < vocab) ++P.idx_bits;
+    if (P.idx_bits == 0) P.idx_bits = 1;
+    mx230_device_guard guard(h->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == MX230_F32) return launch_sample<float>(h, st, P, n_rows);
+    if (dtype == MX230_F16) return launch_sample<__half>(h, st, P, n_rows);
+    return launch_sample<__nv_bfloat16>(h, st, P, n_rows);
+}

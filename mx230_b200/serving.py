@@ -8,7 +8,8 @@ whatever the caller passes in: an object with
     decode_batched(cur: np.ndarray[uint32, n], pos: np.ndarray[int32, n],
                    tables: np.ndarray[int32, n x n_log]) -> sequence of n next tokens
 
-whose attention runs through `llm_attention.prefill_step` / `batched_step` with those block tables.
+whose attention runs through `llm_attention.prefill_step` / `batched_step` with those block tables.  With a `Sampler` both
+return logits instead (device tensors, [vocab] and [n][vocab]), and the tokens are drawn here by each request's settings.
 """
 from __future__ import annotations
 
@@ -17,15 +18,24 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from ._lib import check, lib
+import torch
+
+from ._lib import addr, check, lib, require
+from .common import Handle, stream_ptr
+from .llm_attention import _DTYPES, on_device
 from .paging import KvPool
 
 
 @dataclass
 class Request:
-    """Request, gpu.rs:356-359."""
+    """Request, gpu.rs:356-359, and how its tokens are drawn where a `Sampler` draws them (the settings of `sample`;
+    temperature 0: the most likely one)."""
     prompt: list
     max_new: int
+    temperature: float = 0.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
 
 
 @dataclass
@@ -93,16 +103,72 @@ class Scheduler:
         return ServeStats(f(self._s, 0), f(self._s, 1), f(self._s, 2))
 
 
-def run_continuous(model, pool: KvPool, n_ctx: int, requests: list[Request], max_batch: int, trace=None):
+def sample(h: Handle, token, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, prob=None, stream=None):
+    """The next token of each row of `logits` [n][vocab] (fp32, fp16 or bf16; the values of a row contiguous) into `token` int32 [n],
+    from random numbers `u` fp32 [n] in [0, 1); its probability among what could be drawn into `prob` fp32 [n].  Each setting
+    is a number or a tensor [n] (fp32, top_k int32).  include/mx230_attn.h has the definition at mx230_sample: entries in falling
+    order, the first top_k of them, of those the shortest prefix with top_p of their weight, cut at min_p times the largest
+    weight; the token is where the running weight passes u.  -1 where a row is masked throughout."""
+    require(logits.dim() == 2 and logits.dtype in _DTYPES, f"sample: logits {tuple(logits.shape)} of {logits.dtype}")
+    n, vocab = logits.shape
+    on_device(h, "sample: logits", logits)
+    require(vocab < 2 or logits.stride(1) == 1, "sample: the logits of a row must be contiguous")
+
+    def vector(what, t, dtype):
+        on_device(h, "sample: " + what, t, dtype)
+        require(t.shape == (n,) and (n < 2 or t.stride(0) == 1), f"sample: {what} {tuple(t.shape)} for {n} rows")
+        return addr(t)
+
+    def setting(what, v, dtype, number):
+        return (number(0), vector(what, v, dtype)) if isinstance(v, torch.Tensor) else (number(v), None)
+
+    check(lib().mx230_sample(h._h, stream_ptr(stream, h.device), vector("token", token, torch.int32),
+                             None if prob is None else vector("prob", prob, torch.float32), addr(logits), _DTYPES[logits.dtype], n, vocab,
+                             logits.stride(0), vector("u", u, torch.float32), *setting("temperature", temperature, torch.float32, float),
+                             *setting("top_k", top_k, torch.int32, int), *setting("top_p", top_p, torch.float32, float),
+                             *setting("min_p", min_p, torch.float32, float)))
+
+
+class Sampler:
+    """Draws the tokens of `run_continuous`.  The random number of a request's t-th token depends on (seed, request, t) alone, so a
+    request's tokens do not depend on what is served beside it."""
+
+    def __init__(self, h: Handle, seed: int = 0):
+        self.h, self.seed = h, seed
+
+    def uniform(self, request: int, step: int) -> float:
+        bits = np.random.Philox(key=self.seed, counter=[request, step, 0, 0]).random_raw()
+        return (int(bits) >> 40) * 2.0 ** -24
+
+    def draw(self, logits, rows) -> list[int]:
+        """One token for each of `rows`, (request index, step, Request), from its row of `logits`."""
+        logits = logits.reshape(len(rows), -1)
+        dev = lambda a, t: torch.tensor(a, dtype=t, device=logits.device)  # noqa: E731
+        token = torch.empty(len(rows), dtype=torch.int32, device=logits.device)
+        sample(self.h, token, logits, dev([self.uniform(r, t) for r, t, _ in rows], torch.float32),
+               dev([q.temperature for *_, q in rows], torch.float32), dev([q.top_k for *_, q in rows], torch.int32),
+               dev([q.top_p for *_, q in rows], torch.float32), dev([q.min_p for *_, q in rows], torch.float32))
+        out = token.tolist()
+        for (r, t, _), tok in zip(rows, out):
+            require(tok >= 0, f"request {r}: every logit of token {t} is masked")
+        return out
+
+
+def run_continuous(model, pool: KvPool, n_ctx: int, requests: list[Request], max_batch: int, trace=None,
+                   sampler: Sampler | None = None):
     """Serves `requests` keeping up to `max_batch` sequences decoding together; returns each
     request's generated tokens (request order) and the occupancy statistics.  `trace`, when given,
-    receives one tuple per event (for tests)."""
+    receives one tuple per event (for tests).  `sampler`: the model returns logits, and it draws the tokens."""
     s = Scheduler(pool, n_ctx, max_batch, requests)
+    owner = {}   # first block of a running request's table -> the request
     try:
         while True:
             while (adm := s.admit()) is not None:
                 r, table = adm
                 first = model.prefill(r, requests[r].prompt, table)
+                if sampler is not None:
+                    owner[int(table[0])] = r
+                    first = sampler.draw(first, [(r, 0, requests[r])])[0]
                 if trace is not None:
                     trace.append(("admit", r, table.tolist(), int(first)))
                 s.admitted(r, first)
@@ -110,6 +176,9 @@ def run_continuous(model, pool: KvPool, n_ctx: int, requests: list[Request], max
             if cur.size == 0:
                 break
             nxt = model.decode_batched(cur.copy(), pos.copy(), tables.copy())
+            if sampler is not None:
+                rows = [owner[int(t[0])] for t in tables]
+                nxt = sampler.draw(nxt, [(r, int(p) - len(requests[r].prompt) + 1, requests[r]) for r, p in zip(rows, pos)])
             if trace is not None:
                 trace.append(("step", cur.tolist(), pos.tolist(), tables.tolist(), [int(x) for x in nxt]))
             s.step_done(nxt)

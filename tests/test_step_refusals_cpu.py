@@ -68,3 +68,16 @@ def test_int4_refuses(L):
     # 16 x 64 tiles of 512 bytes, 64 bytes per 16 outputs and group
     assert L.mx230_int4_bytes(256, 64, 64) == 4 * 4 * 512 + 4 * 4 * 64 and L.mx230_int4_bytes(65, 17, 32) == 2 * 2 * 512 + 2 * 3 * 64
     assert L.mx230_int4_bytes(0, 64, 64) == 0 and L.mx230_int4_bytes(1 << 17, 1 << 19, 64) == (1 << 15) * (1 << 11) * 576
+
+
+def test_sample_refuses(L):
+    ok = dict(h=H, st=None, token=P, prob=None, logits=P, dt=0, rows=4, vocab=100, stride=100, u=P, t=1.0, ts=None, k=0, ks=None, p=1.0, ps=None,
+              m=0.0, ms=None)
+    cases = [dict(h=None), dict(token=None), dict(logits=None), dict(u=None), dict(dt=3), dict(rows=-1), dict(vocab=0), dict(vocab=-1), dict(stride=-1),
+             dict(logits=P + 2), dict(logits=P + 1, dt=1), dict(token=P + 2), dict(prob=P + 1), dict(u=P + 2), dict(ts=P + 2), dict(ks=P + 1),
+             dict(ps=P + 3), dict(ms=P + 2)]
+    for c in cases:
+        assert L.mx230_sample(*{**ok, **c}.values()) == _lib.ERR_INVALID_ARG, c
+    assert L.mx230_sample(*{**ok, "vocab": 360193}.values()) == _lib.ERR_UNSUPPORTED
+    assert L.mx230_sample(*{**ok, "rows": 1 << 28}.values()) == _lib.ERR_UNSUPPORTED
+    assert L.mx230_sample(*{**ok, "rows": 0}.values()) == 0
