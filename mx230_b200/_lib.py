@@ -90,10 +90,11 @@ def check(code: int) -> None:
         raise Mx230Error(code, lib().mx230_last_error().decode())
 
 
-def require(cond, msg: str) -> None:
-    """The bindings' own checks, for what no pointer shows (shapes, types, devices): the error that the library would raise."""
+def require(cond, msg) -> None:
+    """The bindings' own checks, for what no pointer shows (shapes, types, devices): the error that the library would raise.
+    `msg`: the text, or what makes it (a text with values in it costs more than the check)."""
     if not cond:
-        raise Mx230Error(ERR_INVALID_ARG, msg)
+        raise Mx230Error(ERR_INVALID_ARG, msg if isinstance(msg, str) else msg())
 
 
 def ptr(t) -> C.c_void_p | None:

@@ -75,16 +75,19 @@ def _stream_getter():
 _current_raw_stream = None
 
 
-def stream_ptr(stream=None, device=None):
+def raw_stream(stream=None, device=None) -> int:
     """Raw CUstream of a torch stream (None = torch's current stream, of the current device or of `device`)."""
-    if isinstance(stream, int):
-        return C.c_void_p(stream)
     if stream is not None:
-        return C.c_void_p(stream.cuda_stream)
+        return stream if isinstance(stream, int) else stream.cuda_stream
     global _current_raw_stream
     if _current_raw_stream is None:
         _current_raw_stream = _stream_getter()
-    return C.c_void_p(_current_raw_stream(device))
+    return _current_raw_stream(device)
+
+
+def stream_ptr(stream=None):
+    """The same as a pointer, of torch's current device."""
+    return C.c_void_p(raw_stream(stream))
 
 
 def time_median_ms(stream, warmup: int, iters: int, f) -> float:

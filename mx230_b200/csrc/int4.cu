@@ -4,18 +4,20 @@
 // Bounded by HBM on the weights: half a byte each, read once, and 4 bytes of scale and zero point per group.  At that rate an SM
 // takes 46 weights a cycle, so a weight may cost about two instructions of a lane; multiply-adds on CUDA cores, with the
 // conversion from 4 bits in front, would take more for a single row and that many times more for several.  Hence warp-level
-// tensor-core tiles (m16n8k16) with the weights as A: 16 outputs x 16 inputs, q - z formed exactly in fp16 (two instructions for
-// two weights: the four bits or'ed into the mantissa of 1024, or of 64 + z in sixteenths, and the offset taken off), and the rows as
-// the eight columns of B, two columns a row:
+// tensor-core tiles (m16n8k16) with the weights as A: 16 outputs x 16 inputs.  Four bits in the lowest places of an fp16 are the
+// number q 2^-24 (a subnormal, which the tensor cores take as it is), in the next four places 16 q 2^-24, so a pair of weights costs
+// one "and", and half the inputs carry a factor of 1/16 against it.  The rows are the eight columns of B, two columns a row:
 //   x 2^e = hi + lo, both fp16, e such that the largest of the 64 values of a tile lies in [2^14, 2^15):
-// |x 2^e - hi - lo| <= 2^-24 |x 2^e|, as exact as x itself (but for values 2^-15 times the tile's largest and less, which keep an
-// absolute error of 2^-40 of that).  Products are then exact in fp32; sums are fp32, per tile of 64 inputs (32, if groups are of
-// 32), and are multiplied by s 2^-e into the row's fp32 total.
+// |x 2^e - hi - lo| <= 2^-24 |x 2^e|, as exact as x itself (but for values 2^-13 times the tile's largest and less, which keep an
+// absolute error of 2^-35 of that).  Products are then exact in fp32; sums are fp32, per tile of 64 inputs (32, if groups are of
+// 32).  The zero point meets the sum of the tile's x: the row's total gets s 2^(24 - e) (sum x q - z sum x), whose error goes by
+// sum |x| (q + z) instead of sum |x (q - z)|, about four times that, and saves the subtraction per weight (161 instructions a
+// warp and tile with it, of which 36 for the conversion; the kernel was bound by them: 37 us for 4096 x 14336, one row).
 //
 // Layout, made once by mx230_pack_int4: tiles of 16 outputs x 64 inputs, 512 bytes, of which lane (g = lane / 4, j = lane % 4) has 16:
 // words [row g: inputs 8j .. 8j+7][row g: inputs 32 + 8j ..][row g + 8: 8j ..][row g + 8: 32 + 8j ..], input 2p of eight at bits
 // 4p, input 2p + 1 at bits 16 + 4p.  (Which input a k index of the MMA stands for is free, as long as A and B agree.)  Tiles of an
-// output row follow one another along the inputs; behind all tiles, per (16 outputs, group), 16 words (s, 1024 + z) of fp16.
+// output row follow one another along the inputs; behind all tiles, per (16 outputs, group), 16 words (s, z) of fp16.
 //
 // Order of the sums: the inputs are cut into S slices (a power of two that depends on n_in and n_out alone), each summed by one warp
 // in index order, and the slices are added pairwise.  So a row has the same bits whatever rows are computed with it.
@@ -31,6 +33,7 @@ constexpr int W4_WARPS = 8;
 constexpr int W4_THREADS = W4_WARPS * 32;
 constexpr int W4_CLUSTER = 8;     // most CTAs whose sums are added through shared memory
 constexpr int W4_X_BYTES = 64 * 1024;   // of shared memory for rows, about
+constexpr int SLICE_WARPS = 16, TWO_WARPS = 16, KW_MOST = 8;
 
 struct Int4Params {
     float *y;
@@ -46,7 +49,7 @@ struct Int4Params {
     long long x_stride, y_stride, add_stride;
 };
 
-// (s, 1024 + z) and codes of one output tile and input tile; padding: s = 0
+// (s, z) and codes of one output tile and input tile; padding: s = 0
 __global__ void pack_int4_kernel(uint4 *codes_out, uint32_t *sz_out, const uint8_t *codes, const __half *scales, const uint8_t *zeros,
                                  int n_in, int n_out, int group, int n_tiles, int k_tiles, int groups) {
     const long long n_codes = (long long)n_tiles * k_tiles * 32, n_sz = (long long)n_tiles * groups * 16;
@@ -69,10 +72,10 @@ __global__ void pack_int4_kernel(uint4 *codes_out, uint32_t *sz_out, const uint8
             const long long s = i - n_codes;
             const long long t = s >> 4;
             const int nt = (int)(t / groups), gr = (int)(t - (long long)nt * groups), o = nt * W4_N + (int)(s & 15);
-            __half sc = __float2half(0.0f), z = __float2half(1024.0f + 8.0f);
+            __half sc = __float2half(0.0f), z = __float2half(8.0f);
             if (o < n_out) {
                 sc = scales[(size_t)gr * n_out + o];
-                if (zeros) z = __float2half(1024.0f + (float)zeros[(size_t)gr * n_out + o]);
+                if (zeros) z = __float2half((float)zeros[(size_t)gr * n_out + o]);
             }
             sz_out[s] = (uint32_t)__half_as_ushort(sc) | (uint32_t)__half_as_ushort(z) << 16;
         }
@@ -86,22 +89,13 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {   // (a & b) | c in one instruction
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-    return r;
-}
 __device__ __forceinline__ uint32_t h2_u(__half2 v) { return *(uint32_t *)&v; }
 __device__ __forceinline__ __half2 u_h2(uint32_t v) { return *(__half2 *)&v; }
 
-// eight codes -> four pairs (inputs 2p, 2p + 1) of q - z; z1024 = (1024 + z) twice, z64 = -(64 + z) twice
-__device__ __forceinline__ void dequant8(uint32_t w, __half2 z1024, __half2 z64, uint32_t (&a)[4]) {
-    const __half2 sixteenth = __float2half2_rn(0.0625f);
+// eight codes -> four pairs (inputs 2p, 2p + 1) of q 2^-24 (p even) or 16 q 2^-24 (p odd)
+__device__ __forceinline__ void pairs8(uint32_t w, uint32_t (&a)[4]) {
     const uint32_t v = w >> 8;
-    a[0] = h2_u(__hsub2(u_h2(and_or(w, 0x000F000Fu, 0x64006400u)), z1024));
-    a[1] = h2_u(__hfma2(u_h2(and_or(w, 0x00F000F0u, 0x64006400u)), sixteenth, z64));   // (1024 + 16 q) / 16 - 64 - z
-    a[2] = h2_u(__hsub2(u_h2(and_or(v, 0x000F000Fu, 0x64006400u)), z1024));
-    a[3] = h2_u(__hfma2(u_h2(and_or(v, 0x00F000F0u, 0x64006400u)), sixteenth, z64));
+    a[0] = w & 0x000F000Fu, a[1] = w & 0x00F000F0u, a[2] = v & 0x000F000Fu, a[3] = v & 0x00F000F0u;
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -121,8 +115,9 @@ __device__ __forceinline__ float tree_sum(const float *p, int n, int step) {
 }
 
 // NT: column tiles of four rows.  T: output tiles of a warp.  G32: groups of 32 inputs (else a multiple of 64).
-// Shared memory: rows [kw][xq][NT][lanes][8 words], their scales [kw][xq][NT * 4], ring [8 warps][STAGES][T][512 + 64 or 128],
-// sums [8 warps][T * NT * 64]; in the first CTA of a cluster also the other CTAs' sums.
+// Shared memory: ring [8 warps][STAGES][T][512 + 64 or 128], sums [8 warps][T * NT * 64], in the first CTA of a cluster also the
+// other CTAs' sums; per (slice, tile, row) {2^-e, 2^(e - 24) sum x, or that of either half}; 32 bytes of zeros; rows
+// [kw][xq][NT][lanes][8 words].
 constexpr int STAGES = 6;
 template <int NT, int T, bool G32>
 struct Int4Smem {
@@ -140,43 +135,51 @@ __global__ void __launch_bounds__(W4_THREADS) gemv_int4_kernel(const Int4Params 
     const int kw = P.kw, tg = W4_WARPS / kw, C = P.ctas_k;
     const int rank = blockIdx.x % C, grp = blockIdx.x / C;
     const int row0 = blockIdx.y * (4 * NT), rows = min(4 * NT, P.n_rows - row0);
-    const int rt = min(4, rows);                            // rows of a column tile that are there at all
-    const int x_lanes = NT == 1 ? 8 * rt : 32;
+    const int rt = NT == 1 ? rows : 4;                      // rows of a column tile that are there at all
+    const int x_lanes = 8 * rt;
     unsigned char *ring = smem + warp * (STAGES * S::STAGE);
     float *sums = (float *)(smem + S::RING);                // [8][SUMS]
     float *parts = sums + W4_WARPS * S::SUMS;               // [C][tg][SUMS], first CTA
-    float *xscale = parts + (C > 1 ? C * tg * S::SUMS : 0); // [kw][xq][NT * 4]
-    uint32_t *xf = (uint32_t *)(xscale + kw * P.xq * NT * 4);   // [kw][xq][NT][x_lanes][8]
+    float4 *xrow = (float4 *)(parts + (C > 1 ? C * tg * S::SUMS : 0));   // [kw][xq][NT * 4]
+    uint4 *zeros = (uint4 *)(xrow + kw * P.xq * NT * 4);    // 32 bytes
+    uint4 *xf = zeros + 2;                                  // [kw][xq][NT][x_lanes][2]
 
     mx::pdl_trigger();
     if (C > 1) mx::cluster_arrive_relaxed();   // waited for before the first store to another CTA's memory
+    if (tid < 2) zeros[tid] = make_uint4(0, 0, 0, 0);
     mx::pdl_wait();
 
     // this warp's slice and output tiles
     const int ws = warp % kw, slice = rank * kw + ws, n_slices = C * kw;
     const int t_first = (grp * tg + warp / kw) * T;
     const int k0 = (int)((long long)P.k_tiles * slice / n_slices), k1 = (int)((long long)P.k_tiles * (slice + 1) / n_slices);
+    // what is requested next: tile kq, with its group gq of which left_q tiles are still to come
+    constexpr int LPT = S::SZ / 16;                         // lanes that fetch (s, z) of a tile
+    const bool any = t_first < P.n_tiles, szl = lane < T * LPT;
     const int per_group = G32 ? 1 : P.group / W4_K;
-    auto request = [&](int kt, int stage) {
-        if (kt < k1 && t_first < P.n_tiles) {
-            unsigned char *dst = ring + stage * S::STAGE;
+    const uint4 *code_q[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) code_q[t] = P.codes + ((size_t)min(t_first + t, P.n_tiles - 1) * P.k_tiles + k0) * 32 + lane;
+    const uint32_t *sz_row = P.sz + (size_t)min(t_first + lane / LPT, P.n_tiles - 1) * P.groups * 16 + (lane & 3) * 4;
+    int kq = k0, gq = G32 ? 2 * k0 + ((lane & (LPT - 1)) >> 2) : k0 / per_group, left_q = G32 ? 1 : per_group - (k0 - gq * per_group);
+    auto request = [&](int stage) {
+        if (any && kq < k1) {
+            const uint32_t dst = mx::smem_u32(ring + stage * S::STAGE) + lane * 16;
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                const int nt = min(t_first + t, P.n_tiles - 1);
-                cp_async16(mx::smem_u32(dst + t * 512 + lane * 16), P.codes + ((size_t)nt * P.k_tiles + kt) * 32 + lane);
+                cp_async16(dst + t * 512, code_q[t]);
+                code_q[t] += 32;
             }
-            constexpr int LPT = S::SZ / 16;                 // lanes that fetch (s, z) of a tile
-            if (lane < T * LPT) {
-                const int nt = min(t_first + lane / LPT, P.n_tiles - 1);
-                // (a second group of 32 behind the last one: the padding of the inputs, whatever it is multiplied by is 0)
-                const int gr = G32 ? min(2 * kt + (lane % LPT) / 4, P.groups - 1) : kt / per_group;
-                cp_async16(mx::smem_u32(dst + T * 512 + lane * 16), P.sz + ((size_t)nt * P.groups + gr) * 16 + (lane & 3) * 4);
-            }
+            // (a second group of 32 behind the last one: the padding of the inputs, whatever it is multiplied by is 0)
+            if (szl) cp_async16(dst + T * 512, sz_row + (size_t)(G32 ? min(gq, P.groups - 1) : gq) * 16);
+            if (G32) gq += 2;
+            else if (--left_q == 0) left_q = per_group, ++gq;
+            ++kq;
         }
         cp_async_commit();
     };
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) request(k0 + s, s);
+    for (int s = 0; s < STAGES - 1; ++s) request(s);
 
     float total[T][NT][2];
 #pragma unroll
@@ -190,10 +193,10 @@ __global__ void __launch_bounds__(W4_THREADS) gemv_int4_kernel(const Int4Params 
         if (c0) __syncthreads();
         // ---- rows of the next xq tiles of every slice: scaled, split, in the order of B's fragments ----
         // a thread takes the 16 inputs (8j .. , 32 + 8j ..) of a (slice, tile, row); the four of a row follow one another
-        const int n_x = kw * P.xq * NT * 4 * 4;
+        const int rr = NT == 1 ? rt : 4 * NT, n_x = kw * P.xq * rr * 4;
         for (int i0 = tid & ~31; i0 < n_x; i0 += W4_THREADS) {   // (whole warps, for the shuffles)
             const int i = min(i0 + lane, n_x - 1);
-            const int jj = i & 3, r = (i >> 2) & (NT * 4 - 1), q = (i >> 2) / (NT * 4), sl = q / P.xq, kk = q - sl * P.xq;
+            const int jj = i & 3, q = (i >> 2) / rr, r = (i >> 2) - q * rr, sl = q / P.xq, kk = q - sl * P.xq;
             const int s_ = rank * kw + sl;
             const int kt = (int)((long long)P.k_tiles * s_ / n_slices) + c0 + kk;
             const bool in = i0 + lane < n_x && r < rows && c0 + kk < most && kt < P.k_tiles;
@@ -212,62 +215,69 @@ __global__ void __launch_bounds__(W4_THREADS) gemv_int4_kernel(const Int4Params 
             float amax = 0.0f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(v[e]));
-            amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
-            // 2^(14 - exponent of amax) and its inverse, by their bits
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+            // e = 14 - exponent of amax; 2^e and 2^-e by their bits
             const int eb = max((int)(__float_as_uint(amax) >> 23), 15);
-            const float up = __uint_as_float((uint32_t)(268 - eb) << 23);
+            float up = __uint_as_float((uint32_t)(268 - eb) << 23), down = __uint_as_float((uint32_t)(eb - 14) << 23);
+            if (amax == INFINITY) {   // infinite values alone count: as 1, and the tile's sum times infinity
+                up = 1.0f, down = INFINITY;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = isinf(v[e]) ? copysignf(1.0f, v[e]) : v[e] == v[e] ? 0.0f : v[e];
+            }
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] *= up, sum[e >> 3] += v[e];
+            if (!G32) sum[0] += sum[1];
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                sum[0] += __shfl_xor_sync(0xFFFFFFFFu, sum[0], o);
+                if (G32) sum[1] += __shfl_xor_sync(0xFFFFFFFFu, sum[1], o);
+            }
             if (i0 + lane >= n_x) continue;
-            if (jj == 0) xscale[q * (NT * 4) + r] = __uint_as_float((uint32_t)(eb - 14) << 23);
+            if (jj == 0) xrow[q * (NT * 4) + r] = make_float4(down, sum[0] * 0x1p-24f, sum[1] * 0x1p-24f, 0.0f);
             uint32_t hi[8], lo[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float a = v[2 * e] * up, b = v[2 * e + 1] * up;
-                const __half ha = __float2half_rn(a), hb = __float2half_rn(b);
-                const float fa = __half2float(ha), fb = __half2float(hb);
-                hi[e] = h2_u(__halves2half2(ha, hb));
-                // (an infinite value has no second part)
-                lo[e] = h2_u(__halves2half2(__float2half_rn(isinf(fa) ? 0.0f : a - fa), __float2half_rn(isinf(fb) ? 0.0f : b - fb)));
+                const float f = (e & 1) ? 0.0625f : 1.0f, a = v[2 * e] * f, b = v[2 * e + 1] * f;
+                const __half2 h = __floats2half2_rn(a, b);
+                const float2 back = __half22float2(h);
+                hi[e] = h2_u(h), lo[e] = h2_u(__floats2half2_rn(a - back.x, b - back.y));
             }
-            const int n = r >> 2, l = (r & 3) * 8 + jj;     // lanes of columns 2 (r % 4) and 2 (r % 4) + 1
-            if (l < x_lanes) {
-                // pairs 0 .. 3 of each half of the tile: MMA steps 2 hf, 2 hf + 1 take two each
-                uint4 *dst = (uint4 *)(xf + ((size_t)(q * NT + n) * x_lanes + l) * 8);
-                dst[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]), dst[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-                dst += 8;
-                dst[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]), dst[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
-            }
+            // lanes of columns 2 (r % 4) and 2 (r % 4) + 1; pairs 0 .. 3 of each half of the tile: MMA steps 2 hf, 2 hf + 1
+            uint4 *dst = xf + ((size_t)(q * NT + (r >> 2)) * x_lanes + (r & 3) * 8 + jj) * 2;
+            dst[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]), dst[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+            dst[8] = make_uint4(lo[0], lo[1], lo[2], lo[3]), dst[9] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
         }
         __syncthreads();
         // ---- this warp's tiles ----
         const int end = min(k1 - k0, c0 + P.xq);
+        const bool has_x = lane < x_lanes;                    // columns of rows that are not there: zeros
+        const uint4 *xp = has_x ? xf + ((size_t)ws * P.xq * NT * x_lanes + lane) * 2 : zeros;
+        const float4 *rp = xrow + ws * P.xq * (NT * 4) + (NT == 1 ? min(j, rt - 1) : j);   // the row whose sums this lane gets
+        const int x_step = has_x ? x_lanes * 2 : 0;
         for (int kk = c0; kk < end; ++kk) {
             cp_async_wait<STAGES - 2>();
             __syncwarp();
             const unsigned char *st = ring + stage * S::STAGE;
-            const int q = ws * P.xq + kk - c0;
             uint4 b[NT][2];
-            float xs[NT];
+            float4 xr[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const uint4 *src = (const uint4 *)(xf + ((size_t)(q * NT + n) * x_lanes + lane) * 8);
-                b[n][0] = b[n][1] = make_uint4(0, 0, 0, 0);
-                if (lane < x_lanes) b[n][0] = src[0], b[n][1] = src[1];
-                xs[n] = xscale[q * (NT * 4) + n * 4 + j];   // of the row whose sums this lane gets
+                b[n][0] = xp[0], b[n][1] = xp[1];
+                xp += x_step;
+                xr[n] = rp[n * 4];
             }
+            rp += NT * 4;
 #pragma unroll
             for (int t = 0; t < T; ++t) {
                 const uint4 w = *(const uint4 *)(st + t * 512 + lane * 16);
                 float acc[NT][4];
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    const uint32_t *sz = (const uint32_t *)(st + T * 512 + t * S::SZ + (G32 ? hf * 64 : 0));
-                    const __half2 s0 = u_h2(sz[g]), s1 = u_h2(sz[g + 8]);
-                    const __half2 sub = __float2half2_rn(960.0f);
-                    const __half2 z0 = __high2half2(s0), z1 = __high2half2(s1);
                     uint32_t a0[4], a1[4];
-                    dequant8(hf ? w.y : w.x, z0, __hsub2(sub, z0), a0);   // 960 - (1024 + z) = -(64 + z)
-                    dequant8(hf ? w.w : w.z, z1, __hsub2(sub, z1), a1);
+                    pairs8(hf ? w.y : w.x, a0);
+                    pairs8(hf ? w.w : w.z, a1);
                     if (G32 || hf == 0)
 #pragma unroll
                         for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
@@ -276,16 +286,21 @@ __global__ void __launch_bounds__(W4_THREADS) gemv_int4_kernel(const Int4Params 
                         mma_f16(acc[n], a0[0], a1[0], a0[1], a1[1], b[n][hf].x, b[n][hf].y);
                         mma_f16(acc[n], a0[2], a1[2], a0[3], a1[3], b[n][hf].z, b[n][hf].w);
                     }
-                    if (G32 || hf == 1)
+                    if (G32 || hf == 1) {
+                        const uint32_t *sz = (const uint32_t *)(st + T * 512 + t * S::SZ + (G32 ? hf * 64 : 0));
+                        const float2 s0 = __half22float2(u_h2(sz[g])), s1 = __half22float2(u_h2(sz[g + 8]));
+                        const float m0 = s0.x * 0x1p24f, m1 = s1.x * 0x1p24f;
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            total[t][n][0] = fmaf(__low2float(s0) * xs[n], acc[n][0] + acc[n][1], total[t][n][0]);
-                            total[t][n][1] = fmaf(__low2float(s1) * xs[n], acc[n][2] + acc[n][3], total[t][n][1]);
+                            const float xs = G32 && hf ? xr[n].z : xr[n].y;
+                            total[t][n][0] = fmaf(m0, fmaf(-s0.y, xs, acc[n][0] + acc[n][1]) * xr[n].x, total[t][n][0]);
+                            total[t][n][1] = fmaf(m1, fmaf(-s1.y, xs, acc[n][2] + acc[n][3]) * xr[n].x, total[t][n][1]);
                         }
+                    }
                 }
             }
             __syncwarp();
-            request(k0 + kk + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+            request(stage == 0 ? STAGES - 1 : stage - 1);
             stage = stage == STAGES - 1 ? 0 : stage + 1;
         }
     }
@@ -325,11 +340,11 @@ int launch_int4(mx230_handle *h, cudaStream_t st, Int4Params P) {
     using S = Int4Smem<NT, T, G32>;
     const int tg = W4_WARPS / P.kw, C = P.ctas_k, n_slices = P.kw * C;
     const int most = (P.k_tiles + n_slices - 1) / n_slices;
-    const int per_tile = P.kw * NT * (32 * (NT == 1 ? 8 * (P.n_rows < 4 ? P.n_rows : 4) : 32) + 16);
+    const int per_tile = P.kw * NT * (32 * (NT == 1 ? 8 * (P.n_rows < 4 ? P.n_rows : 4) : 32) + 64);
     P.xq = W4_X_BYTES / per_tile;
     if (P.xq > most) P.xq = most;
     if (P.xq < 1) P.xq = 1;
-    const size_t sm = (size_t)S::RING + (size_t)(W4_WARPS + (C > 1 ? C * tg : 0)) * S::SUMS * 4 + (size_t)P.xq * per_tile;
+    const size_t sm = (size_t)S::RING + (size_t)(W4_WARPS + (C > 1 ? C * tg : 0)) * S::SUMS * 4 + 32 + (size_t)P.xq * per_tile;
     MX_SMEM_ATTR_ONCE(h->device, (gemv_int4_kernel<NT, T, G32>), 227 * 1024);
     const long long groups_n = (P.n_tiles + (long long)tg * T - 1) / ((long long)tg * T);
     const dim3 grid((unsigned)(groups_n * C), (unsigned)((P.n_rows + 4 * NT - 1) / (4 * NT)));
@@ -395,14 +410,20 @@ extern "C" int mx230_gemv_int4(mx230_handle *h, void *stream, float *y, const fl
     P.n_tiles = (int)((n_out + (long long)W4_N - 1) / W4_N), P.k_tiles = (int)((n_in + (long long)W4_K - 1) / W4_K);
     P.x_stride = x_stride, P.y_stride = y_stride, P.add_stride = add_stride;
     P.x_vec = ((uintptr_t)x & 15) == 0 && (n_rows < 2 || x_stride % 4 == 0);
-    // Slices of the inputs: enough warps for eight per SM, as far as there are tiles.  This fixes the order of the sums.
+    // Slices of the inputs: enough warps for sixteen per SM, as far as there are tiles.  This fixes the order of the sums.
     int n_slices = 1;
-    while (n_slices < W4_WARPS * W4_CLUSTER && 2 * n_slices <= P.k_tiles && (long long)P.n_tiles * n_slices < 8ll * h->sm_count) n_slices *= 2;
-    P.kw = n_slices < W4_WARPS ? n_slices : W4_WARPS;
+    while (n_slices < W4_WARPS * W4_CLUSTER && 2 * n_slices <= P.k_tiles && (long long)P.n_tiles * n_slices < SLICE_WARPS * h->sm_count) n_slices *= 2;
+    const bool two = (long long)P.n_tiles * n_slices >= TWO_WARPS * h->sm_count;
+    P.kw = n_slices < KW_MOST ? n_slices : KW_MOST;
+    while (n_slices / P.kw > W4_CLUSTER) P.kw *= 2;
     P.ctas_k = n_slices / P.kw;
     mx230_device_guard guard(h->device);
     cudaStream_t st = (cudaStream_t)stream;
     const bool g32 = group == 32;
-    if (n_rows <= 4) return g32 ? launch_int4<1, 1, true>(h, st, P) : launch_int4<1, 1, false>(h, st, P);
+    if (n_rows <= 4) {
+        if (two) return g32 ? launch_int4<1, 2, true>(h, st, P) : launch_int4<1, 2, false>(h, st, P);
+        return g32 ? launch_int4<1, 1, true>(h, st, P) : launch_int4<1, 1, false>(h, st, P);
+    }
+    if (two) return g32 ? launch_int4<2, 2, true>(h, st, P) : launch_int4<2, 2, false>(h, st, P);
     return g32 ? launch_int4<2, 1, true>(h, st, P) : launch_int4<2, 1, false>(h, st, P);
 }

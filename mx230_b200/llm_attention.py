@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 from ._lib import addr, check, lib, ptr, require
-from .common import Handle, stream_ptr
+from .common import Handle, raw_stream, stream_ptr
 
 KV_BLOCK = 16  # 03-llm-engine/src/gpu.rs:209
 
@@ -91,8 +91,8 @@ _SCALINGS = {"linear": (1, ()), "ntk": (2, ()), "wavelength": (3, ("low", "high"
 
 def on_device(h: Handle, what: str, t, dtype=None):
     """A CUDA tensor of the handle's device, and of `dtype`."""
-    require(isinstance(t, torch.Tensor) and t.is_cuda and t.device.index == h.device, f"{what}: not a tensor of device {h.device}")
-    require(dtype is None or t.dtype == dtype, f"{what}: {t.dtype}, not {dtype}")
+    require(isinstance(t, torch.Tensor) and t.get_device() == h.device, lambda: f"{what}: not a tensor of device {h.device}")
+    require(dtype is None or t.dtype == dtype, lambda: f"{what}: {t.dtype}, not {dtype}")
 
 
 class Rotary:
@@ -109,27 +109,30 @@ class Rotary:
         low, high, length = [given[n] for n in names] or (0.0, 0.0, 0)
         table, factor = (C.c_uint64 * max(1, rot_dim // 2))(), C.c_float()
         check(lib().mx230_rotary_table(table, C.byref(factor), rot_dim, theta, kind, given.get("factor", 1.0), low, high, length))
-        self.rot_dim, self.interleaved, self.factor = rot_dim, interleaved, factor.value
+        self.rot_dim, self.interleaved, self.factor = rot_dim, int(interleaved), factor.value
         # (torch has no arithmetic on unsigned 64-bit words; only the bits matter)
         self.turns = torch.frombuffer(table, dtype=torch.int64).to(device)
+        self._addr, self._device = self.turns.data_ptr(), self.turns.get_device()
 
 
 def rotary(h: Handle, out, x, pos, plan: Rotary, inverse=False, stream=None):
     """Rotates the first plan.rot_dim values of every head of x [n_rows][n_head][head_dim] (fp32, fp16 or bf16; any strides between
     rows and heads) into `out` of the same shape, which may be x.  `pos`: an int32 tensor [n_rows], or the first row's position.
     `inverse` turns back; it takes the gradient of `out` to that of x."""
-    require(x.dim() == 3 and out.shape == x.shape, f"rotary: x {tuple(x.shape)}, out {tuple(out.shape)}")
-    require(x.dtype in _DTYPES, f"rotary: {x.dtype}")
-    on_device(h, "rotary: x", x), on_device(h, "rotary: out", out, x.dtype), on_device(h, "rotary: plan", plan.turns)
-    n, heads, dim = x.shape
-    require(dim == 1 or (x.stride(2) == 1 and out.stride(2) == 1), "rotary: the values of a head must be contiguous")
-    dyn = isinstance(pos, torch.Tensor)
-    if dyn:
+    shape, dtype, dev = x.shape, x.dtype, h.device
+    require(len(shape) == 3 and out.shape == shape, lambda: f"rotary: x {tuple(x.shape)}, out {tuple(out.shape)}")
+    require(dtype in _DTYPES and out.dtype == dtype, lambda: f"rotary: x {x.dtype}, out {out.dtype}")
+    require(x.get_device() == dev and out.get_device() == dev and plan._device == dev, lambda: f"rotary: x, out or plan not on device {dev}")
+    n, heads, dim = shape
+    (xr, xh, xd), (outr, outh, outd) = x.stride(), out.stride()
+    require(dim == 1 or (xd == 1 and outd == 1), "rotary: the values of a head must be contiguous")
+    at, first = None, pos
+    if isinstance(pos, torch.Tensor):
         on_device(h, "rotary: pos", pos, torch.int32)
-        require(pos.shape == (n,) and (n < 2 or pos.stride(0) == 1), f"rotary: positions {tuple(pos.shape)} for {n} rows")
-    check(lib().mx230_rotary(h._h, stream_ptr(stream, h.device), addr(out), addr(x), _DTYPES[x.dtype], addr(pos) if dyn else None,
-                             0 if dyn else pos, addr(plan.turns), plan.factor, n, heads, dim, plan.rot_dim, int(plan.interleaved),
-                             int(inverse), x.stride(0), x.stride(1), out.stride(0), out.stride(1)))
+        require(pos.shape == (n,) and (n < 2 or pos.stride(0) == 1), lambda: f"rotary: positions {tuple(pos.shape)} for {n} rows")
+        at, first = pos.data_ptr(), 0
+    check(lib().mx230_rotary(h._h, raw_stream(stream, dev), out.data_ptr(), x.data_ptr(), _DTYPES[dtype], at, first, plan._addr, plan.factor,
+                             n, heads, dim, plan.rot_dim, plan.interleaved, inverse, xr, xh, outr, outh))
 
 
 # ---------------------------------------------------------------- fp32 KV write
@@ -442,6 +445,7 @@ class Int4Weights:
 
     def __init__(self, packed, n_in: int, n_out: int, group: int):
         self.packed, self.n_in, self.n_out, self.group = packed, n_in, n_out, group
+        self._addr, self._device = packed.data_ptr(), packed.get_device()
 
     def nbytes(self) -> int:
         return self.packed.numel()
@@ -456,36 +460,41 @@ def pack_int4(h: Handle, codes, scales, zeros=None, group: int | None = None, st
     groups = scales.shape[0]
     if group is None:
         fits = [g for g in (32, 64, 128, 256, 512, 1024) if -(-n_in // g) == groups]
-        require(len(fits) == 1, f"pack_int4: {groups} groups of {n_in} inputs: give the group")
+        require(len(fits) == 1, lambda: f"pack_int4: {groups} groups of {n_in} inputs: give the group")
         group = fits[0]
-    require(group > 0 and -(-n_in // group) == groups, f"pack_int4: {groups} groups of {group} for {n_in} inputs")
+    require(group > 0 and -(-n_in // group) == groups, lambda: f"pack_int4: {groups} groups of {group} for {n_in} inputs")
     on_device(h, "pack_int4: codes", codes, torch.uint8), on_device(h, "pack_int4: scales", scales, torch.float16)
     require(codes.is_contiguous() and scales.is_contiguous(), "pack_int4: codes and scales must be contiguous")
     if zeros is not None:
         on_device(h, "pack_int4: zeros", zeros, torch.uint8)
         require(zeros.shape == scales.shape and zeros.is_contiguous(), "pack_int4: zeros must be contiguous, of the scales' shape")
     packed = torch.empty(lib().mx230_int4_bytes(n_in, n_out, group), dtype=torch.uint8, device=codes.device)
-    check(lib().mx230_pack_int4(h._h, stream_ptr(stream, h.device), addr(packed), addr(codes), addr(scales), addr(zeros), n_in, n_out, group))
+    check(lib().mx230_pack_int4(h._h, raw_stream(stream, h.device), packed.data_ptr(), addr(codes), addr(scales), addr(zeros), n_in, n_out, group))
     return Int4Weights(packed, n_in, n_out, group)
 
 
 def gemv_int4(h: Handle, y, x, w: Int4Weights, b=None, add=None, stream=None):
     """y = x W + b + add over 4-bit weights: x [n_in] or [n_rows][n_in], y and add (which may be y: the residual row) with n_out.
     A row's bits do not depend on the rows beside it."""
-    x2, y2 = (x, y) if x.dim() == 2 else (x[None], y[None])
-    a2 = add if add is None or add.dim() == 2 else add[None]
-    n = x2.shape[0]
-    require(x.dim() in (1, 2) and y.dim() == x.dim() and x2.shape[1] == w.n_in and y2.shape == (n, w.n_out),
-            f"gemv_int4: x {tuple(x.shape)}, y {tuple(y.shape)}, weights [{w.n_in}][{w.n_out}]")
-    require(a2 is None or a2.shape == y2.shape, "gemv_int4: add must have the shape of y")
-    for what, t in (("x", x2), ("y", y2), ("add", a2), ("bias", b)):
-        if t is not None:
-            on_device(h, "gemv_int4: " + what, t, torch.float32)
-            require(t.shape[-1] < 2 or t.stride(-1) == 1, f"gemv_int4: the values of a row of {what} must be contiguous")
-    on_device(h, "gemv_int4: weights", w.packed)
-    require(b is None or b.shape == (w.n_out,), "gemv_int4: bias must be [n_out]")
-    check(lib().mx230_gemv_int4(h._h, stream_ptr(stream, h.device), addr(y2), addr(x2), addr(w.packed), addr(b), addr(a2), n, w.n_in, w.n_out,
-                                w.group, x2.stride(0), y2.stride(0), 0 if a2 is None else a2.stride(0)))
+    xs, ys, dev, f32 = x.shape, y.shape, h.device, torch.float32
+    rows, n_out = xs[:-1], w.n_out
+    require(0 < len(xs) < 3 and xs[-1] == w.n_in and ys == (*rows, n_out), lambda: f"gemv_int4: x {tuple(xs)}, y {tuple(ys)}, weights [{w.n_in}][{n_out}]")
+    require(x.dtype == f32 and y.dtype == f32 and x.get_device() == dev and y.get_device() == dev and w._device == dev,
+            lambda: f"gemv_int4: x {x.dtype}, y {y.dtype} must be fp32, they and the weights on device {dev}")
+    xd, yd = x.stride(), y.stride()
+    require((w.n_in == 1 or xd[-1] == 1) and (n_out == 1 or yd[-1] == 1), "gemv_int4: the values of a row must be contiguous")
+    bias = plus = None
+    ad = (0,)
+    if b is not None:
+        on_device(h, "gemv_int4: bias", b, f32)
+        require(b.shape == (n_out,) and (n_out == 1 or b.stride(0) == 1), "gemv_int4: bias must be [n_out], contiguous")
+        bias = b.data_ptr()
+    if add is not None:
+        on_device(h, "gemv_int4: add", add, f32)
+        ad, plus = add.stride(), add.data_ptr()
+        require(add.shape == ys and (n_out == 1 or ad[-1] == 1), "gemv_int4: add must have the shape of y, its rows contiguous")
+    check(lib().mx230_gemv_int4(h._h, raw_stream(stream, dev), y.data_ptr(), x.data_ptr(), w._addr, bias, plus, rows[0] if rows else 1, w.n_in,
+                                n_out, w.group, xd[0], yd[0], ad[0]))
 
 
 def qkv_rope_kvwrite(h: Handle, qkv, x, w, b, pos, c: KvCache, n_head, n_kv_head, theta, pg: Paging | None = None,

@@ -20,8 +20,8 @@ import numpy as np
 
 import torch
 
-from ._lib import addr, check, lib, require
-from .common import Handle, stream_ptr
+from ._lib import check, lib, require
+from .common import Handle, raw_stream
 from .llm_attention import _DTYPES, on_device
 from .paging import KvPool
 
@@ -109,24 +109,24 @@ def sample(h: Handle, token, logits, u, temperature=1.0, top_k=0, top_p=1.0, min
     is a number or a tensor [n] (fp32, top_k int32).  include/mx230_attn.h has the definition at mx230_sample: entries in falling
     order, the first top_k of them, of those the shortest prefix with top_p of their weight, cut at min_p times the largest
     weight; the token is where the running weight passes u.  -1 where a row is masked throughout."""
-    require(logits.dim() == 2 and logits.dtype in _DTYPES, f"sample: logits {tuple(logits.shape)} of {logits.dtype}")
-    n, vocab = logits.shape
+    dev, dtype = h.device, _DTYPES.get(logits.dtype)
+    require(logits.dim() == 2 and dtype is not None, lambda: f"sample: logits {tuple(logits.shape)} of {logits.dtype}")
+    (n, vocab), (row, one) = logits.shape, logits.stride()
     on_device(h, "sample: logits", logits)
-    require(vocab < 2 or logits.stride(1) == 1, "sample: the logits of a row must be contiguous")
+    require(vocab < 2 or one == 1, "sample: the logits of a row must be contiguous")
 
-    def vector(what, t, dtype):
-        on_device(h, "sample: " + what, t, dtype)
-        require(t.shape == (n,) and (n < 2 or t.stride(0) == 1), f"sample: {what} {tuple(t.shape)} for {n} rows")
-        return addr(t)
+    def vector(what, t, ty):
+        on_device(h, what, t, ty)
+        require(t.shape == (n,) and (n < 2 or t.stride(0) == 1), lambda: f"{what} {tuple(t.shape)} for {n} rows")
+        return t.data_ptr()
 
-    def setting(what, v, dtype, number):
-        return (number(0), vector(what, v, dtype)) if isinstance(v, torch.Tensor) else (number(v), None)
-
-    check(lib().mx230_sample(h._h, stream_ptr(stream, h.device), vector("token", token, torch.int32),
-                             None if prob is None else vector("prob", prob, torch.float32), addr(logits), _DTYPES[logits.dtype], n, vocab,
-                             logits.stride(0), vector("u", u, torch.float32), *setting("temperature", temperature, torch.float32, float),
-                             *setting("top_k", top_k, torch.int32, int), *setting("top_p", top_p, torch.float32, float),
-                             *setting("min_p", min_p, torch.float32, float)))
+    t, ts = (0.0, vector("sample: temperature", temperature, torch.float32)) if isinstance(temperature, torch.Tensor) else (temperature, None)
+    k, ks = (0, vector("sample: top_k", top_k, torch.int32)) if isinstance(top_k, torch.Tensor) else (top_k, None)
+    p, ps = (0.0, vector("sample: top_p", top_p, torch.float32)) if isinstance(top_p, torch.Tensor) else (top_p, None)
+    m, ms = (0.0, vector("sample: min_p", min_p, torch.float32)) if isinstance(min_p, torch.Tensor) else (min_p, None)
+    check(lib().mx230_sample(h._h, raw_stream(stream, dev), vector("sample: token", token, torch.int32),
+                             None if prob is None else vector("sample: prob", prob, torch.float32), logits.data_ptr(), dtype, n, vocab, row,
+                             vector("sample: u", u, torch.float32), t, ts, k, ks, p, ps, m, ms))
 
 
 class Sampler:
@@ -150,7 +150,7 @@ class Sampler:
                dev([q.top_p for *_, q in rows], torch.float32), dev([q.min_p for *_, q in rows], torch.float32))
         out = token.tolist()
         for (r, t, _), tok in zip(rows, out):
-            require(tok >= 0, f"request {r}: every logit of token {t} is masked")
+            require(tok >= 0, lambda: f"request {r}: every logit of token {t} is masked")
         return out
 
 

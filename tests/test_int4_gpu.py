@@ -1,9 +1,10 @@
 """Products with 4-bit weights against the same sums in 64 bits.
 
-Tolerance, against the sum of the products' magnitudes M = sum |x s (q - z)|.  Weights and both parts of x are exact in fp16; x is
-off by 2^-24 |x| (or 2^-40 of the largest of its 64).  The tensor core adds the 16 products of a step with at most 17 truncations
-of 2^-24 M: 2^-20 M with the steps of a tile.  A tile's sum times its scale rounds and is added: 2^-23 M a tile, for at most
-the tiles of a slice, and six pairwise sums.  Then the bias and what is added, half a step each.
+Tolerance, against M = sum |x| s (q + z), as the sums of x q and of x are taken apart.  Codes and both parts of x are exact in fp16; x is off by
+2^-24 |x|, or by 2^-35 of the largest of its 64.  The tensor core adds the 16 products of a step with at most 17 truncations of 2^-24 M:
+2^-20 M with the steps of a tile.  A tile's sum of x: 19 rounded additions, 2^-20 M.  The difference, its scale and the
+addition round: 2^-22 M a tile, for at most the tiles of a slice, and six pairwise sums.  Then the bias and what is added, half a
+step each.
 """
 import math
 
@@ -25,19 +26,20 @@ def weights(n_in, n_out, group, zeros, seed):
     return codes, scales, z
 
 
-def dense(codes, scales, z, group):
-    at = torch.arange(codes.shape[0], device="cuda") // group
-    return (codes.double() - (8.0 if z is None else z.double()[at])) * scales.double()[at]
+class Dense:
+    """s (q - z) and s (q + z) in 64 bits."""
 
+    def __init__(self, codes, scales, z, group):
+        at = torch.arange(codes.shape[0], device="cuda") // group
+        zero, s = 8.0 if z is None else z.double()[at], scales.double()[at]
+        self.w, self.mag = (codes.double() - zero) * s, (codes.double() + zero) * s
 
-def limit(x, w, want, *more):
-    m = x.double().abs() @ w.abs()
-    tiles = -(-w.shape[0] // 64)
-    # (2^-40 of the largest x of a tile against the tile's M: covered where the tile's largest product is in M; 1e-12 for the rest)
-    out = m * (2.0 ** -20 + (tiles + 8) * 2.0 ** -23) + want.abs() * 2.0 ** -23 + 1e-30
-    for t in more:
-        out = out + t.double().abs() * 2.0 ** -23
-    return out + x.double().abs().amax(1, keepdim=True) * w.abs().amax(0) * w.shape[0] * 2.0 ** -40
+    def limit(self, x, want, *more):
+        tiles, x = -(-self.w.shape[0] // 64), x.double().abs()
+        out = x @ self.mag * (2.0 ** -19 + (tiles + 8) * 2.0 ** -22) + want.abs() * 2.0 ** -23 + 1e-30
+        for t in more:
+            out = out + t.double().abs() * 2.0 ** -23
+        return out + x.amax(1, keepdim=True) * self.mag.amax(0) * self.w.shape[0] * 2.0 ** -35
 
 
 def check(got, want, lim, what):
@@ -54,14 +56,14 @@ def test_matches_the_sums(handle, n_in, n_out, rows, group, zeros):
     w = la.pack_int4(handle, codes, scales, z, group=group)
     g = torch.Generator(device="cuda").manual_seed(rows)
     x, b, old = (torch.randn(*s, device="cuda", generator=g) for s in ((rows, n_in), (n_out,), (rows, n_out)))
-    d = dense(codes, scales, z, group)
-    want = x.double() @ d
+    d = Dense(codes, scales, z, group)
+    want = x.double() @ d.w
     y = torch.full((rows, n_out), math.nan, device="cuda")
     la.gemv_int4(handle, y, x, w)
-    check(y, want, limit(x, d, want), "plain")
+    check(y, want, d.limit(x, want), "plain")
     la.gemv_int4(handle, y, x, w, b, add=old)
     want = want + b.double() + old.double()
-    check(y, want, limit(x, d, want, b, old), "bias and add")
+    check(y, want, d.limit(x, want, b, old), "bias and add")
     acc = old.clone()
     la.gemv_int4(handle, acc, x, w, b, add=acc)
     assert torch.equal(acc, y), "added in place"
@@ -87,7 +89,7 @@ def test_ranges_of_x(handle, scale):
     n_in, n_out = 640, 200
     codes, scales, z = weights(n_in, n_out, 64, True, 9)
     w = la.pack_int4(handle, codes, scales, z)
-    d = dense(codes, scales, z, 64)
+    d = Dense(codes, scales, z, 64)
     g = torch.Generator(device="cuda").manual_seed(1)
     x = torch.randn(6, n_in, device="cuda", generator=g) * scale
     x[1] = 0.0
@@ -97,15 +99,15 @@ def test_ranges_of_x(handle, scale):
     x[5, 1:] = 0.0
     y = torch.empty(6, n_out, device="cuda")
     la.gemv_int4(handle, y, x, w)
-    want = x.double() @ d
-    check(y, want, limit(x, d, want), scale)
+    want = x.double() @ d.w
+    check(y, want, d.limit(x, want), scale)
     assert (y[1] == 0).all()
 
 
 def test_infinities_and_nan_stay_in_their_row(handle):
     codes, scales, _ = weights(256, 64, 64, False, 2)
     w = la.pack_int4(handle, codes, scales)
-    d = dense(codes, scales, None, 64)
+    d = Dense(codes, scales, None, 64)
     x = torch.randn(7, 256, device="cuda")
     clean = torch.empty(7, 64, device="cuda")
     la.gemv_int4(handle, clean, x, w)
@@ -115,7 +117,7 @@ def test_infinities_and_nan_stay_in_their_row(handle):
     assert torch.equal(y[[0, 1, 3, 6]], clean[[0, 1, 3, 6]])
     assert torch.isnan(y[2]).all()
     for r, k, v in ((4, 3, math.inf), (5, 255, -math.inf)):
-        want = v * d[k]   # NaN where the weight is 0
+        want = v * d.w[k]   # NaN where the weight is 0
         assert torch.equal(torch.isnan(want), torch.isnan(y[r])) and torch.equal(want[~torch.isnan(want)], y[r].double()[~torch.isnan(want)])
 
 
@@ -123,7 +125,7 @@ def test_strides_and_what_lies_beside(handle):
     n_in, n_out, rows = 200, 50, 6
     codes, scales, z = weights(n_in, n_out, 64, True, 3)
     w = la.pack_int4(handle, codes, scales, z)
-    d = dense(codes, scales, z, 64)
+    d = Dense(codes, scales, z, 64)
     for off, wide in ((0, 208), (1, 203), (3, 211)):
         store = torch.randn(rows * wide + 8, device="cuda")
         x = store[off:off + rows * wide].view(rows, wide)[:, :n_in]
@@ -131,8 +133,8 @@ def test_strides_and_what_lies_beside(handle):
         y = whole[1:rows + 1, 3:3 + n_out]
         add = torch.randn(rows, n_out + 1, device="cuda")[:, 1:]
         la.gemv_int4(handle, y, x, w, add=add)
-        want = x.double() @ d + add.double()
-        check(y, want, limit(x, d, want, add), off)
+        want = x.double() @ d.w + add.double()
+        check(y, want, d.limit(x, want, add), off)
         inside = torch.zeros_like(whole, dtype=torch.bool)
         inside[1:rows + 1, 3:3 + n_out] = True
         assert (whole[~inside] == 5).all()
@@ -152,9 +154,9 @@ def test_high_bits_of_codes_and_large_zeros(handle):
     la.gemv_int4(handle, a, x, la.pack_int4(handle, codes, scales, z))
     la.gemv_int4(handle, b, x, la.pack_int4(handle, codes + 240, scales, z))
     assert torch.equal(a, b)
-    d = dense(codes, scales, z, 64)
-    want = x.double() @ d
-    check(a, want, limit(x, d, want), "zeros of 255")
+    d = Dense(codes, scales, z, 64)
+    want = x.double() @ d.w
+    check(a, want, d.limit(x, want), "zeros of 255")
 
 
 def test_captured_replayed_and_on_another_stream(handle):
