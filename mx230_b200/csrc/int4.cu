@@ -32,7 +32,7 @@ constexpr int W4_N = 16;          // outputs of a tile
 constexpr int W4_WARPS = 8;
 constexpr int W4_THREADS = W4_WARPS * 32;
 constexpr int W4_CLUSTER = 8;     // most CTAs whose sums are added through shared memory
-constexpr int W4_X_BYTES = 64 * 1024;   // of shared memory for rows, about
+constexpr int W4_X_BYTES = 32 * 1024;   // of shared memory for rows, about
 constexpr int SLICE_WARPS = 16, TWO_WARPS = 16, KW_MOST = 8;
 
 struct Int4Params {
@@ -82,12 +82,12 @@ __global__ void pack_int4_kernel(uint4 *codes_out, uint32_t *sz_out, const uint8
     }
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// weights: read once, past the first cache
+__device__ __forceinline__ uint4 ld_stream(const uint4 *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ uint32_t h2_u(__half2 v) { return *(uint32_t *)&v; }
 __device__ __forceinline__ __half2 u_h2(uint32_t v) { return *(__half2 *)&v; }
@@ -98,10 +98,16 @@ __device__ __forceinline__ void pairs8(uint32_t w, uint32_t (&a)[4]) {
     a[0] = w & 0x000F000Fu, a[1] = w & 0x00F000F0u, a[2] = v & 0x000F000Fu, a[3] = v & 0x00F000F0u;
 }
 
+// c = a b + c, or a b
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // pairwise sum of n (a power of two, at most 8) values `step` apart
@@ -115,15 +121,12 @@ __device__ __forceinline__ float tree_sum(const float *p, int n, int step) {
 }
 
 // NT: column tiles of four rows.  T: output tiles of a warp.  G32: groups of 32 inputs (else a multiple of 64).
-// Shared memory: ring [8 warps][STAGES][T][512 + 64 or 128], sums [8 warps][T * NT * 64], in the first CTA of a cluster also the
-// other CTAs' sums; per (slice, tile, row) {2^-e, 2^(e - 24) sum x, or that of either half}; 32 bytes of zeros; rows
-// [kw][xq][NT][lanes][8 words].
-constexpr int STAGES = 6;
+// Shared memory: sums [8 warps][T * NT * 64], in the first CTA of a cluster also the other CTAs' sums; per (slice, tile, row)
+// {2^-e, 2^(e - 24) sum x, or that of either half}; 32 bytes of zeros; rows [kw][xq][NT][lanes][8 words].
+// DEPTH tiles of every output tile are on their way to a warp's registers.
+constexpr int DEPTH = 4;
 template <int NT, int T, bool G32>
 struct Int4Smem {
-    static constexpr int SZ = G32 ? 128 : 64;               // bytes of (s, z) of a tile
-    static constexpr int STAGE = T * (512 + SZ);
-    static constexpr int RING = W4_WARPS * STAGES * STAGE;
     static constexpr int SUMS = T * NT * 64;                // floats of a warp
 };
 
@@ -137,8 +140,7 @@ __global__ void __launch_bounds__(W4_THREADS) gemv_int4_kernel(const Int4Params 
     const int row0 = blockIdx.y * (4 * NT), rows = min(4 * NT, P.n_rows - row0);
     const int rt = NT == 1 ? rows : 4;                      // rows of a column tile that are there at all
     const int x_lanes = 8 * rt;
-    unsigned char *ring = smem + warp * (STAGES * S::STAGE);
-    float *sums = (float *)(smem + S::RING);                // [8][SUMS]
+    float *sums = (float *)smem;                            // [8][SUMS]
     float *parts = sums + W4_WARPS * S::SUMS;               // [C][tg][SUMS], first CTA
     float4 *xrow = (float4 *)(parts + (C > 1 ? C * tg * S::SUMS : 0));   // [kw][xq][NT * 4]
     uint4 *zeros = (uint4 *)(xrow + kw * P.xq * NT * 4);    // 32 bytes
@@ -154,32 +156,49 @@ __global__ void __launch_bounds__(W4_THREADS) gemv_int4_kernel(const Int4Params 
     const int t_first = (grp * tg + warp / kw) * T;
     const int k0 = (int)((long long)P.k_tiles * slice / n_slices), k1 = (int)((long long)P.k_tiles * (slice + 1) / n_slices);
     // what is requested next: tile kq, with its group gq of which left_q tiles are still to come
-    constexpr int LPT = S::SZ / 16;                         // lanes that fetch (s, z) of a tile
-    const bool any = t_first < P.n_tiles, szl = lane < T * LPT;
+    const bool any = t_first < P.n_tiles;
     const int per_group = G32 ? 1 : P.group / W4_K;
     const uint4 *code_q[T];
+    const uint32_t *sz_q[T];
 #pragma unroll
-    for (int t = 0; t < T; ++t) code_q[t] = P.codes + ((size_t)min(t_first + t, P.n_tiles - 1) * P.k_tiles + k0) * 32 + lane;
-    const uint32_t *sz_row = P.sz + (size_t)min(t_first + lane / LPT, P.n_tiles - 1) * P.groups * 16 + (lane & 3) * 4;
-    int kq = k0, gq = G32 ? 2 * k0 + ((lane & (LPT - 1)) >> 2) : k0 / per_group, left_q = G32 ? 1 : per_group - (k0 - gq * per_group);
-    auto request = [&](int stage) {
+    for (int t = 0; t < T; ++t) {
+        const int nt = min(t_first + t, P.n_tiles - 1);
+        code_q[t] = P.codes + ((size_t)nt * P.k_tiles + k0) * 32 + lane;
+        sz_q[t] = P.sz + ((size_t)nt * P.groups + (G32 ? 2 * k0 : k0 / per_group)) * 16 + g;
+    }
+    int kq = k0, left_q = G32 ? 1 : per_group - k0 % per_group;
+    uint4 codes[DEPTH][T];
+    uint32_t sz[DEPTH][T][G32 ? 4 : 2];
+    auto request = [&](int d) {
         if (any && kq < k1) {
-            const uint32_t dst = mx::smem_u32(ring + stage * S::STAGE) + lane * 16;
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                cp_async16(dst + t * 512, code_q[t]);
+                codes[d][t] = ld_stream(code_q[t]);
+                sz[d][t][0] = __ldg(sz_q[t]), sz[d][t][1] = __ldg(sz_q[t] + 8);
+                if (G32) {   // (a second group behind the last one: the padding of the inputs, whatever it is multiplied by is 0)
+                    const int more = 2 * kq + 1 < P.groups ? 16 : 0;
+                    sz[d][t][2] = __ldg(sz_q[t] + more), sz[d][t][3] = __ldg(sz_q[t] + more + 8);
+                }
                 code_q[t] += 32;
             }
-            // (a second group of 32 behind the last one: the padding of the inputs, whatever it is multiplied by is 0)
-            if (szl) cp_async16(dst + T * 512, sz_row + (size_t)(G32 ? min(gq, P.groups - 1) : gq) * 16);
-            if (G32) gq += 2;
-            else if (--left_q == 0) left_q = per_group, ++gq;
             ++kq;
+            if (--left_q == 0) {
+                left_q = per_group;
+#pragma unroll
+                for (int t = 0; t < T; ++t) sz_q[t] += G32 ? 32 : 16;
+            }
         }
-        cp_async_commit();
     };
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) request(s);
+    for (int d = 0; d < DEPTH; ++d) {
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            codes[d][t] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < (G32 ? 4 : 2); ++e) sz[d][t][e] = 0;
+        }
+        request(d);
+    }
 
     float total[T][NT][2];
 #pragma unroll
@@ -188,7 +207,6 @@ __global__ void __launch_bounds__(W4_THREADS) gemv_int4_kernel(const Int4Params 
         for (int n = 0; n < NT; ++n) total[t][n][0] = total[t][n][1] = 0.0f;
 
     const int most = (P.k_tiles + n_slices - 1) / n_slices;   // tiles of the longest slice
-    int stage = 0;
     for (int c0 = 0; c0 < most; c0 += P.xq) {
         if (c0) __syncthreads();
         // ---- rows of the next xq tiles of every slice: scaled, split, in the order of B's fragments ----
@@ -256,53 +274,48 @@ __global__ void __launch_bounds__(W4_THREADS) gemv_int4_kernel(const Int4Params 
         const uint4 *xp = has_x ? xf + ((size_t)ws * P.xq * NT * x_lanes + lane) * 2 : zeros;
         const float4 *rp = xrow + ws * P.xq * (NT * 4) + (NT == 1 ? min(j, rt - 1) : j);   // the row whose sums this lane gets
         const int x_step = has_x ? x_lanes * 2 : 0;
-        for (int kk = c0; kk < end; ++kk) {
-            cp_async_wait<STAGES - 2>();
-            __syncwarp();
-            const unsigned char *st = ring + stage * S::STAGE;
-            uint4 b[NT][2];
-            float4 xr[NT];
+        for (int k_ = c0; k_ < end; k_ += DEPTH)               // (xq is a multiple of DEPTH, or all)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                b[n][0] = xp[0], b[n][1] = xp[1];
-                xp += x_step;
-                xr[n] = rp[n * 4];
-            }
-            rp += NT * 4;
+            for (int d = 0; d < DEPTH; ++d) {
+                if (k_ + d >= end) break;
+                uint4 b[NT][2];
+                float4 xr[NT];
 #pragma unroll
-            for (int t = 0; t < T; ++t) {
-                const uint4 w = *(const uint4 *)(st + t * 512 + lane * 16);
-                float acc[NT][4];
+                for (int n = 0; n < NT; ++n) {
+                    b[n][0] = xp[0], b[n][1] = xp[1];
+                    xp += x_step;
+                    xr[n] = rp[n * 4];
+                }
+                rp += NT * 4;
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    uint32_t a0[4], a1[4];
-                    pairs8(hf ? w.y : w.x, a0);
-                    pairs8(hf ? w.w : w.z, a1);
-                    if (G32 || hf == 0)
+                for (int t = 0; t < T; ++t) {
+                    const uint4 w = codes[d][t];
+                    float acc[NT][4];
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma_f16(acc[n], a0[0], a1[0], a0[1], a1[1], b[n][hf].x, b[n][hf].y);
-                        mma_f16(acc[n], a0[2], a1[2], a0[3], a1[3], b[n][hf].z, b[n][hf].w);
-                    }
-                    if (G32 || hf == 1) {
-                        const uint32_t *sz = (const uint32_t *)(st + T * 512 + t * S::SZ + (G32 ? hf * 64 : 0));
-                        const float2 s0 = __half22float2(u_h2(sz[g])), s1 = __half22float2(u_h2(sz[g + 8]));
-                        const float m0 = s0.x * 0x1p24f, m1 = s1.x * 0x1p24f;
+                    for (int hf = 0; hf < 2; ++hf) {
+                        uint32_t a0[4], a1[4];
+                        pairs8(hf ? w.y : w.x, a0);
+                        pairs8(hf ? w.w : w.z, a1);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            const float xs = G32 && hf ? xr[n].z : xr[n].y;
-                            total[t][n][0] = fmaf(m0, fmaf(-s0.y, xs, acc[n][0] + acc[n][1]) * xr[n].x, total[t][n][0]);
-                            total[t][n][1] = fmaf(m1, fmaf(-s1.y, xs, acc[n][2] + acc[n][3]) * xr[n].x, total[t][n][1]);
+                            if (G32 || hf == 0) mma_f16_first(acc[n], a0[0], a1[0], a0[1], a1[1], b[n][hf].x, b[n][hf].y);
+                            else mma_f16(acc[n], a0[0], a1[0], a0[1], a1[1], b[n][hf].x, b[n][hf].y);
+                            mma_f16(acc[n], a0[2], a1[2], a0[3], a1[3], b[n][hf].z, b[n][hf].w);
+                        }
+                        if (G32 || hf == 1) {
+                            const float2 s0 = __half22float2(u_h2(sz[d][t][G32 ? 2 * hf : 0])), s1 = __half22float2(u_h2(sz[d][t][G32 ? 2 * hf + 1 : 1]));
+                            const float m0 = s0.x * 0x1p24f, m1 = s1.x * 0x1p24f;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                const float xs = G32 && hf ? xr[n].z : xr[n].y;
+                                total[t][n][0] = fmaf(m0, fmaf(-s0.y, xs, acc[n][0] + acc[n][1]) * xr[n].x, total[t][n][0]);
+                                total[t][n][1] = fmaf(m1, fmaf(-s1.y, xs, acc[n][2] + acc[n][3]) * xr[n].x, total[t][n][1]);
+                            }
                         }
                     }
                 }
+                request(d);
             }
-            __syncwarp();
-            request(stage == 0 ? STAGES - 1 : stage - 1);
-            stage = stage == STAGES - 1 ? 0 : stage + 1;
-        }
     }
     // ---- slices of the CTA, then of the cluster, pairwise ----
 #pragma unroll
@@ -342,9 +355,8 @@ int launch_int4(mx230_handle *h, cudaStream_t st, Int4Params P) {
     const int most = (P.k_tiles + n_slices - 1) / n_slices;
     const int per_tile = P.kw * NT * (32 * (NT == 1 ? 8 * (P.n_rows < 4 ? P.n_rows : 4) : 32) + 64);
     P.xq = W4_X_BYTES / per_tile;
-    if (P.xq > most) P.xq = most;
-    if (P.xq < 1) P.xq = 1;
-    const size_t sm = (size_t)S::RING + (size_t)(W4_WARPS + (C > 1 ? C * tg : 0)) * S::SUMS * 4 + 32 + (size_t)P.xq * per_tile;
+    P.xq = P.xq >= most ? most : P.xq < DEPTH ? DEPTH : P.xq / DEPTH * DEPTH;
+    const size_t sm = (size_t)(W4_WARPS + (C > 1 ? C * tg : 0)) * S::SUMS * 4 + 32 + (size_t)P.xq * per_tile;
     MX_SMEM_ATTR_ONCE(h->device, (gemv_int4_kernel<NT, T, G32>), 227 * 1024);
     const long long groups_n = (P.n_tiles + (long long)tg * T - 1) / ((long long)tg * T);
     const dim3 grid((unsigned)(groups_n * C), (unsigned)((P.n_rows + 4 * NT - 1) / (4 * NT)));
