@@ -59,19 +59,22 @@ struct Window {
 };
 
 struct alignas(16) Shared {
-    unsigned cnt[SM_BINS], lo[SM_BINS], hi[SM_BINS];   // this CTA's histogram: counts, masses in two words
+    uint2 mass[SM_BINS];         // this CTA's histogram: masses in two words, counts
+    unsigned cnt[SM_BINS];
     // first CTA: running counts and masses over the first histogram's intervals
-    u64 run_mass[SM_BINS];
     unsigned run_cnt[SM_BINS];
+    u64 run_mass[SM_BINS];
     // a list's entries of this CTA, and of all (first CTA); running masses of the sorted list; a later histogram's running sums
     u64 mine[SM_LIST], all[SM_LIST];
     double table[256];
     u64 scan[SM_WARPS];
+    unsigned scan_cnt[SM_WARPS];
     u64 slot_a[SM_CLUSTER], slot_b[SM_CLUSTER];        // a word of each CTA
     float warp_a[SM_WARPS], warp_b[SM_WARPS];
-    Window w[2];             // the one in force and the next: a CTA may still look at one while the first CTA writes the other
-    u64 found_a, found_b, found_c;
-    unsigned n_mine, n_all;
+    Window w[2];                 // the one in force and the next: a CTA may still look at one while the first CTA writes the other
+    u64 low, high;
+    int found[4];                // what was found, in turns: the answer before last is free
+    unsigned n_mine, n_all, at_all;
 };
 
 __device__ __forceinline__ void cluster_sync() {   // (by whole warps)
@@ -85,6 +88,11 @@ __device__ __forceinline__ uint32_t ld_cluster32(uint32_t addr) {
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
 }
+__device__ __forceinline__ u64 ld_cluster64(uint32_t addr) {
+    u64 v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ uint32_t add_cluster(uint32_t addr, uint32_t v) {
     uint32_t old;
     asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(v) : "memory");
@@ -96,8 +104,8 @@ template <> __device__ __forceinline__ float logit(float v) { return v; }
 template <> __device__ __forceinline__ float logit(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float logit(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// as it is kept: NaN is masked, infinity the largest number, -0 is 0
-__device__ __forceinline__ float kept_logit(float l) { return l == l ? fminf(l, FLT_MAX) + 0.0f : -INFINITY; }
+// as it is kept: NaN is masked, infinity the largest number
+__device__ __forceinline__ float kept_logit(float l) { return l == l ? fminf(l, FLT_MAX) : -INFINITY; }
 
 // whole numbers in the order of the floats, and back
 __device__ __forceinline__ uint32_t order_key(float l) {
@@ -106,11 +114,9 @@ __device__ __forceinline__ uint32_t order_key(float l) {
 }
 __device__ __forceinline__ float key_float(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k); }
 
-// 2^(j / 256), j of a table, times the polynomial of 2^r for |r| <= 1/512
-__device__ __forceinline__ double weight(float l, float m, double log2e_t, const double *table) {
-    if (l == m) return 1.0;
-    const double x = ((double)l - (double)m) * log2e_t;
-    if (!(x > -42.0)) return 0.0;
+// 2^(j / 256), j of a table, times the polynomial of 2^r for |r| <= 1/512; at most 42 octaves below 1, exactly 1 for l = m
+__device__ __forceinline__ double weight(float l, double m, double log2e_t, const double *table) {
+    const double x = ((double)l - m) * log2e_t;
     const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's last bits are the rounded whole number
     const double t = fma(x, 256.0, magic);
     const int n = __double2loint(t);
@@ -127,63 +133,94 @@ __device__ __forceinline__ u64 to_mass(double w) {   // (ties cannot be: no weig
     return (u64)__double_as_longlong(fma(w, SM_MASS, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
 }
 
-// interval of max - l; SM_BINS and above: no weight.  Monotone in l: a difference, a product and a sum, each rounded.
-__device__ __forceinline__ int interval(float l, float m, float scale) {
-    if (l == -INFINITY) return SM_BINS;
-    return (int)(__float_as_uint(fminf((m - l) * scale, (float)SM_BINS) + 8388608.0f) & 0x7FFFFFu);
+// interval of max - l; SM_BINS: no weight, or masked (an infinite difference, or NaN where the scale is 0).  Monotone in l: a
+// difference, a product and a sum, each rounded.
+__device__ __forceinline__ unsigned interval(float l, float m, float scale) {
+    return __float_as_uint(fminf((m - l) * scale, (float)SM_BINS) + 8388608.0f) & 0x7FFFFFu;
 }
 
-// inclusive sums over the block, in the order of the threads
-__device__ __forceinline__ u64 block_scan(u64 v, u64 *scratch) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// running sums of n counts and masses (n <= 2 * SM_THREADS), two a thread, in place; counts may be null
+__device__ __forceinline__ void running_sums(unsigned *cnt, u64 *mass, int n, Shared &S) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = 2 * threadIdx.x;
+    const u64 m0 = i < n ? mass[i] : 0, m1 = i + 1 < n ? mass[i + 1] : 0;
+    const unsigned c0 = cnt && i < n ? cnt[i] : 0, c1 = cnt && i + 1 < n ? cnt[i + 1] : 0;
+    u64 m = m0 + m1;
+    unsigned c = c0 + c1;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const u64 up = __shfl_up_sync(0xFFFFFFFFu, v, o);
-        if (lane >= o) v += up;
+        const u64 mu = __shfl_up_sync(0xFFFFFFFFu, m, o);
+        const unsigned cu = __shfl_up_sync(0xFFFFFFFFu, c, o);
+        if (lane >= o) m += mu, c += cu;
+    }
+    if (lane == 31) S.scan[warp] = m, S.scan_cnt[warp] = c;
+    __syncthreads();
+    // (the sums of the warps in front: a lane takes one, then all are added)
+    u64 before = lane < warp ? S.scan[lane] : 0;
+    unsigned cb = lane < warp ? S.scan_cnt[lane] : 0;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+        before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
+        cb += __shfl_xor_sync(0xFFFFFFFFu, cb, o);
+    }
+    m += __shfl_sync(0xFFFFFFFFu, before, 0), c += __shfl_sync(0xFFFFFFFFu, cb, 0);
+    if (i < n) {
+        mass[i] = m - m1;
+        if (cnt) cnt[i] = c - c1;
+    }
+    if (i + 1 < n) {
+        mass[i + 1] = m;
+        if (cnt) cnt[i + 1] = c;
     }
     __syncthreads();
-    if (lane == 31) scratch[warp] = v;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) v += scratch[w];
-    return v;
 }
 
-// running sums of n values (n <= 2 * SM_THREADS), two a thread, into out
-template <typename In, typename Out>
-__device__ __forceinline__ void running_sums(const In *in, Out *out, int n, u64 *scratch) {
-    const int i = 2 * threadIdx.x;
-    const u64 a = i < n ? in[i] : 0, b = i + 1 < n ? in[i + 1] : 0;
-    const u64 s = block_scan(a + b, scratch);   // (its barriers stand between the reads and the writes)
-    if (i < n) out[i] = (Out)(s - b);
-    if (i + 1 < n) out[i + 1] = (Out)s;
-    __syncthreads();
-}
-
-// first index whose running sum exceeds t, n where none does; to be read behind the barrier
+// first index whose running sum exceeds t (there is one)
 template <typename R>
-__device__ __forceinline__ int first_over(const R *run, int n, u64 t, u64 *found) {
-    __syncthreads();
-    if (threadIdx.x == 0) *found = (u64)n;
-    __syncthreads();
+__device__ __forceinline__ int first_over(const R *run, int n, u64 t, int *found) {
     for (int i = threadIdx.x; i < n; i += SM_THREADS)
-        if ((u64)run[i] > t && (i == 0 || (u64)run[i - 1] <= t)) *found = (u64)i;
+        if ((u64)run[i] > t && (i == 0 || (u64)run[i - 1] <= t)) *found = i;
     __syncthreads();
-    return (int)*found;
+    return *found;
 }
 
-// sorts n2 (a power of two, at least 2) entries, largest first.  A warp's pairs of strides below 64 lie in 64 entries of its own.
-__device__ __forceinline__ void sort_down(u64 *v, int n2) {
-    for (int k = 2; k <= n2; k <<= 1)
+// Sorts n <= SM_LIST entries of v, largest first, by the bitonic network: a thread has one of each half; strides below 32 go
+// through the warp, larger ones through v and `other` in turns (a barrier each).
+__device__ __forceinline__ void sort_down(u64 *v, u64 *other, int n) {
+    static_assert(SM_LIST == 2 * SM_THREADS, "two entries a thread");
+    const int tid = threadIdx.x;
+    u64 e[2] = {tid < n ? v[tid] : 0, tid + SM_THREADS < n ? v[tid + SM_THREADS] : 0};
+    u64 *buf = other, *next = v;
+    for (int k = 2; k < 2 * n; k <<= 1) {
         for (int j = k >> 1; j > 0; j >>= 1) {
-            if (j >= 32) __syncthreads();
-            else __syncwarp();
-            for (int t = threadIdx.x; t < n2 / 2; t += SM_THREADS) {
-                const int i = 2 * (t & ~(j - 1)) | (t & (j - 1)), o = i | j;
-                const u64 a = v[i], b = v[o];
-                if ((a < b) == ((i & k) == 0)) v[i] = b, v[o] = a;
+            if (j == SM_THREADS) {
+                const u64 a = max(e[0], e[1]), b = min(e[0], e[1]);
+                e[0] = a, e[1] = b;
+                continue;
             }
-            if (j >= 32) __syncthreads();
+            u64 o[2];
+            if (j >= 32) {
+                buf[tid] = e[0];
+                if (n > SM_THREADS) buf[tid + SM_THREADS] = e[1];
+                __syncthreads();
+                o[0] = buf[tid ^ j];
+                o[1] = n > SM_THREADS ? buf[(tid ^ j) + SM_THREADS] : 0;
+                u64 *const b = buf;
+                buf = next, next = b;
+            } else {
+                o[0] = __shfl_xor_sync(0xFFFFFFFFu, e[0], j);
+                o[1] = n > SM_THREADS ? __shfl_xor_sync(0xFFFFFFFFu, e[1], j) : 0;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int i = tid + h * SM_THREADS;
+                const bool larger = ((i & j) == 0) == ((i & k) == 0);   // this place of the pair gets the larger one
+                e[h] = larger ? max(e[h], o[h]) : min(e[h], o[h]);
+            }
         }
+    }
+    __syncthreads();   // (the last exchange has been read)
+    if (tid < n) v[tid] = e[0];
+    if (tid + SM_THREADS < n) v[tid + SM_THREADS] = e[1];
     __syncthreads();
 }
 
@@ -213,32 +250,42 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
     const int v0 = (int)((long long)pieces * rank / C), v1 = (int)((long long)pieces * (rank + 1) / C);
     const int n = (v1 - v0) * VE, idx0 = v0 * VE - shift;         // data[i] is logit idx0 + i
     float hi = -INFINITY, lo = INFINITY;
-    for (int v = tid; v < v1 - v0; v += SM_THREADS) {
-        const int at = idx0 + v * VE;
-        float f[VE];
-        if (at >= 0 && at + VE <= P.vocab) {
-            const uint4 raw = *(const uint4 *)(src + at);
-            const T *e = (const T *)&raw;
+    constexpr int LOADS = 4;   // in flight
+    for (int v = tid; v < v1 - v0; v += LOADS * SM_THREADS) {
+        uint4 raw[LOADS];
 #pragma unroll
-            for (int i = 0; i < VE; ++i) f[i] = kept_logit(logit(e[i]));
-        } else {
-#pragma unroll
-            for (int i = 0; i < VE; ++i) f[i] = at + i >= 0 && at + i < P.vocab ? kept_logit(logit(src[at + i])) : -INFINITY;
+        for (int l = 0; l < LOADS; ++l) {
+            const int at = idx0 + (v + l * SM_THREADS) * VE;
+            if (v + l * SM_THREADS < v1 - v0 && at >= 0 && at + VE <= P.vocab) raw[l] = *(const uint4 *)(src + at);
         }
 #pragma unroll
-        for (int i = 0; i < VE; i += 4) *(float4 *)(data + v * VE + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+        for (int l = 0; l < LOADS; ++l) {
+            const int w = v + l * SM_THREADS, at = idx0 + w * VE;
+            if (w >= v1 - v0) break;
+            const T *e = (const T *)&raw[l];
+            float f[VE];
+            if (at >= 0 && at + VE <= P.vocab) {
 #pragma unroll
-        for (int i = 0; i < VE; ++i) {
-            hi = fmaxf(hi, f[i]);
-            if (f[i] != -INFINITY) lo = fminf(lo, f[i]);
+                for (int i = 0; i < VE; ++i) f[i] = kept_logit(logit(e[i]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) f[i] = at + i >= 0 && at + i < P.vocab ? kept_logit(logit(src[at + i])) : -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < VE; i += 4) *(float4 *)(data + w * VE + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                hi = fmaxf(hi, f[i]);
+                lo = fminf(lo, f[i] == -INFINITY ? INFINITY : f[i]);
+            }
         }
     }
     hi = mx::warp_max(hi), lo = mx::warp_min(lo);
     if (lane == 0) S.warp_a[warp] = hi, S.warp_b[warp] = lo;
     cluster_sync();   // (every CTA of the cluster runs)
-    if (tid < C) {
-        for (int w = 0; w < SM_WARPS; ++w) hi = fmaxf(hi, S.warp_a[w]), lo = fminf(lo, S.warp_b[w]);
-        st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_a[rank]), tid), (u64)__float_as_uint(hi) << 32 | __float_as_uint(lo));
+    if (warp == 0) {
+        hi = mx::warp_max(S.warp_a[lane % SM_WARPS]), lo = mx::warp_min(S.warp_b[lane % SM_WARPS]);
+        if (lane < C) st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_a[rank]), lane), (u64)__float_as_uint(hi) << 32 | __float_as_uint(lo));
     }
     cluster_sync();
     float m = -INFINITY, least = INFINITY;
@@ -271,51 +318,54 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
     }
     T_ = fminf(T_, 1e30f);   // (28.7 T stays finite)
     if (k <= 0 || k >= P.vocab) k = 0;
-    const double log2e_t = 1.4426950408889634 / (double)T_;
+    const double log2e_t = 1.4426950408889634 / (double)T_, m64 = (double)m;
     // intervals over what has weight (2^-41 and more: 28.42 T) and what there is
     const float range = fminf(28.7f * T_, m - least);
     const float scale = range > 0.0f ? fminf((float)(SM_BINS - 1) / range, FLT_MAX) : 0.0f;
+    const float floor_l = fmaxf(m - 28.75f * T_, -FLT_MAX);   // no weight here and below (at most 41.5 octaves below 1)
     const double min_w = min_p > 0.0f ? (double)fminf(min_p, 1.0f) : 0.0;
 
-    auto entry = [&](int i) { return (u64)order_key(data[i]) << P.idx_bits | (((1u << P.idx_bits) - 1) - (unsigned)(idx0 + i)); };
+    auto entry = [&](int i) {   // (-0 is 0)
+        return (u64)order_key(data[i] + 0.0f) << P.idx_bits | (((1u << P.idx_bits) - 1) - (unsigned)(idx0 + i));
+    };
     auto entry_logit = [&](u64 e) { return key_float((uint32_t)(e >> P.idx_bits)); };
-    auto add_to = [&](int b, u64 mass) {   // a 64-bit sum by two words
-        const unsigned l = (unsigned)mass, old = atomicAdd(&S.lo[b], l);
+    auto add_to = [&](unsigned b, u64 mass) {   // a 64-bit sum by two words
+        const unsigned l = (unsigned)mass, old = atomicAdd(&S.mass[b].x, l);
         const unsigned h = (unsigned)(mass >> 32) + (old + l < old);
-        if (h) atomicAdd(&S.hi[b], h);
+        if (h) atomicAdd(&S.mass[b].y, h);
     };
     auto clear = [&]() {
-        for (int b = tid; b < SM_BINS; b += SM_THREADS) S.cnt[b] = S.lo[b] = S.hi[b] = 0;
+        for (int b = tid; b < SM_BINS; b += SM_THREADS) S.cnt[b] = 0, S.mass[b] = make_uint2(0, 0);
         __syncthreads();
     };
+    int turn = 0;
+    auto answer = [&]() { return &S.found[turn++ & 3]; };
     // the CTAs' histograms, added up by shares of the intervals into the first CTA's arrays, there as running sums
     auto merge = [&](unsigned *to_cnt, u64 *to_mass) {
         cluster_sync();
-        const int b0 = SM_BINS * rank / C, b1 = SM_BINS * (rank + 1) / C;
-        for (int b = b0 + tid; b < b1; b += SM_THREADS) {
+        const int b0 = SM_BINS / C * rank;
+        for (int b = b0 + tid; b < b0 + SM_BINS / C; b += SM_THREADS) {
             unsigned c = 0;
             u64 ms = 0;
+#pragma unroll 8
             for (int r = 0; r < C; ++r) {
                 c += ld_cluster32(mx::cluster_map(mx::smem_u32(&S.cnt[b]), r));
-                ms += (u64)ld_cluster32(mx::cluster_map(mx::smem_u32(&S.hi[b]), r)) << 32 | ld_cluster32(mx::cluster_map(mx::smem_u32(&S.lo[b]), r));
+                ms += ld_cluster64(mx::cluster_map(mx::smem_u32(&S.mass[b]), r));
             }
             st_cluster(mx::cluster_map(mx::smem_u32(&to_cnt[b]), 0), c);
             st_cluster(mx::cluster_map(mx::smem_u32(&to_mass[b]), 0), ms);
         }
         cluster_sync();
-        if (first_cta) {
-            running_sums(to_cnt, to_cnt, SM_BINS, S.scan);
-            running_sums(to_mass, to_mass, SM_BINS, S.scan);
-        }
+        if (first_cta) running_sums(to_cnt, to_mass, SM_BINS, S);
     };
-    // first CTA: the next window goes to all; then it is the one in force
+    // first CTA, by warp 0, of whose lane 0 this is the next window: it goes to all; then it is the one in force
     int wp = 0;
-    auto tell = [&]() {
-        if (first_cta) {
-            if (tid == 0) S.n_all = 0;
-            __syncthreads();
+    auto tell = [&](const Window &next) {
+        if (first_cta && warp == 0) {
             constexpr int W = sizeof(Window) / 4;
-            for (int i = tid; i < (C - 1) * W; i += SM_THREADS) {
+            if (lane == 0) S.w[wp ^ 1] = next, S.n_all = 0;
+            __syncwarp();
+            for (int i = lane; i < (C - 1) * W; i += 32) {
                 uint32_t *word = (uint32_t *)&S.w[wp ^ 1] + i % W;
                 st_cluster(mx::cluster_map(mx::smem_u32(word), 1 + i / W), *word);
             }
@@ -323,123 +373,113 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
         cluster_sync();
         wp ^= 1;
     };
-    auto inside = [&](int i) {
-        const Window &w = S.w[wp];
-        if (w.kind == 0) {
-            const int b = interval(data[i], m, scale);
-            return b >= w.b0 && b <= w.b1;
+    // f(i) for every logit of this CTA that lies in the window
+    auto for_window = [&](auto f) {
+        const Window w = S.w[wp];
+        const unsigned b0 = w.b0, span = w.b1 - w.b0;
+        for (int i = tid * 4; i < n; i += SM_THREADS * 4) {
+            const float4 l4 = *(const float4 *)(data + i);
+            const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+            unsigned in = 0;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                bool is = interval(l[v], m, scale) - b0 <= span;
+                if (w.kind == 1 && is) {
+                    const u64 e = entry(i + v);
+                    is = e >= w.lo && e <= w.hi;
+                }
+                in |= (unsigned)is << v;
+            }
+            for (; in; in &= in - 1) f(i + __ffs(in) - 1);
         }
-        if (data[i] == -INFINITY) return false;
-        const u64 e = entry(i);
-        return e >= w.lo && e <= w.hi;
     };
     // the window's entries, sorted, and their running masses (first CTA: S.all, S.mine); at most SM_LIST
     auto collect = [&]() {
         if (tid == 0) S.n_mine = 0;
         __syncthreads();
-        for (int i = tid; i < n; i += SM_THREADS)
-            if (inside(i)) {
-                const unsigned at = atomicAdd(&S.n_mine, 1u);
-                if (at < SM_LIST) S.mine[at] = entry(i);
-            }
+        for_window([&](int i) {
+            const unsigned at = atomicAdd(&S.n_mine, 1u);
+            if (at < SM_LIST) S.mine[at] = entry(i);
+        });
         __syncthreads();
         // into the first CTA's list, behind what others have put there; nobody looks at this CTA's memory any more
         const unsigned c = min(S.n_mine, (unsigned)SM_LIST);
-        if (tid == 0 && c) S.found_a = add_cluster(mx::cluster_map(mx::smem_u32(&S.n_all), 0), c);
-        __syncthreads();
-        const unsigned base = (unsigned)S.found_a;
-        for (unsigned i = tid; i < c; i += SM_THREADS)
-            if (base + i < SM_LIST) st_cluster(mx::cluster_map(mx::smem_u32(&S.all[base + i]), 0), S.mine[i]);
+        if (c) {
+            if (tid == 0) S.at_all = add_cluster(mx::cluster_map(mx::smem_u32(&S.n_all), 0), c);
+            __syncthreads();
+            const unsigned base = S.at_all;
+            for (unsigned i = tid; i < c; i += SM_THREADS)
+                if (base + i < SM_LIST) st_cluster(mx::cluster_map(mx::smem_u32(&S.all[base + i]), 0), S.mine[i]);
+        }
         cluster_sync();
         int total = 0;
         if (first_cta) {
             total = (int)min(S.n_all, (unsigned)SM_LIST);
-            int n2 = 2;
-            while (n2 < total) n2 <<= 1;
-            for (int i = total + tid; i < n2; i += SM_THREADS) S.all[i] = 0;
+            sort_down(S.all, S.mine, total);
+            for (int i = tid; i < total; i += SM_THREADS) S.mine[i] = to_mass(weight(entry_logit(S.all[i]), m64, log2e_t, S.table));
             __syncthreads();
-            sort_down(S.all, n2);
-            for (int i = tid; i < total; i += SM_THREADS) S.mine[i] = to_mass(weight(entry_logit(S.all[i]), m, log2e_t, S.table));
-            __syncthreads();
-            running_sums(S.mine, S.mine, total, S.scan);
+            running_sums(nullptr, S.mine, total, S);
         }
         return total;
     };
     // first entry of the order whose running count (by_mass: mass) exceeds t; in the first CTA: its number in the sorted list,
     // the window and S.mine say what lies in front of it
     auto search = [&](u64 t, bool by_mass) {
+        Window next{};
         if (first_cta) {
-            int b = by_mass ? first_over(S.run_mass, SM_BINS, t, &S.found_a) : first_over(S.run_cnt, SM_BINS, t, &S.found_a);
-            b = min(b, SM_BINS - 1);
-            if (tid == 0) {
-                Window &w = S.w[wp ^ 1];
-                w.kind = 0, w.b0 = w.b1 = b;
-                w.base_count = b ? S.run_cnt[b - 1] : 0, w.base_mass = b ? S.run_mass[b - 1] : 0;
-                w.count = (int)(S.run_cnt[b] - (unsigned)w.base_count);
-            }
+            const int b = by_mass ? first_over(S.run_mass, SM_BINS, t, answer()) : first_over(S.run_cnt, SM_BINS, t, answer());
+            next.b0 = next.b1 = b;
+            if (b) next.base_count = S.run_cnt[b - 1], next.base_mass = S.run_mass[b - 1];
+            next.count = (int)(S.run_cnt[b] - (unsigned)next.base_count);
         }
-        tell();
+        tell(next);
         while (S.w[wp].count > SM_LIST) {
             // the range of the window's entries
             u64 e_lo = ~0ull, e_hi = 0;
-            for (int i = tid; i < n; i += SM_THREADS)
-                if (inside(i)) {
-                    const u64 e = entry(i);
-                    e_lo = min(e_lo, e), e_hi = max(e_hi, e);
-                }
+            for_window([&](int i) {
+                const u64 e = entry(i);
+                e_lo = min(e_lo, e), e_hi = max(e_hi, e);
+            });
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
                 e_lo = min(e_lo, __shfl_xor_sync(0xFFFFFFFFu, e_lo, o));
                 e_hi = max(e_hi, __shfl_xor_sync(0xFFFFFFFFu, e_hi, o));
             }
+            if (tid == 0) S.low = ~0ull, S.high = 0;
             clear();
-            if (tid == 0) S.found_b = ~0ull, S.found_c = 0;
-            __syncthreads();
-            if (lane == 0) atomicMin(&S.found_b, e_lo), atomicMax(&S.found_c, e_hi);
+            if (lane == 0) atomicMin(&S.low, e_lo), atomicMax(&S.high, e_hi);
             __syncthreads();
             if (tid < C) {
-                st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_a[rank]), tid), S.found_b);
-                st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_b[rank]), tid), S.found_c);
+                st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_a[rank]), tid), S.low);
+                st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_b[rank]), tid), S.high);
             }
             cluster_sync();
             for (int c = 0; c < C; ++c) e_lo = min(e_lo, S.slot_a[c]), e_hi = max(e_hi, S.slot_b[c]);
             int shr = 0;
             while ((e_hi - e_lo) >> shr >= SM_BINS) ++shr;
-            for (int i = tid; i < n; i += SM_THREADS)
-                if (inside(i)) {
-                    const u64 e = entry(i);
-                    const int b = (int)((e_hi - e) >> shr);
-                    atomicAdd(&S.cnt[b], 1u);
-                    add_to(b, to_mass(weight(data[i], m, log2e_t, S.table)));
-                }
+            for_window([&](int i) {
+                const unsigned b = (unsigned)((e_hi - entry(i)) >> shr);
+                atomicAdd(&S.cnt[b], 1u);
+                add_to(b, to_mass(weight(data[i], m64, log2e_t, S.table)));
+            });
             unsigned *c_run = (unsigned *)S.all;   // (no list is in use)
             merge(c_run, S.mine);
             if (first_cta) {
-                const Window &now = S.w[wp];
-                const u64 base = by_mass ? now.base_mass : now.base_count;
-                int b = by_mass ? first_over(S.mine, SM_BINS, t - base, &S.found_a) : first_over(c_run, SM_BINS, t - base, &S.found_a);
-                b = min(b, SM_BINS - 1);
-                __syncthreads();
-                if (tid == 0) {
-                    const u64 c_before = b ? c_run[b - 1] : 0;
-                    Window &w = S.w[wp ^ 1];
-                    w.kind = 1;
-                    w.hi = e_hi - ((u64)b << shr);
-                    w.lo = w.hi - e_lo < (1ull << shr) ? e_lo : w.hi - ((1ull << shr) - 1);
-                    w.count = (int)(c_run[b] - c_before);
-                    w.base_count = now.base_count + c_before, w.base_mass = now.base_mass + (b ? S.mine[b - 1] : 0);
-                }
+                next = S.w[wp];
+                const u64 left = t - (by_mass ? next.base_mass : next.base_count);
+                const int b = by_mass ? first_over(S.mine, SM_BINS, left, answer()) : first_over(c_run, SM_BINS, left, answer());
+                const u64 c_before = b ? c_run[b - 1] : 0;
+                next.kind = 1;
+                next.hi = e_hi - ((u64)b << shr);
+                next.lo = next.hi - e_lo < (1ull << shr) ? e_lo : next.hi - ((1ull << shr) - 1);
+                next.count = (int)(c_run[b] - c_before);
+                next.base_count += c_before, next.base_mass += b ? S.mine[b - 1] : 0;
             }
-            tell();
+            tell(next);
         }
         const int total = collect();
-        int at = 0;
-        if (first_cta) {
-            if (by_mass) at = first_over(S.mine, total, t - S.w[wp].base_mass, &S.found_a);
-            else at = (int)(t - S.w[wp].base_count);
-            at = max(0, min(at, total - 1));
-        }
-        return at;
+        if (!first_cta) return 0;
+        return by_mass ? first_over(S.mine, total, t - S.w[wp].base_mass, answer()) : (int)(t - S.w[wp].base_count);
     };
     auto share = [&](double of, u64 total) { return (u64)fmin(of * (double)total, (double)total); };   // (cut off, not rounded)
 
@@ -449,19 +489,31 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
         // ---- histogram over max - l ----
         clear();
         u64 sum_min = 0;
-        for (int i = tid; i < n; i += SM_THREADS) {
-            const float l = data[i];
-            const int b = interval(l, m, scale);
-            if (b >= SM_BINS) continue;
-            atomicAdd(&S.cnt[b], 1u);
+        for (int i = tid * 4; i < n; i += SM_THREADS * 4) {
+            const float4 l4 = *(const float4 *)(data + i);
+            const float l[4] = {l4.x, l4.y, l4.z, l4.w};
             if (with_mass) {
-                const double w = weight(l, m, log2e_t, S.table);
-                const u64 mass = to_mass(w);
-                add_to(b, mass);
-                if (w >= min_w) sum_min += mass;
+                double w[4];
+#pragma unroll
+                for (int v = 0; v < 4; ++v) w[v] = weight(fmaxf(l[v], floor_l), m64, log2e_t, S.table);
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const unsigned b = interval(l[v], m, scale);
+                    const u64 mass = to_mass(w[v]);
+                    if (b >= SM_BINS) continue;
+                    atomicAdd(&S.cnt[b], 1u);
+                    add_to(b, mass);
+                    if (min_w > 0.0 && w[v] >= min_w) sum_min += mass;
+                }
+            } else {
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const unsigned b = interval(l[v], m, scale);
+                    if (b < SM_BINS) atomicAdd(&S.cnt[b], 1u);
+                }
             }
         }
-        if (with_mass) {
+        if (with_mass && min_w > 0.0) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum_min += __shfl_xor_sync(0xFFFFFFFFu, sum_min, o);
             if (lane == 0) S.scan[warp] = sum_min;
@@ -473,26 +525,20 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
         }
         merge(S.run_cnt, S.run_mass);
         // ---- everything that can be kept, if that is one list ----
+        Window next{};
         if (first_cta) {
+            const unsigned there = S.run_cnt[SM_BINS - 1];
+            z = z_min = S.run_mass[SM_BINS - 1];
             int b = SM_BINS - 1;
-            if (k) b = min(b, first_over(S.run_cnt, SM_BINS, (u64)(k - 1), &S.found_a));
-            else if (p < 1.0f) {
-                z = S.run_mass[SM_BINS - 1];
-                b = min(b, first_over(S.run_mass, SM_BINS, (u64)ceil((double)p * (double)z) - 1, &S.found_a));
-            }
-            if (with_mass) {
-                z = S.run_mass[SM_BINS - 1];
+            if (k) b = first_over(S.run_cnt, SM_BINS, (u64)min((unsigned)k, there) - 1, answer());
+            else if (p < 1.0f) b = first_over(S.run_mass, SM_BINS, (u64)ceil((double)p * (double)z) - 1, answer());
+            if (with_mass && min_w > 0.0) {
                 z_min = 0;
                 for (int c = 0; c < C; ++c) z_min += S.slot_b[c];
             }
-            __syncthreads();
-            if (tid == 0) {
-                Window &w = S.w[wp ^ 1];
-                w.kind = 0, w.b0 = 0, w.b1 = b, w.base_count = w.base_mass = 0;
-                w.count = (int)S.run_cnt[b];
-            }
+            next.b1 = b, next.count = (int)S.run_cnt[b];
         }
-        tell();
+        tell(next);
         if (S.w[wp].count <= SM_LIST || with_mass) break;
         with_mass = true;   // (many equal logits, or many close to the k-th)
     }
@@ -502,19 +548,18 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
         if (!first_cta) return;
         if (k) z = S.mine[min(k, total) - 1];
         u64 keep = z;
-        if (p < 1.0f) keep = S.mine[min(first_over(S.mine, total, (u64)ceil((double)p * (double)z) - 1, &S.found_a), total - 1)];
+        if (p < 1.0f) keep = S.mine[first_over(S.mine, total, (u64)ceil((double)p * (double)z) - 1, answer())];
         if (min_w > 0.0) {
             // the last entry of M among the list's; M beyond the list keeps all that P keeps
-            if (tid == 0) S.found_b = 0;
+            if (tid == 0) S.low = 0;
             __syncthreads();
             for (int i = tid; i < total; i += SM_THREADS)
-                if (weight(entry_logit(S.all[i]), m, log2e_t, S.table) >= min_w) atomicMax(&S.found_b, S.mine[i]);
+                if (weight(entry_logit(S.all[i]), m64, log2e_t, S.table) >= min_w) atomicMax(&S.low, S.mine[i]);
             __syncthreads();
-            keep = min(keep, S.found_b);
+            keep = min(keep, S.low);
         }
         z = keep;
-        const u64 t = min(share((double)u, z), z - 1);
-        at = min(first_over(S.mine, total, t, &S.found_a), total - 1);
+        at = first_over(S.mine, total, min(share((double)u, z), z - 1), answer());
     } else {
         if (k) {
             const int i = search(first_cta ? (u64)min((unsigned)k, S.run_cnt[SM_BINS - 1]) - 1 : 0, false);
@@ -528,7 +573,6 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
         at = search(first_cta ? min(share((double)u, z), z - 1) : 0, true);
         if (!first_cta) return;
     }
-    __syncthreads();
     if (tid == 0) {
         const u64 e = S.all[at];
         P.token[row] = (int)(((1u << P.idx_bits) - 1) - (unsigned)(e & ((1ull << P.idx_bits) - 1)));
