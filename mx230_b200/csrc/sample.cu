@@ -51,12 +51,13 @@ struct SampleParams {
 
 // What the first CTA tells the others (whole words, so that it can be copied as such).
 struct Window {
-    int kind;                // 0: intervals b0 .. b1 of the histogram over max - l; 1: entries lo .. hi; 2: done
-    int b0, b1;
+    int kind;                // entries of: 0: intervals b0 .. b1 of the histogram over max - l, and c0 .. c1; 1: lo .. hi as well
+    int b0, b1, c0, c1;
     int count;               // entries in it
     u64 lo, hi;
     u64 base_count, base_mass;   // of the entries in front of it
 };
+constexpr int W_EVERYTHING = SM_LIST + 1;   // count of the window that says: more than a list
 
 struct alignas(16) Shared {
     uint2 mass[SM_BINS];         // this CTA's histogram: masses in two words, counts
@@ -183,45 +184,58 @@ __device__ __forceinline__ int first_over(const R *run, int n, u64 t, int *found
     return *found;
 }
 
-// Sorts n <= SM_LIST entries of v, largest first, by the bitonic network: a thread has one of each half; strides below 32 go
-// through the warp, larger ones through v and `other` in turns (a barrier each).
-__device__ __forceinline__ void sort_down(u64 *v, u64 *other, int n) {
-    static_assert(SM_LIST == 2 * SM_THREADS, "two entries a thread");
+// Sorts n <= E * SM_THREADS entries of v, largest first, by the bitonic network: a thread has E of them, SM_THREADS apart; strides
+// below 32 go through the warp, larger ones through v and `other` in turns.  Warps without entries stay out of it.
+template <int E>
+__device__ __forceinline__ void sort_entries(u64 *v, u64 *other, int n) {
     const int tid = threadIdx.x;
-    u64 e[2] = {tid < n ? v[tid] : 0, tid + SM_THREADS < n ? v[tid + SM_THREADS] : 0};
-    u64 *buf = other, *next = v;
-    for (int k = 2; k < 2 * n; k <<= 1) {
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            if (j == SM_THREADS) {
-                const u64 a = max(e[0], e[1]), b = min(e[0], e[1]);
-                e[0] = a, e[1] = b;
-                continue;
+    int threads = 32;
+    while (threads < n && threads < SM_THREADS) threads <<= 1;
+    u64 e[E];
+    if (tid < threads) {
+#pragma unroll
+        for (int h = 0; h < E; ++h) e[h] = tid + h * SM_THREADS < n ? v[tid + h * SM_THREADS] : 0;
+        u64 *buf = other, *next = v;
+        for (int k = 2; k < 2 * n; k <<= 1) {
+            int j = k >> 1;
+            if (E == 2 && j == SM_THREADS) {
+                const u64 a = max(e[0], e[E - 1]);
+                e[E - 1] = min(e[0], e[E - 1]), e[0] = a;
+                j >>= 1;
             }
-            u64 o[2];
-            if (j >= 32) {
-                buf[tid] = e[0];
-                if (n > SM_THREADS) buf[tid + SM_THREADS] = e[1];
-                __syncthreads();
-                o[0] = buf[tid ^ j];
-                o[1] = n > SM_THREADS ? buf[(tid ^ j) + SM_THREADS] : 0;
+            for (; j >= 32; j >>= 1) {
+#pragma unroll
+                for (int h = 0; h < E; ++h) buf[tid + h * SM_THREADS] = e[h];
+                asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
+#pragma unroll
+                for (int h = 0; h < E; ++h) {
+                    const int i = tid + h * SM_THREADS;
+                    const u64 o = buf[i ^ j];
+                    e[h] = ((i & j) == 0) == ((i & k) == 0) ? max(e[h], o) : min(e[h], o);   // this place of the pair gets the larger one
+                }
                 u64 *const b = buf;
                 buf = next, next = b;
-            } else {
-                o[0] = __shfl_xor_sync(0xFFFFFFFFu, e[0], j);
-                o[1] = n > SM_THREADS ? __shfl_xor_sync(0xFFFFFFFFu, e[1], j) : 0;
             }
+            for (; j > 0; j >>= 1)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int i = tid + h * SM_THREADS;
-                const bool larger = ((i & j) == 0) == ((i & k) == 0);   // this place of the pair gets the larger one
-                e[h] = larger ? max(e[h], o[h]) : min(e[h], o[h]);
-            }
+                for (int h = 0; h < E; ++h) {
+                    const int i = tid + h * SM_THREADS;
+                    const u64 o = __shfl_xor_sync(0xFFFFFFFFu, e[h], j);
+                    e[h] = ((i & j) == 0) == ((i & k) == 0) ? max(e[h], o) : min(e[h], o);
+                }
         }
     }
     __syncthreads();   // (the last exchange has been read)
-    if (tid < n) v[tid] = e[0];
-    if (tid + SM_THREADS < n) v[tid + SM_THREADS] = e[1];
+    if (tid < threads)
+#pragma unroll
+        for (int h = 0; h < E; ++h)
+            if (tid + h * SM_THREADS < n) v[tid + h * SM_THREADS] = e[h];
     __syncthreads();
+}
+__device__ __forceinline__ void sort_down(u64 *v, u64 *other, int n) {
+    static_assert(SM_LIST == 2 * SM_THREADS, "two entries a thread");
+    if (n <= SM_THREADS) sort_entries<1>(v, other, n);
+    else sort_entries<2>(v, other, n);
 }
 
 template <typename T>
@@ -233,6 +247,8 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
     const int C = P.ctas, row = blockIdx.x / C, rank = blockIdx.x - row * C;
     const bool first_cta = rank == 0;
     mx::pdl_trigger();
+    __syncwarp();
+    mx::cluster_arrive_relaxed();   // waited for before the first store to another CTA's memory
     if (tid < 256) S.table[tid] = exp2((double)tid / 256.0);
     mx::pdl_wait();
 
@@ -282,7 +298,8 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
     }
     hi = mx::warp_max(hi), lo = mx::warp_min(lo);
     if (lane == 0) S.warp_a[warp] = hi, S.warp_b[warp] = lo;
-    cluster_sync();   // (every CTA of the cluster runs)
+    __syncthreads();
+    mx::cluster_wait();
     if (warp == 0) {
         hi = mx::warp_max(S.warp_a[lane % SM_WARPS]), lo = mx::warp_min(S.warp_b[lane % SM_WARPS]);
         if (lane < C) st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_a[rank]), lane), (u64)__float_as_uint(hi) << 32 | __float_as_uint(lo));
@@ -376,14 +393,15 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
     // f(i) for every logit of this CTA that lies in the window
     auto for_window = [&](auto f) {
         const Window w = S.w[wp];
-        const unsigned b0 = w.b0, span = w.b1 - w.b0;
+        const unsigned b0 = w.b0, span_b = w.b1 - w.b0, c0 = w.c0, span_c = w.c1 - w.c0;
         for (int i = tid * 4; i < n; i += SM_THREADS * 4) {
             const float4 l4 = *(const float4 *)(data + i);
             const float l[4] = {l4.x, l4.y, l4.z, l4.w};
             unsigned in = 0;
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                bool is = interval(l[v], m, scale) - b0 <= span;
+                const unsigned b = interval(l[v], m, scale);
+                bool is = b - b0 <= span_b || b - c0 <= span_c;
                 if (w.kind == 1 && is) {
                     const u64 e = entry(i + v);
                     is = e >= w.lo && e <= w.hi;
@@ -428,7 +446,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
         Window next{};
         if (first_cta) {
             const int b = by_mass ? first_over(S.run_mass, SM_BINS, t, answer()) : first_over(S.run_cnt, SM_BINS, t, answer());
-            next.b0 = next.b1 = b;
+            next.b0 = next.b1 = next.c0 = next.c1 = b;
             if (b) next.base_count = S.run_cnt[b - 1], next.base_mass = S.run_mass[b - 1];
             next.count = (int)(S.run_cnt[b] - (unsigned)next.base_count);
         }
@@ -524,7 +542,8 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
             }
         }
         merge(S.run_cnt, S.run_mass);
-        // ---- everything that can be kept, if that is one list ----
+        // ---- what is to be looked at: all that can be kept, if that is a list; else (k = 0) the interval where P ends and those where
+        // the token then can be, if they are; else more than that ----
         Window next{};
         if (first_cta) {
             const unsigned there = S.run_cnt[SM_BINS - 1];
@@ -536,7 +555,22 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
                 z_min = 0;
                 for (int c = 0; c < C; ++c) z_min += S.slot_b[c];
             }
-            next.b1 = b, next.count = (int)S.run_cnt[b];
+            next.b1 = next.c1 = b, next.count = (int)S.run_cnt[b];
+            if (next.count > SM_LIST && k == 0) {
+                // the kept mass lies between these, and u's share of it too
+                const u64 z0 = min(z_min, p < 1.0f ? (b ? S.run_mass[b - 1] : 0) : z), z1 = min(z_min, p < 1.0f ? S.run_mass[b] : z);
+                next.c0 = first_over(S.run_mass, SM_BINS, z0 ? min(share((double)u, z0), z0 - 1) : 0, answer());
+                next.c1 = first_over(S.run_mass, SM_BINS, min(share((double)u, z1), z1 - 1), answer());
+                if (p < 1.0f) {
+                    if (next.c1 >= b) next.c1 = b;
+                    next.b0 = next.b1 = b;
+                    if (next.c1 == b) next.b0 = next.c0;   // (next to each other: one range)
+                } else next.b0 = next.c0, next.b1 = next.c1;
+                const unsigned in_b = S.run_cnt[next.b1] - (next.b0 ? S.run_cnt[next.b0 - 1] : 0);
+                const unsigned in_c = S.run_cnt[next.c1] - (next.c0 ? S.run_cnt[next.c0 - 1] : 0);
+                next.count = (int)(next.c1 == next.b1 ? in_b : in_b + in_c);
+            }
+            if (next.count > SM_LIST) next.count = W_EVERYTHING;
         }
         tell(next);
         if (S.w[wp].count <= SM_LIST || with_mass) break;
@@ -546,20 +580,34 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
     if (S.w[wp].count <= SM_LIST) {
         const int total = collect();
         if (!first_cta) return;
+        // the list's running masses are those of the whole order less what lies in front of its ranges: of c (or b, if it is one
+        // range), and between c and b
+        const Window w = S.w[wp];
+        const bool one = w.c1 == w.b1;
+        const u64 front = w.c0 ? S.run_mass[w.c0 - 1] : 0;
+        u64 between = 0;
+        if (!one) {
+            const u64 in_c = S.mine[S.run_cnt[w.c1] - (w.c0 ? S.run_cnt[w.c0 - 1] : 0) - 1];
+            between = S.run_mass[w.b0 - 1] - front - in_c;
+        }
         if (k) z = S.mine[min(k, total) - 1];
         u64 keep = z;
-        if (p < 1.0f) keep = S.mine[first_over(S.mine, total, (u64)ceil((double)p * (double)z) - 1, answer())];
+        if (p < 1.0f) keep = front + between + S.mine[first_over(S.mine, total, (u64)ceil((double)p * (double)z) - 1 - front - between, answer())];
         if (min_w > 0.0) {
-            // the last entry of M among the list's; M beyond the list keeps all that P keeps
-            if (tid == 0) S.low = 0;
-            __syncthreads();
-            for (int i = tid; i < total; i += SM_THREADS)
-                if (weight(entry_logit(S.all[i]), m64, log2e_t, S.table) >= min_w) atomicMax(&S.low, S.mine[i]);
-            __syncthreads();
-            keep = min(keep, S.low);
+            if (with_mass) keep = min(keep, z_min);
+            else {   // the last entry of M among the list's; M beyond the list keeps all that P keeps
+                if (tid == 0) S.low = 0;
+                __syncthreads();
+                for (int i = tid; i < total; i += SM_THREADS)
+                    if (weight(entry_logit(S.all[i]), m64, log2e_t, S.table) >= min_w) atomicMax(&S.low, S.mine[i]);
+                __syncthreads();
+                keep = min(keep, S.low);
+            }
         }
         z = keep;
-        at = first_over(S.mine, total, min(share((double)u, z), z - 1), answer());
+        const u64 t = min(share((double)u, z), z - 1) - front;
+        // (behind c: in b)
+        at = first_over(S.mine, total, one || t < S.mine[S.run_cnt[w.c1] - (w.c0 ? S.run_cnt[w.c0 - 1] : 0) - 1] ? t : t - between, answer());
     } else {
         if (k) {
             const int i = search(first_cta ? (u64)min((unsigned)k, S.run_cnt[SM_BINS - 1]) - 1 : 0, false);
