@@ -560,7 +560,7 @@ int mx230_qkv_rope_kvwrite(mx230_handle *h, void *stream, float *qkv, const floa
  *   prob     (may be null) its share of that weight
  * temperature <= 0 or NaN: the first of the order, prob 1; above 1e30 it is 1e30.  -inf and NaN logits are masked, +inf counts as
  * the largest finite number; a row with nothing left gets token -1, prob 0.  u below 0 or NaN is 0; at 1 and above the last kept
- * entry is drawn.  Sums are over whole numbers: a row gives the same token in any batch.  At most 360192 logits a row.
+ * entry is drawn.  Sums are over whole numbers: a row gives the same token in any batch.  At most 4194304 logits a row.
  * No workspace. */
 int mx230_sample(mx230_handle *h, void *stream, int *token, float *prob, const void *logits, int dtype, int n_rows, int vocab,
                  long long row_stride, const float *u, float temperature, const float *temperatures, int top_k,

@@ -11,15 +11,16 @@
 // to be found is always "the first entry of the order whose running count or mass exceeds t"; three of them at most, each
 // target known from the one before (the intersection of two prefixes has the smaller of their masses).
 //
-// Bounded by HBM: the logits are read once.  A cluster of up to eight CTAs holds a row in its shared memory.  A histogram over 1024
+// Bounded by HBM: the logits are read once.  A cluster of up to eight CTAs holds a row in its shared memory.  A histogram over 2048
 // equal intervals of max - l, as far as weights are not 0 (28.5 T), in counts and masses says which interval holds an entry that is
 // sought; the entries of that interval alone are collected, sorted and summed.  Where an interval has more entries
 // than the list, a histogram over the range of their (value, index) takes its place, as often as it takes.
-// Weights take eleven fp64 instructions an entry (a table of 256 steps of 2^(1/256) and a polynomial of degree four, below
-// 1e-15); rows with a small k take them for the entries of the list only.
+// A weight takes fifteen fp64 instructions; rows with a small k take them for the entries of the list only.
 #include <cuda_fp16.h>
 #include <float.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -29,24 +30,36 @@ typedef unsigned long long u64;
 
 constexpr int SM_THREADS = 512;
 constexpr int SM_WARPS = SM_THREADS / 32;
-constexpr int SM_BINS = 1024;
+constexpr int SM_BINS = 2048;
 constexpr int SM_LIST = 1024;        // entries that are sorted, most
 constexpr int SM_CLUSTER = 8;
-constexpr int SM_MAX_DATA = 45056;   // logits that a CTA can hold
+constexpr int SM_MAX = 1 << 22;      // logits of a row: their masses stay below 2^63
 constexpr double SM_MASS = 1099511627776.0;   // 2^40
+typedef std::integral_constant<int, 0> First;    // passes over the logits
+typedef std::integral_constant<int, 1> Weigh;
+typedef std::integral_constant<int, 2> Look;
+constexpr size_t SM_ALL = 224 * 1024, SM_HALF = 112 * 1024;   // shared memory of a CTA that has an SM to itself, that shares it
 
+struct Coefficients {
+    double magic, two52, c[9];
+};
+const Coefficients POWER_OF_TWO = {
+    6755399441055744.0,   // 1.5 * 2^52: the last bits of a sum with it are the rounded whole number
+    4503599627370496.0,   // 2^52
+    {1.0203121063391729e-07, 1.3255224878668817e-06, 1.525268684626772e-05, 0.00015403455852453838, 0.0013333558179043112,
+     0.009618129159402558, 0.055504108664760424, 0.2402265069581299, 0.6931471805599453}};
 struct SampleParams {
     int *token;
     float *prob;
     const void *logits;
     long long row_stride;
     int vocab, ctas, idx_bits;
-    int cap;                 // logits of a CTA's share, at most
     const float *u;
     float temperature, top_p, min_p;
     int top_k;
     const float *temperatures, *top_ps, *min_ps;
     const int *top_ks;
+    Coefficients power;
 };
 
 // What the first CTA tells the others (whole words, so that it can be copied as such).
@@ -60,14 +73,13 @@ struct Window {
 constexpr int W_EVERYTHING = SM_LIST + 1;   // count of the window that says: more than a list
 
 struct alignas(16) Shared {
-    uint2 mass[SM_BINS];         // this CTA's histogram: masses in two words, counts
-    unsigned cnt[SM_BINS];
+    // this CTA's histogram: counts, masses in two words; what has no weight is counted behind them, by lanes
+    unsigned cnt[SM_BINS + 32], lo[SM_BINS + 32], hi[SM_BINS + 32];
     // first CTA: running counts and masses over the first histogram's intervals
     unsigned run_cnt[SM_BINS];
     u64 run_mass[SM_BINS];
     // a list's entries of this CTA, and of all (first CTA); running masses of the sorted list; a later histogram's running sums
     u64 mine[SM_LIST], all[SM_LIST];
-    double table[256];
     u64 scan[SM_WARPS];
     unsigned scan_cnt[SM_WARPS];
     u64 slot_a[SM_CLUSTER], slot_b[SM_CLUSTER];        // a word of each CTA
@@ -89,11 +101,6 @@ __device__ __forceinline__ uint32_t ld_cluster32(uint32_t addr) {
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
 }
-__device__ __forceinline__ u64 ld_cluster64(uint32_t addr) {
-    u64 v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
-    return v;
-}
 __device__ __forceinline__ uint32_t add_cluster(uint32_t addr, uint32_t v) {
     uint32_t old;
     asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(v) : "memory");
@@ -105,8 +112,24 @@ template <> __device__ __forceinline__ float logit(float v) { return v; }
 template <> __device__ __forceinline__ float logit(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float logit(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// as it is kept: NaN is masked, infinity the largest number
-__device__ __forceinline__ float kept_logit(float l) { return l == l ? fminf(l, FLT_MAX) : -INFINITY; }
+// a row's first or last piece of 16 bytes, masked where it is outside the row
+template <typename T>
+__device__ __noinline__ uint4 ragged_piece(const T *src, int at, int vocab) {
+    constexpr int VE = 16 / (int)sizeof(T);
+    const T masked = (T)-INFINITY;
+    uint32_t word[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        T v[VE / 4];
+#pragma unroll
+        for (int c = 0; c < VE / 4; ++c) {
+            const int x = at + i * (VE / 4) + c;
+            v[c] = x >= 0 && x < vocab ? src[x] : masked;
+        }
+        word[i] = *(const uint32_t *)v;
+    }
+    return make_uint4(word[0], word[1], word[2], word[3]);
+}
 
 // whole numbers in the order of the floats, and back
 __device__ __forceinline__ uint32_t order_key(float l) {
@@ -115,38 +138,55 @@ __device__ __forceinline__ uint32_t order_key(float l) {
 }
 __device__ __forceinline__ float key_float(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k); }
 
-// 2^(j / 256), j of a table, times the polynomial of 2^r for |r| <= 1/512; at most 42 octaves below 1, exactly 1 for l = m
-__device__ __forceinline__ double weight(float l, double m, double log2e_t, const double *table) {
-    const double x = ((double)l - m) * log2e_t;
-    const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's last bits are the rounded whole number
-    const double t = fma(x, 256.0, magic);
-    const int n = __double2loint(t);
-    const double r = fma(t - magic, -0.00390625, x);
-    // ln 2^i / i!
-    double p = fma(r, 9.618129107628477e-3, 5.550410866482158e-2);
-    p = fma(r, p, 2.402265069591007e-1);
-    p = fma(r, p, 6.931471805599453e-1);
-    p = fma(r, p, 1.0);
-    p *= table[n & 255];
-    return __hiloint2double(__double2hiint(p) + ((n >> 8) << 20), __double2loint(p));
+// Weight of a logit d <= 0 above the largest, e^(d / T) = 2^n 2^r: 2^n, and 2^r for |r| <= 1/2 by a polynomial of degree nine that
+// is 1 at 0 and meets 2^r at the Chebyshev nodes (3.7e-14 of it elsewhere).  fp64 throughout: a table of powers in shared memory, in
+// place of five of the steps, was read by 32 lanes at random, and that and the histogram's sums took what its banks give.  The
+// coefficients come with the launch's parameters, from where an instruction takes them as an operand; as literals they were
+// moved into registers again and again.
+struct Weight {
+    int n;
+    double p;
+};
+__device__ __forceinline__ Weight weight_of(double d, double log2e_t, const Coefficients &k) {
+    const double t = fma(d, log2e_t, k.magic), r = fma(d, log2e_t, k.magic - t);
+    double p = fma(r, k.c[0], k.c[1]);
+#pragma unroll
+    for (int i = 2; i < 9; ++i) p = fma(r, p, k.c[i]);
+    return {__double2loint(t), fma(r, p, 1.0)};
 }
-__device__ __forceinline__ u64 to_mass(double w) {   // (ties cannot be: no weight but 1 is a binary fraction)
-    return (u64)__double_as_longlong(fma(w, SM_MASS, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+__device__ __forceinline__ double weight(double d, double log2e_t, const Coefficients &k) {
+    const Weight w = weight_of(d, log2e_t, k);
+    return w.p * __hiloint2double((1023 + w.n) * (1 << 20), 0);
+}
+// as a whole number of 2^-40: added to 2^52, it is the last bits of the sum (ties cannot be: no weight but 1 is a binary fraction)
+__device__ __forceinline__ u64 mass_of(double d, double log2e_t, const Coefficients &k) {
+    const Weight w = weight_of(d, log2e_t, k);
+    return (u64)__double_as_longlong(fma(w.p, __hiloint2double((1023 + 40 + w.n) * (1 << 20), 0), k.two52)) & 0xFFFFFFFFFFFFFull;
+}
+__device__ __forceinline__ float finite(float l) {   // infinity is the largest number; NaN stays
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(l), "f"(FLT_MAX));
+    return r;
 }
 
-// interval of max - l; SM_BINS: no weight, or masked (an infinite difference, or NaN where the scale is 0).  Monotone in l: a
-// difference, a product and a sum, each rounded.
-__device__ __forceinline__ unsigned interval(float l, float m, float scale) {
-    return __float_as_uint(fminf((m - l) * scale, (float)SM_BINS) + 8388608.0f) & 0x7FFFFFu;
-}
+// Interval of max - l, as the float 2^23 + interval: a difference, and a product and a sum rounded once, so it is monotone in l.
+// Masked logits get infinity or NaN: no interval is larger or smaller than NaN, so "it is below a bound" leaves both out.
+constexpr float SM_INTERVAL = 8388608.0f;
+__device__ __forceinline__ float interval(float l, float m, float scale) { return fmaf(m - l, scale, SM_INTERVAL); }
 
-// running sums of n counts and masses (n <= 2 * SM_THREADS), two a thread, in place; counts may be null
+// running sums of n counts and masses (n <= PER * SM_THREADS), PER a thread, in place; counts may be null
+template <int PER>
 __device__ __forceinline__ void running_sums(unsigned *cnt, u64 *mass, int n, Shared &S) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = 2 * threadIdx.x;
-    const u64 m0 = i < n ? mass[i] : 0, m1 = i + 1 < n ? mass[i + 1] : 0;
-    const unsigned c0 = cnt && i < n ? cnt[i] : 0, c1 = cnt && i + 1 < n ? cnt[i + 1] : 0;
-    u64 m = m0 + m1;
-    unsigned c = c0 + c1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i0 = PER * threadIdx.x;
+    u64 ms[PER], m = 0;
+    unsigned cs[PER], c = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        m += i0 + i < n ? mass[i0 + i] : 0, c += cnt && i0 + i < n ? cnt[i0 + i] : 0;
+        ms[i] = m, cs[i] = c;
+    }
+    const u64 own_m = m;
+    const unsigned own_c = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const u64 mu = __shfl_up_sync(0xFFFFFFFFu, m, o);
@@ -163,25 +203,23 @@ __device__ __forceinline__ void running_sums(unsigned *cnt, u64 *mass, int n, Sh
         before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
         cb += __shfl_xor_sync(0xFFFFFFFFu, cb, o);
     }
-    m += __shfl_sync(0xFFFFFFFFu, before, 0), c += __shfl_sync(0xFFFFFFFFu, cb, 0);
-    if (i < n) {
-        mass[i] = m - m1;
-        if (cnt) cnt[i] = c - c1;
-    }
-    if (i + 1 < n) {
-        mass[i + 1] = m;
-        if (cnt) cnt[i + 1] = c;
-    }
+    before = __shfl_sync(0xFFFFFFFFu, before, 0) + m - own_m, cb = __shfl_sync(0xFFFFFFFFu, cb, 0) + c - own_c;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (i0 + i < n) {
+            mass[i0 + i] = before + ms[i];
+            if (cnt) cnt[i0 + i] = cb + cs[i];
+        }
     __syncthreads();
 }
 
-// first index whose running sum exceeds t (there is one)
+// first index whose running sum exceeds t (there is one; whatever is found, it is an index)
 template <typename R>
 __device__ __forceinline__ int first_over(const R *run, int n, u64 t, int *found) {
     for (int i = threadIdx.x; i < n; i += SM_THREADS)
         if ((u64)run[i] > t && (i == 0 || (u64)run[i - 1] <= t)) *found = i;
     __syncthreads();
-    return *found;
+    return max(0, min(*found, n - 1));
 }
 
 // Sorts n <= E * SM_THREADS entries of v, largest first, by the bitonic network: a thread has E of them, SM_THREADS apart; strides
@@ -238,8 +276,9 @@ __device__ __forceinline__ void sort_down(u64 *v, u64 *other, int n) {
     else sort_entries<2>(v, other, n);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P) {
+// KEEP: a CTA's share of the row stays in its shared memory; else it is read again where it is needed again.
+template <typename T, bool KEEP>
+__global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParams P) {
     extern __shared__ __align__(16) unsigned char smem[];
     Shared &S = *(Shared *)smem;
     float *data = (float *)(smem + sizeof(Shared));
@@ -249,7 +288,6 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
     mx::pdl_trigger();
     __syncwarp();
     mx::cluster_arrive_relaxed();   // waited for before the first store to another CTA's memory
-    if (tid < 256) S.table[tid] = exp2((double)tid / 256.0);
     mx::pdl_wait();
 
     float T_ = P.temperatures ? P.temperatures[row] : P.temperature;
@@ -265,37 +303,49 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
     const int pieces = (P.vocab + shift + VE - 1) / VE;
     const int v0 = (int)((long long)pieces * rank / C), v1 = (int)((long long)pieces * (rank + 1) / C);
     const int n = (v1 - v0) * VE, idx0 = v0 * VE - shift;         // data[i] is logit idx0 + i
+    // f(i, l) for four logits of this CTA at a time, l[0] being logit idx0 + i; in the first pass they are put in shared memory (KEEP)
+    float m = -INFINITY, least = INFINITY;   // the row's largest and smallest (unmasked) logit
+    auto for_logits = [&](auto f, auto pass) {
+        constexpr bool first = pass.value == 0;
+        if (KEEP && !first) {
+            for (int i = tid * 4; i < n; i += SM_THREADS * 4) {
+                const float4 l4 = *(const float4 *)(data + i);
+                const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+                f(i, l);
+            }
+            return;
+        }
+        constexpr int LOADS = pass.value == 1 ? 1 : 4;   // in flight (weights take their time, and registers)
+        for (int v = tid; v < v1 - v0; v += LOADS * SM_THREADS) {
+            uint4 raw[LOADS];
+#pragma unroll
+            for (int q = 0; q < LOADS; ++q) {
+                const int w = v + q * SM_THREADS, at = idx0 + w * VE;
+                if (w >= v1 - v0) break;
+                if (at >= 0 && at + VE <= P.vocab) raw[q] = *(const uint4 *)(src + at);
+                else raw[q] = ragged_piece(src, at, P.vocab);
+            }
+#pragma unroll
+            for (int q = 0; q < LOADS; ++q) {
+                const int w = v + q * SM_THREADS;
+                if (w >= v1 - v0) break;
+                const T *e = (const T *)&raw[q];
+#pragma unroll
+                for (int i = 0; i < VE; i += 4) {
+                    const float l[4] = {logit(e[i]), logit(e[i + 1]), logit(e[i + 2]), logit(e[i + 3])};
+                    if (KEEP) *(float4 *)(data + w * VE + i) = make_float4(l[0], l[1], l[2], l[3]);
+                    f(w * VE + i, l);
+                }
+            }
+        }
+    };
+    // (infinity is the largest number; NaN is passed over)
     float hi = -INFINITY, lo = INFINITY;
-    constexpr int LOADS = 4;   // in flight
-    for (int v = tid; v < v1 - v0; v += LOADS * SM_THREADS) {
-        uint4 raw[LOADS];
+    for_logits([&](int, const float (&l)[4]) {
 #pragma unroll
-        for (int l = 0; l < LOADS; ++l) {
-            const int at = idx0 + (v + l * SM_THREADS) * VE;
-            if (v + l * SM_THREADS < v1 - v0 && at >= 0 && at + VE <= P.vocab) raw[l] = *(const uint4 *)(src + at);
-        }
-#pragma unroll
-        for (int l = 0; l < LOADS; ++l) {
-            const int w = v + l * SM_THREADS, at = idx0 + w * VE;
-            if (w >= v1 - v0) break;
-            const T *e = (const T *)&raw[l];
-            float f[VE];
-            if (at >= 0 && at + VE <= P.vocab) {
-#pragma unroll
-                for (int i = 0; i < VE; ++i) f[i] = kept_logit(logit(e[i]));
-            } else {
-#pragma unroll
-                for (int i = 0; i < VE; ++i) f[i] = at + i >= 0 && at + i < P.vocab ? kept_logit(logit(src[at + i])) : -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < VE; i += 4) *(float4 *)(data + w * VE + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
-#pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                hi = fmaxf(hi, f[i]);
-                lo = fminf(lo, f[i] == -INFINITY ? INFINITY : f[i]);
-            }
-        }
-    }
+        for (int c = 0; c < 4; ++c) hi = fmaxf(hi, l[c]), lo = fminf(lo, l[c] == -INFINITY ? INFINITY : l[c]);
+    }, First());
+    hi = fminf(hi, FLT_MAX), lo = fminf(lo, FLT_MAX);
     hi = mx::warp_max(hi), lo = mx::warp_min(lo);
     if (lane == 0) S.warp_a[warp] = hi, S.warp_b[warp] = lo;
     __syncthreads();
@@ -305,7 +355,6 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
         if (lane < C) st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_a[rank]), lane), (u64)__float_as_uint(hi) << 32 | __float_as_uint(lo));
     }
     cluster_sync();
-    float m = -INFINITY, least = INFINITY;
     for (int c = 0; c < C; ++c) m = fmaxf(m, __uint_as_float((uint32_t)(S.slot_a[c] >> 32))), least = fminf(least, __uint_as_float((uint32_t)S.slot_a[c]));
     if (m == -INFINITY) {   // nothing is left to choose from
         if (first_cta && tid == 0) {
@@ -319,8 +368,11 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
         if (tid == 0) S.n_mine = 0xFFFFFFFFu;
         __syncthreads();
         unsigned best = 0xFFFFFFFFu;
-        for (int i = tid; i < n; i += SM_THREADS)
-            if (data[i] == m) best = min(best, (unsigned)(idx0 + i));
+        for_logits([&](int i, const float (&l)[4]) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (finite(l[c]) == m) best = min(best, (unsigned)(idx0 + i + c));
+        }, Look());
         if (best != 0xFFFFFFFFu) atomicMin(&S.n_mine, best);
         __syncthreads();
         if (tid == 0) st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_b[rank]), 0), (u64)S.n_mine);
@@ -339,41 +391,52 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
     // intervals over what has weight (2^-41 and more: 28.42 T) and what there is
     const float range = fminf(28.7f * T_, m - least);
     const float scale = range > 0.0f ? fminf((float)(SM_BINS - 1) / range, FLT_MAX) : 0.0f;
-    const float floor_l = fmaxf(m - 28.75f * T_, -FLT_MAX);   // no weight here and below (at most 41.5 octaves below 1)
+    // M: w >= min_w, in doubt only close to the logit for which it is equal
     const double min_w = min_p > 0.0f ? (double)fminf(min_p, 1.0f) : 0.0;
+    const bool has_min = min_w > 0.0;
+    const float m_at = min_w > 0.0 ? m + logf((float)min_w) * T_ : -FLT_MAX, m_slack = 1e-5f * (fabsf(m) + fabsf(m_at) + T_);
+    const float m_low = m_at - m_slack, m_high = m_at + m_slack;
 
-    auto entry = [&](int i) {   // (-0 is 0)
-        return (u64)order_key(data[i] + 0.0f) << P.idx_bits | (((1u << P.idx_bits) - 1) - (unsigned)(idx0 + i));
+    auto entry = [&](int i, float l) {   // (-0 is 0)
+        return (u64)order_key(l + 0.0f) << P.idx_bits | (((1u << P.idx_bits) - 1) - (unsigned)(idx0 + i));
     };
     auto entry_logit = [&](u64 e) { return key_float((uint32_t)(e >> P.idx_bits)); };
+    bool with_mass = k == 0 || k > SM_LIST / 2;   // (a small k: only its entries' weights are asked for)
+    const bool with_count = k != 0;
+    auto mass = [&](float l) { return mass_of((double)l - m64, log2e_t, P.power); };
     auto add_to = [&](unsigned b, u64 mass) {   // a 64-bit sum by two words
-        const unsigned l = (unsigned)mass, old = atomicAdd(&S.mass[b].x, l);
+        const unsigned l = (unsigned)mass, old = atomicAdd(&S.lo[b], l);
         const unsigned h = (unsigned)(mass >> 32) + (old + l < old);
-        if (h) atomicAdd(&S.mass[b].y, h);
+        if (h) atomicAdd(&S.hi[b], h);
     };
     auto clear = [&]() {
-        for (int b = tid; b < SM_BINS; b += SM_THREADS) S.cnt[b] = 0, S.mass[b] = make_uint2(0, 0);
+        for (int b = tid; b < SM_BINS + 32; b += SM_THREADS) S.cnt[b] = S.lo[b] = S.hi[b] = 0;
         __syncthreads();
     };
     int turn = 0;
     auto answer = [&]() { return &S.found[turn++ & 3]; };
     // the CTAs' histograms, added up by shares of the intervals into the first CTA's arrays, there as running sums
-    auto merge = [&](unsigned *to_cnt, u64 *to_mass) {
+    auto merge = [&](unsigned *to_cnt, u64 *to_mass, bool counted, auto bins) {
         cluster_sync();
-        const int b0 = SM_BINS / C * rank;
-        for (int b = b0 + tid; b < b0 + SM_BINS / C; b += SM_THREADS) {
+        const int b0 = bins.value / C * rank;
+        for (int b = b0 + tid; b < b0 + bins.value / C; b += SM_THREADS) {
             unsigned c = 0;
             u64 ms = 0;
 #pragma unroll 8
             for (int r = 0; r < C; ++r) {
                 c += ld_cluster32(mx::cluster_map(mx::smem_u32(&S.cnt[b]), r));
-                ms += ld_cluster64(mx::cluster_map(mx::smem_u32(&S.mass[b]), r));
+                ms += (u64)ld_cluster32(mx::cluster_map(mx::smem_u32(&S.hi[b]), r)) << 32 | ld_cluster32(mx::cluster_map(mx::smem_u32(&S.lo[b]), r));
+            }
+            if (!counted) {
+                // at most so many have this mass: none has less than the interval's end (the masses are whole; below 1: any number)
+                const double least_mass = floor(weight(fmax(-(b + 0.51) / (double)scale, -28.75 * (double)T_), log2e_t, P.power) * (SM_MASS * (1 - 1e-6)) - 0.5);
+                c = least_mass >= 1.0 ? (unsigned)fmin((double)ms / least_mass + 1.0, SM_LIST + 1.0) : SM_LIST + 1;
             }
             st_cluster(mx::cluster_map(mx::smem_u32(&to_cnt[b]), 0), c);
             st_cluster(mx::cluster_map(mx::smem_u32(&to_mass[b]), 0), ms);
         }
         cluster_sync();
-        if (first_cta) running_sums(to_cnt, to_mass, SM_BINS, S);
+        if (first_cta) running_sums<bins.value / SM_THREADS>(to_cnt, to_mass, bins.value, S);
     };
     // first CTA, by warp 0, of whose lane 0 this is the next window: it goes to all; then it is the one in force
     int wp = 0;
@@ -390,34 +453,41 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
         cluster_sync();
         wp ^= 1;
     };
-    // f(i) for every logit of this CTA that lies in the window
+    // f(i, l) for every logit of this CTA that lies in the window
     auto for_window = [&](auto f) {
         const Window w = S.w[wp];
-        const unsigned b0 = w.b0, span_b = w.b1 - w.b0, c0 = w.c0, span_c = w.c1 - w.c0;
-        for (int i = tid * 4; i < n; i += SM_THREADS * 4) {
-            const float4 l4 = *(const float4 *)(data + i);
-            const float l[4] = {l4.x, l4.y, l4.z, l4.w};
-            unsigned in = 0;
+        const bool exact = w.kind == 1;
+        // logits of intervals b0 .. b1 lie between these, by more than the interval's own rounding
+        auto above = [&](int b) { return b == 0 ? INFINITY : m - ((float)b - 0.6f) / scale + 1e-6f * (fabsf(m) + (float)b / scale); };
+        auto below = [&](int b) { return m - ((float)b + 0.6f) / scale - 1e-6f * (fabsf(m) + (float)b / scale); };
+        const bool flat = !(scale > 0.0f);
+        const float b_hi = flat ? INFINITY : above(w.b0), b_lo = flat ? -INFINITY : below(w.b1);
+        const float c_hi = flat ? INFINITY : above(w.c0), c_lo = flat ? -INFINITY : below(w.c1);
+        for_logits([&](int i, const float (&l)[4]) {
+            bool in[4];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const unsigned b = interval(l[v], m, scale);
-                bool is = b - b0 <= span_b || b - c0 <= span_c;
-                if (w.kind == 1 && is) {
-                    const u64 e = entry(i + v);
-                    is = e >= w.lo && e <= w.hi;
-                }
-                in |= (unsigned)is << v;
-            }
-            for (; in; in &= in - 1) f(i + __ffs(in) - 1);
-        }
+            for (int v = 0; v < 4; ++v) in[v] = (l[v] >= b_lo & l[v] <= b_hi) | (l[v] >= c_lo & l[v] <= c_hi);
+            if (in[0] | in[1] | in[2] | in[3])
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    if (in[v]) {
+                        const float x = finite(l[v]), b = interval(x, m, scale) - SM_INTERVAL;
+                        if (!((b >= w.b0 && b <= w.b1) || (b >= w.c0 && b <= w.c1))) continue;
+                        if (exact) {
+                            const u64 e = entry(i + v, x);
+                            if (e < w.lo || e > w.hi) continue;
+                        }
+                        f(i + v, x);
+                    }
+        }, Look());
     };
     // the window's entries, sorted, and their running masses (first CTA: S.all, S.mine); at most SM_LIST
     auto collect = [&]() {
         if (tid == 0) S.n_mine = 0;
         __syncthreads();
-        for_window([&](int i) {
+        for_window([&](int i, float l) {
             const unsigned at = atomicAdd(&S.n_mine, 1u);
-            if (at < SM_LIST) S.mine[at] = entry(i);
+            if (at < SM_LIST) S.mine[at] = entry(i, l);
         });
         __syncthreads();
         // into the first CTA's list, behind what others have put there; nobody looks at this CTA's memory any more
@@ -434,9 +504,9 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
         if (first_cta) {
             total = (int)min(S.n_all, (unsigned)SM_LIST);
             sort_down(S.all, S.mine, total);
-            for (int i = tid; i < total; i += SM_THREADS) S.mine[i] = to_mass(weight(entry_logit(S.all[i]), m64, log2e_t, S.table));
+            for (int i = tid; i < total; i += SM_THREADS) S.mine[i] = mass(entry_logit(S.all[i]));
             __syncthreads();
-            running_sums(nullptr, S.mine, total, S);
+            running_sums<SM_LIST / SM_THREADS>(nullptr, S.mine, total, S);
         }
         return total;
     };
@@ -454,8 +524,8 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
         while (S.w[wp].count > SM_LIST) {
             // the range of the window's entries
             u64 e_lo = ~0ull, e_hi = 0;
-            for_window([&](int i) {
-                const u64 e = entry(i);
+            for_window([&](int i, float l) {
+                const u64 e = entry(i, l);
                 e_lo = min(e_lo, e), e_hi = max(e_hi, e);
             });
 #pragma unroll
@@ -474,18 +544,18 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
             cluster_sync();
             for (int c = 0; c < C; ++c) e_lo = min(e_lo, S.slot_a[c]), e_hi = max(e_hi, S.slot_b[c]);
             int shr = 0;
-            while ((e_hi - e_lo) >> shr >= SM_BINS) ++shr;
-            for_window([&](int i) {
-                const unsigned b = (unsigned)((e_hi - entry(i)) >> shr);
+            while ((e_hi - e_lo) >> shr >= SM_LIST) ++shr;
+            for_window([&](int i, float l) {
+                const unsigned b = (unsigned)((e_hi - entry(i, l)) >> shr);
                 atomicAdd(&S.cnt[b], 1u);
-                add_to(b, to_mass(weight(data[i], m64, log2e_t, S.table)));
+                add_to(b, mass(l));
             });
             unsigned *c_run = (unsigned *)S.all;   // (no list is in use)
-            merge(c_run, S.mine);
+            merge(c_run, S.mine, true, std::integral_constant<int, SM_LIST>());
             if (first_cta) {
                 next = S.w[wp];
                 const u64 left = t - (by_mass ? next.base_mass : next.base_count);
-                const int b = by_mass ? first_over(S.mine, SM_BINS, left, answer()) : first_over(c_run, SM_BINS, left, answer());
+                const int b = by_mass ? first_over(S.mine, SM_LIST, left, answer()) : first_over(c_run, SM_LIST, left, answer());
                 const u64 c_before = b ? c_run[b - 1] : 0;
                 next.kind = 1;
                 next.hi = e_hi - ((u64)b << shr);
@@ -501,36 +571,51 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
     };
     auto share = [&](double of, u64 total) { return (u64)fmin(of * (double)total, (double)total); };   // (cut off, not rounded)
 
-    bool with_mass = k == 0 || k > SM_LIST / 2;
+    u64 sum_min = 0;   // mass of M among this thread's logits
+    auto histogram = [&](auto counts, auto masses) {
+        // (byte address of an interval's sum from its float; what has no weight goes behind the intervals)
+        const uint32_t at0 = mx::smem_u32(S.cnt) - 4u * __float_as_uint(SM_INTERVAL), none = mx::smem_u32(&S.cnt[SM_BINS + lane]);
+        constexpr uint32_t TO_LO = sizeof(S.cnt), TO_HI = 2 * sizeof(S.cnt);
+        for_logits([&](int, const float (&raw)[4]) {
+            uint32_t at[4];
+            float l[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                l[v] = finite(raw[v]);
+                const float x = interval(l[v], m, scale);
+                at[v] = x < SM_INTERVAL + SM_BINS ? at0 + 4u * __float_as_uint(x) : none;
+                if constexpr (decltype(counts)::value) asm volatile("red.shared.add.u32 [%0], 1;" ::"r"(at[v]) : "memory");
+            }
+            if constexpr (decltype(masses)::value) {
+                u64 ms[4];
+                unsigned old[4];
+#pragma unroll
+                for (int v = 0; v < 4; ++v) ms[v] = mass(l[v]);
+                // (the four sums' low words together, then what is carried)
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    asm volatile("atom.shared.add.u32 %0, [%1], %2;" : "=r"(old[v]) : "r"(at[v] + TO_LO), "r"((unsigned)ms[v]) : "memory");
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const unsigned h = (unsigned)(ms[v] >> 32) + (old[v] + (unsigned)ms[v] < old[v]);
+                    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p red.shared.add.u32 [%0], %1;\n\t}" ::"r"(at[v] + TO_HI), "r"(h)
+                                 : "memory");
+                }
+                if (has_min)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+                        if (at[v] != none && l[v] >= m_low && (l[v] >= m_high || weight((double)l[v] - m64, log2e_t, P.power) >= min_w)) sum_min += ms[v];
+            }
+        }, Weigh());
+    };
     u64 z = 0, z_min = 0;   // first CTA: mass of K, then of what is kept; of M
     for (;;) {
         // ---- histogram over max - l ----
         clear();
-        u64 sum_min = 0;
-        for (int i = tid * 4; i < n; i += SM_THREADS * 4) {
-            const float4 l4 = *(const float4 *)(data + i);
-            const float l[4] = {l4.x, l4.y, l4.z, l4.w};
-            if (with_mass) {
-                double w[4];
-#pragma unroll
-                for (int v = 0; v < 4; ++v) w[v] = weight(fmaxf(l[v], floor_l), m64, log2e_t, S.table);
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    const unsigned b = interval(l[v], m, scale);
-                    const u64 mass = to_mass(w[v]);
-                    if (b >= SM_BINS) continue;
-                    atomicAdd(&S.cnt[b], 1u);
-                    add_to(b, mass);
-                    if (min_w > 0.0 && w[v] >= min_w) sum_min += mass;
-                }
-            } else {
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    const unsigned b = interval(l[v], m, scale);
-                    if (b < SM_BINS) atomicAdd(&S.cnt[b], 1u);
-                }
-            }
-        }
+        sum_min = 0;
+        if (!with_mass) histogram(std::true_type(), std::false_type());
+        else if (with_count) histogram(std::true_type(), std::true_type());
+        else histogram(std::false_type(), std::true_type());
         if (with_mass && min_w > 0.0) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum_min += __shfl_xor_sync(0xFFFFFFFFu, sum_min, o);
@@ -541,7 +626,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
                 st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_b[rank]), 0), sum_min);
             }
         }
-        merge(S.run_cnt, S.run_mass);
+        merge(S.run_cnt, S.run_mass, with_count, std::integral_constant<int, SM_BINS>());
         // ---- what is to be looked at: all that can be kept, if that is a list; else (k = 0) the interval where P ends and those where
         // the token then can be, if they are; else more than that ----
         Window next{};
@@ -585,11 +670,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
         const Window w = S.w[wp];
         const bool one = w.c1 == w.b1;
         const u64 front = w.c0 ? S.run_mass[w.c0 - 1] : 0;
-        u64 between = 0;
-        if (!one) {
-            const u64 in_c = S.mine[S.run_cnt[w.c1] - (w.c0 ? S.run_cnt[w.c0 - 1] : 0) - 1];
-            between = S.run_mass[w.b0 - 1] - front - in_c;
-        }
+        const u64 in_c = S.run_mass[w.c1] - front, between = one ? 0 : S.run_mass[w.b0 - 1] - S.run_mass[w.c1];
         if (k) z = S.mine[min(k, total) - 1];
         u64 keep = z;
         if (p < 1.0f) keep = front + between + S.mine[first_over(S.mine, total, (u64)ceil((double)p * (double)z) - 1 - front - between, answer())];
@@ -599,15 +680,14 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams P
                 if (tid == 0) S.low = 0;
                 __syncthreads();
                 for (int i = tid; i < total; i += SM_THREADS)
-                    if (weight(entry_logit(S.all[i]), m64, log2e_t, S.table) >= min_w) atomicMax(&S.low, S.mine[i]);
+                    if (weight((double)entry_logit(S.all[i]) - m64, log2e_t, P.power) >= min_w) atomicMax(&S.low, S.mine[i]);
                 __syncthreads();
                 keep = min(keep, S.low);
             }
         }
         z = keep;
         const u64 t = min(share((double)u, z), z - 1) - front;
-        // (behind c: in b)
-        at = first_over(S.mine, total, one || t < S.mine[S.run_cnt[w.c1] - (w.c0 ? S.run_cnt[w.c0 - 1] : 0) - 1] ? t : t - between, answer());
+        at = first_over(S.mine, total, one || t < in_c ? t : t - between, answer());   // (else behind c, in b)
     } else {
         if (k) {
             const int i = search(first_cta ? (u64)min((unsigned)k, S.run_cnt[SM_BINS - 1]) - 1 : 0, false);
@@ -632,15 +712,21 @@ template <typename T>
 int launch_sample(mx230_handle *h, cudaStream_t st, SampleParams P, int n_rows) {
     constexpr int VE = 16 / (int)sizeof(T);
     const int pieces = P.vocab / VE + 2;
-    // Smallest cluster whose CTAs can hold the row; more CTAs while SMs have none and each still has a few thousand logits.
+    // CTAs of a row: up to four while there are no three of them for every SM, eight for a few rows (clusters of eight that fill their
+    // SMs find few places: 16 rows of 128000, kept, 26 us with eight, 19 with four; one row 21 and 28), each with a few thousand logits.
     int c = 1;
-    auto share_of = [&](int n) { return ((pieces + n - 1) / n + 1) * VE; };
-    while (c < SM_CLUSTER && share_of(c) > SM_MAX_DATA) c *= 2;
-    while (c < SM_CLUSTER && (long long)n_rows * c < 2ll * h->sm_count && P.vocab / c > 4096) c *= 2;
-    P.ctas = c, P.cap = share_of(c);
-    const size_t sm = sizeof(Shared) + (size_t)P.cap * sizeof(float);
-    MX_SMEM_ATTR_ONCE(h->device, sample_kernel<T>, 227 * 1024);
-    MX_LAUNCH(h, st, MX230_K_SAMPLE, mx_launch(sample_kernel<T>, dim3((unsigned)(n_rows * c)), SM_THREADS, sm, st, c, true, P));
+    while (c < SM_CLUSTER && (long long)n_rows * 2 * c <= (c < 4 ? 3 * h->sm_count : h->sm_count / 2) && P.vocab / c > 4096) c *= 2;
+    const int share = ((pieces + c - 1) / c + 1) * VE;
+    P.ctas = c;
+    P.power = POWER_OF_TWO;
+    const dim3 grid((unsigned)(n_rows * c));
+    // The row stays in shared memory where its CTAs all have their places with that (32 rows of 128000, four CTAs each: 33 us, read
+    // again 45); else it is read again (64 rows: 51, kept 62).
+    const size_t kept = sizeof(Shared) + (size_t)share * sizeof(float);
+    MX_SMEM_ATTR_ONCE(h->device, (sample_kernel<T, true>), SM_ALL);
+    MX_SMEM_ATTR_ONCE(h->device, (sample_kernel<T, false>), sizeof(Shared));
+    if ((kept <= SM_HALF && (long long)n_rows * c <= 2ll * h->sm_count) || (kept <= SM_ALL && (long long)n_rows * c <= h->sm_count)) MX_LAUNCH(h, st, MX230_K_SAMPLE, mx_launch(sample_kernel<T, true>, grid, SM_THREADS, kept, st, c, true, P));
+    else MX_LAUNCH(h, st, MX230_K_SAMPLE, mx_launch(sample_kernel<T, false>, grid, SM_THREADS, sizeof(Shared), st, c, true, P));
     return MX230_OK;
 }
 
@@ -652,8 +738,7 @@ extern "C" int mx230_sample(mx230_handle *h, void *stream, int *token, float *pr
     MX_REQUIRE(h, MX230_ERR_INVALID_ARG, "sample: null handle");
     MX_REQUIRE(dtype == MX230_F32 || dtype == MX230_F16 || dtype == MX230_BF16, MX230_ERR_INVALID_ARG, "sample: element type %d", dtype);
     MX_REQUIRE(n_rows >= 0 && vocab > 0, MX230_ERR_INVALID_ARG, "sample: %d rows of %d logits", n_rows, vocab);
-    MX_REQUIRE(vocab <= SM_CLUSTER * (SM_MAX_DATA - 32), MX230_ERR_UNSUPPORTED, "sample: %d logits a row (at most %d)", vocab,
-               SM_CLUSTER * (SM_MAX_DATA - 32));
+    MX_REQUIRE(vocab <= SM_MAX, MX230_ERR_UNSUPPORTED, "sample: %d logits a row (at most %d)", vocab, SM_MAX);
     MX_REQUIRE(n_rows <= (1 << 27), MX230_ERR_UNSUPPORTED, "sample: %d rows", n_rows);
     if (n_rows == 0) return MX230_OK;
     MX_REQUIRE(token && logits && u, MX230_ERR_INVALID_ARG, "sample: null argument");

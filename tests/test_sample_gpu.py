@@ -89,9 +89,28 @@ def test_matches_the_definition(handle, vocab, dtype, s):
 
 
 def test_the_largest_vocabulary(handle):
-    x = logits_of(2, 360192, 2.0, 5, torch.float32)
+    x = logits_of(1, 1 << 22, 2.0, 5, torch.float32)
     for s in (dict(p=0.9), dict(k=50), dict(t=50.0, k=100_000, p=0.9)):
-        check(handle, x, [0.3, 0.999], **s)
+        check(handle, x, [0.3], **s)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,vocab", [(40, 128000), (160, 50257), (300, 7001), (19, 200003)])
+def test_batches_of_every_size(handle, n, vocab, dtype):
+    """Rows over eight CTAs to one, kept in shared memory or read again: the tokens of the same rows by themselves, and some rows
+    against the definition."""
+    x = logits_of(4, vocab, 2.0, vocab, dtype).repeat(-(-n // 4), 1)[:n].cuda()
+    u = torch.rand(n, generator=torch.Generator().manual_seed(n)).cuda()
+    for s in (dict(top_p=0.95), dict(temperature=0.8, top_k=40, top_p=0.9), dict(min_p=0.02), dict(temperature=0.0), dict(temperature=3.0, top_k=3000)):
+        token, one, prob = (torch.empty(n, dtype=t, device="cuda") for t in (torch.int32, torch.int32, torch.float32))
+        serving.sample(handle, token, x, u, **s, prob=prob)
+        for r in range(0, n, 7):
+            serving.sample(handle, one[r:r + 1], x[r:r + 1], u[r:r + 1], **s)
+        assert torch.equal(token[::7], one[::7]), s
+        rows = x[:2].float().cpu().numpy()
+        for r in range(2):
+            want = draw(rows[r], u[r].item(), s.get("temperature", 1.0), s.get("top_k", 0), s.get("top_p", 1.0), s.get("min_p", 0.0))
+            assert token[r].item() == want[0] and abs(prob[r].item() - want[1]) < 1e-7, (s, r)
 
 
 def test_settings_of_each_row(handle):
@@ -192,5 +211,5 @@ def test_refusals(handle):
             call()
         assert e.value.code == _lib.ERR_INVALID_ARG
     with pytest.raises(_lib.Mx230Error) as e:
-        serving.sample(handle, tok[:1], torch.zeros(1, 400_000, device="cuda"), u[:1])
+        serving.sample(handle, tok[:1], torch.zeros(1, (1 << 22) + 1, device="cuda"), u[:1])
     assert e.value.code == _lib.ERR_UNSUPPORTED

@@ -78,6 +78,6 @@ def test_sample_refuses(L):
              dict(ps=P + 3), dict(ms=P + 2)]
     for c in cases:
         assert L.mx230_sample(*{**ok, **c}.values()) == _lib.ERR_INVALID_ARG, c
-    assert L.mx230_sample(*{**ok, "vocab": 360193}.values()) == _lib.ERR_UNSUPPORTED
+    assert L.mx230_sample(*{**ok, "vocab": (1 << 22) + 1}.values()) == _lib.ERR_UNSUPPORTED
     assert L.mx230_sample(*{**ok, "rows": 1 << 28}.values()) == _lib.ERR_UNSUPPORTED
     assert L.mx230_sample(*{**ok, "rows": 0}.values()) == 0
