@@ -22,7 +22,7 @@ namespace {
 
 constexpr int RT_THREADS = 256;
 constexpr int RT_PAIRS = 2048;    // angles in shared memory, most
-constexpr int RT_UNROLL = 4;      // heads whose loads a thread has in flight
+constexpr int RT_UNROLL = 2;      // heads whose loads a thread has in flight
 
 struct RotaryParams {
     void *out;
@@ -37,20 +37,55 @@ struct RotaryParams {
     long long x_row, x_head, out_row, out_head;   // in elements
 };
 
-template <typename T> __device__ __forceinline__ float to_f(T v);
-template <> __device__ __forceinline__ float to_f(float v) { return v; }
-template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T from_f(float v);
-template <> __device__ __forceinline__ float from_f(float v) { return v; }
-template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
-
-// N elements of T, loaded and stored together
+// N elements of T, loaded and stored together, and as floats (16-bit ones by twos)
 template <typename T, int N>
 struct alignas(sizeof(T) * N) Piece {
     T v[N];
 };
+template <int N>
+__device__ __forceinline__ void unpack(const Piece<float, N> &p, float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = p.v[i];
+}
+template <int N>
+__device__ __forceinline__ void pack(Piece<float, N> &p, const float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p.v[i] = f[i];
+}
+template <int N>
+__device__ __forceinline__ void unpack(const Piece<__half, N> &p, float (&f)[N]) {
+    if constexpr (N == 1) f[0] = __half2float(p.v[0]);
+    else
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 t = __half22float2(*(const __half2 *)&p.v[i]);
+            f[i] = t.x, f[i + 1] = t.y;
+        }
+}
+template <int N>
+__device__ __forceinline__ void pack(Piece<__half, N> &p, const float (&f)[N]) {
+    if constexpr (N == 1) p.v[0] = __float2half_rn(f[0]);
+    else
+#pragma unroll
+        for (int i = 0; i < N; i += 2) *(__half2 *)&p.v[i] = __floats2half2_rn(f[i], f[i + 1]);
+}
+template <int N>
+__device__ __forceinline__ void unpack(const Piece<__nv_bfloat16, N> &p, float (&f)[N]) {
+    if constexpr (N == 1) f[0] = __bfloat162float(p.v[0]);
+    else
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const uint32_t w = *(const uint32_t *)&p.v[i];
+            f[i] = __uint_as_float(w << 16), f[i + 1] = __uint_as_float(w & 0xFFFF0000u);
+        }
+}
+template <int N>
+__device__ __forceinline__ void pack(Piece<__nv_bfloat16, N> &p, const float (&f)[N]) {
+    if constexpr (N == 1) p.v[0] = __float2bfloat16_rn(f[0]);
+    else
+#pragma unroll
+        for (int i = 0; i < N; i += 2) *(uint32_t *)&p.v[i] = mx::pack_bf16(f[i], f[i + 1]);
+}
 
 // cos and sin of `t` * 2^-64 turns: the nearest quarter turn is taken off as an integer, so that what is left has 27 bits behind
 // the point as a float, and put back by exchanging and negating.
@@ -69,7 +104,7 @@ __device__ __forceinline__ float2 turn_cos_sin(uint64_t t) {
 // behind are pieces of what is not rotated.  INTER: unit u is a piece of the head; N == 1 stands for pairs (and single elements of
 // the rest) by themselves, in either layout.  IN_PLACE: what is not rotated stays as it is.
 template <typename T, int N, bool INTER>
-__global__ void __launch_bounds__(RT_THREADS) rotary_kernel(const RotaryParams P) {
+__global__ void __launch_bounds__(RT_THREADS, 4) rotary_kernel(const RotaryParams P) {
     __shared__ float2 cs[RT_PAIRS];
     mx::pdl_trigger();
     mx::pdl_wait();
@@ -101,46 +136,51 @@ __global__ void __launch_bounds__(RT_THREADS) rotary_kernel(const RotaryParams P
         // items (row, head) of this slot: slot, slot + slots, ...
         int r = slot / nh, h = slot - r * nh;
         const int dr = P.slots / nh, dh = P.slots - dr * nh;
+        const T *src = x + (long long)(r0 + r) * P.x_row + (long long)(h0 + h) * P.x_head;
+        T *dst = out + (long long)(r0 + r) * P.out_row + (long long)(h0 + h) * P.out_head;
+        const long long src_step = dr * P.x_row + dh * P.x_head, dst_step = dr * P.out_row + dh * P.out_head;
+        const long long src_wrap = src_step + P.x_row - nh * P.x_head, dst_wrap = dst_step + P.out_row - nh * P.out_head;
         while (r < nr) {
             Piece<T, N> a[RT_UNROLL], b[RT_UNROLL];
-            int ri[RT_UNROLL], hi[RT_UNROLL];
+            T *to[RT_UNROLL];
+            int ri[RT_UNROLL];
 #pragma unroll
             for (int k = 0; k < RT_UNROLL; ++k) {
-                ri[k] = r, hi[k] = h;
+                ri[k] = r, to[k] = dst;
                 if (r < nr) {
-                    const T *src = x + (long long)(r0 + r) * P.x_row + (long long)(h0 + h) * P.x_head;
                     a[k] = *(const Piece<T, N> *)(src + d0);
                     if (two) b[k] = *(const Piece<T, N> *)(src + d1);
                 }
                 r += dr, h += dh;
-                if (h >= nh) h -= nh, ++r;
+                const bool wrap = h >= nh;
+                if (wrap) h -= nh, ++r;
+                src += wrap ? src_wrap : src_step, dst += wrap ? dst_wrap : dst_step;
             }
 #pragma unroll
             for (int k = 0; k < RT_UNROLL; ++k) {
                 if (ri[k] >= nr) break;
                 const float2 *c = cs + ri[k] * half;
-                if (INTER && !SINGLE) {
+                float f[N];
+                unpack(a[k], f);
+                if constexpr (INTER && !SINGLE) {
 #pragma unroll
-                    for (int e = 0; e < N; e += 2) {
+                    for (int e = 0; e + 1 < N; e += 2) {
                         const int p = (d0 + e) >> 1;
-                        if (p < half) {
-                            float x1 = to_f(a[k].v[e]), x2 = to_f(a[k].v[e + (N > 1)]);
-                            mx::rope_pair(x1, x2, c[p].x, c[p].y);
-                            a[k].v[e] = from_f<T>(x1), a[k].v[e + (N > 1)] = from_f<T>(x2);
-                        }
+                        if (p < half) mx::rope_pair(f[e], f[e + 1], c[p].x, c[p].y);
                     }
+                    pack(a[k], f);
                 } else if (rot) {
+                    float g[N];
+                    unpack(b[k], g);
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
                         const float2 t = c[SINGLE ? u : d0 + e];
-                        float x1 = to_f(a[k].v[e]), x2 = to_f(b[k].v[e]);
-                        mx::rope_pair(x1, x2, t.x, t.y);
-                        a[k].v[e] = from_f<T>(x1), b[k].v[e] = from_f<T>(x2);
+                        mx::rope_pair(f[e], g[e], t.x, t.y);
                     }
+                    pack(a[k], f), pack(b[k], g);
                 }
-                T *dst = out + (long long)(r0 + ri[k]) * P.out_row + (long long)(h0 + hi[k]) * P.out_head;
-                *(Piece<T, N> *)(dst + d0) = a[k];
-                if (two) *(Piece<T, N> *)(dst + d1) = b[k];
+                *(Piece<T, N> *)(to[k] + d0) = a[k];
+                if (two) *(Piece<T, N> *)(to[k] + d1) = b[k];
             }
         }
     }
@@ -165,9 +205,9 @@ int launch_t(mx230_handle *h, cudaStream_t st, RotaryParams P, bool inter) {
     while (n > 1 && (any & (unsigned)(n - 1))) n >>= 1;
     P.units = n == 1 ? P.half + tail : inter ? P.head_dim / n : (P.half + tail) / n;
     P.slots = P.units >= RT_THREADS ? 1 : RT_THREADS / P.units;
-    // Rows and heads of a block: enough for every thread to have RT_UNROLL heads in flight, unless that left SMs without a block.
+    // Rows and heads of a block: enough for every thread to have its heads in flight twice, unless that left SMs without a block.
     P.heads_per_block = P.n_head;
-    int rows = (RT_UNROLL * P.slots + P.n_head - 1) / P.n_head;
+    int rows = (2 * RT_UNROLL * P.slots + P.n_head - 1) / P.n_head;
     const int fill = (P.n_rows + 2 * h->sm_count - 1) / (2 * h->sm_count);
     if (rows > fill) rows = fill;
     if (rows > RT_PAIRS / P.half) rows = RT_PAIRS / P.half;
