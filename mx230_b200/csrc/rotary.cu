@@ -105,7 +105,12 @@ __device__ __forceinline__ float2 turn_cos_sin(uint64_t t) {
 // the rest) by themselves, in either layout.  IN_PLACE: what is not rotated stays as it is.
 template <typename T, int N, bool INTER>
 __global__ void __launch_bounds__(RT_THREADS, 4) rotary_kernel(const RotaryParams P) {
-    __shared__ float2 cs[RT_PAIRS];
+    // the angles of a row lie so that lanes with pieces next to each other read words next to each other: the first two pairs of
+    // every piece, then the next two (16 rows of words apart they were read four at a time: 84 us for the interleaved case of 64)
+    __shared__ __align__(16) float2 cs[RT_PAIRS];
+    constexpr int PAIRS = INTER ? (N > 1 ? N / 2 : 1) : N;     // of a piece
+    const int pieces = (P.half + PAIRS - 1) / PAIRS, row_cs = pieces * PAIRS;
+    auto place = [&](int p) { return PAIRS == 1 ? p : (p % PAIRS / 2 * pieces + p / PAIRS) * 2 + (p & 1); };
     mx::pdl_trigger();
     mx::pdl_wait();
     const int half = P.half, tid = threadIdx.x;
@@ -116,7 +121,7 @@ __global__ void __launch_bounds__(RT_THREADS, 4) rotary_kernel(const RotaryParam
         const long long pos = P.pos ? (long long)P.pos[r0 + r] : (long long)P.pos0 + r0 + r;
         float2 a = turn_cos_sin((uint64_t)pos * P.turns[p]);
         a.x *= P.factor, a.y *= P.inverse ? -P.factor : P.factor;
-        cs[i] = a;
+        cs[r * row_cs + place(p)] = a;
     }
     __syncthreads();
     const T *x = (const T *)P.x;
@@ -159,24 +164,30 @@ __global__ void __launch_bounds__(RT_THREADS, 4) rotary_kernel(const RotaryParam
 #pragma unroll
             for (int k = 0; k < RT_UNROLL; ++k) {
                 if (ri[k] >= nr) break;
-                const float2 *c = cs + ri[k] * half;
+                const float2 *c = cs + ri[k] * row_cs;
+                float2 t[PAIRS];
+                if constexpr (PAIRS == 1) {
+                    if (rot) t[0] = c[INTER && !SINGLE ? min(u, half - 1) : u];
+                } else if (rot) {
+                    const int v = min(u, pieces - 1);   // (behind the rotated part: not used)
+#pragma unroll
+                    for (int q = 0; q < PAIRS; q += 2) {
+                        const float4 two_pairs = *(const float4 *)(c + (q / 2 * pieces + v) * 2);
+                        t[q] = make_float2(two_pairs.x, two_pairs.y), t[q + 1] = make_float2(two_pairs.z, two_pairs.w);
+                    }
+                }
                 float f[N];
                 unpack(a[k], f);
                 if constexpr (INTER && !SINGLE) {
 #pragma unroll
-                    for (int e = 0; e + 1 < N; e += 2) {
-                        const int p = (d0 + e) >> 1;
-                        if (p < half) mx::rope_pair(f[e], f[e + 1], c[p].x, c[p].y);
-                    }
+                    for (int e = 0; e + 1 < N; e += 2)
+                        if ((d0 + e) >> 1 < half) mx::rope_pair(f[e], f[e + 1], t[e / 2].x, t[e / 2].y);
                     pack(a[k], f);
                 } else if (rot) {
                     float g[N];
                     unpack(b[k], g);
 #pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const float2 t = c[SINGLE ? u : d0 + e];
-                        mx::rope_pair(f[e], g[e], t.x, t.y);
-                    }
+                    for (int e = 0; e < N; ++e) mx::rope_pair(f[e], g[e], t[e].x, t[e].y);
                     pack(a[k], f), pack(b[k], g);
                 }
                 *(Piece<T, N> *)(to[k] + d0) = a[k];
@@ -210,7 +221,8 @@ int launch_t(mx230_handle *h, cudaStream_t st, RotaryParams P, bool inter) {
     int rows = (2 * RT_UNROLL * P.slots + P.n_head - 1) / P.n_head;
     const int fill = (P.n_rows + 2 * h->sm_count - 1) / (2 * h->sm_count);
     if (rows > fill) rows = fill;
-    if (rows > RT_PAIRS / P.half) rows = RT_PAIRS / P.half;
+    const int pairs = n == 1 ? 1 : inter ? n / 2 : n, row_cs = (P.half + pairs - 1) / pairs * pairs;
+    if (rows > RT_PAIRS / row_cs) rows = RT_PAIRS / row_cs;
     if (rows < 1) rows = 1;
     P.rows_per_block = rows;
     // few rows: the heads of a row over several blocks
