@@ -32,8 +32,7 @@ constexpr int W4_N = 16;          // outputs of a tile
 constexpr int W4_WARPS = 8;
 constexpr int W4_THREADS = W4_WARPS * 32;
 constexpr int W4_CLUSTER = 8;     // most CTAs whose sums are added through shared memory
-constexpr int W4_X_BYTES = 32 * 1024;   // of shared memory for rows, about
-constexpr int SLICE_WARPS = 16, TWO_WARPS = 16, KW_MOST = 8;
+constexpr int W4_X_BYTES = 80 * 1024;   // of shared memory for rows, about: an SM holds two CTAs
 
 struct Int4Params {
     float *y;
@@ -44,6 +43,8 @@ struct Int4Params {
     int n_rows, n_in, n_out, group, groups;
     int n_tiles, k_tiles;
     int kw, ctas_k;          // warps of a CTA along the inputs, CTAs of a cluster; kw * ctas_k slices
+    int n_groups, n_clusters;   // of output tiles that a cluster computes at a time; clusters, each with every n_clusters-th of them
+    int buffers;             // of sums: two where a cluster has more than one of them
     int xq;                  // tiles of a slice whose rows are in shared memory at a time
     int x_vec;               // rows are 16-byte aligned
     long long x_stride, y_stride, add_stride;
@@ -89,6 +90,9 @@ __device__ __forceinline__ uint4 ld_stream(const uint4 *p) {
     return v;
 }
 
+__device__ __forceinline__ void prefetch_bulk(const void *src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ uint32_t h2_u(__half2 v) { return *(uint32_t *)&v; }
 __device__ __forceinline__ __half2 u_h2(uint32_t v) { return *(__half2 *)&v; }
 
@@ -121,74 +125,95 @@ __device__ __forceinline__ float tree_sum(const float *p, int n, int step) {
 }
 
 // NT: column tiles of four rows.  T: output tiles of a warp.  G32: groups of 32 inputs (else a multiple of 64).
-// Shared memory: sums [8 warps][T * NT * 64], in the first CTA of a cluster also the other CTAs' sums; per (slice, tile, row)
-// {2^-e, 2^(e - 24) sum x, or that of either half}; 32 bytes of zeros; rows [kw][xq][NT][lanes][8 words].
-// DEPTH tiles of every output tile are on their way to a warp's registers.
-constexpr int DEPTH = 4;
+// Shared memory: sums [buffers][8 warps][T * NT * 64]; in clusters, this CTA's share of everybody's sums [buffers][C][8 / kw * T * NT *
+// 64 / C]; per (slice, tile, row) {2^-e, 2^(e - 24) sum x, or that of either half}; 32 bytes of zeros; rows [kw][xq][NT][lanes][8 words].
+// A warp has DEPTH tiles of each of its output tiles on their way to its registers, across the end of a group of output tiles too.
 template <int NT, int T, bool G32>
-struct Int4Smem {
+struct Int4Form {
     static constexpr int SUMS = T * NT * 64;                // floats of a warp
+    static constexpr int DEPTH = T == 4 ? 2 : 4;
 };
 
 template <int NT, int T, bool G32>
-__global__ void __launch_bounds__(W4_THREADS) gemv_int4_kernel(const Int4Params P) {
-    using S = Int4Smem<NT, T, G32>;
+__global__ void __launch_bounds__(W4_THREADS, 2) gemv_int4_kernel(const Int4Params P) {
+    using S = Int4Form<NT, T, G32>;
+    constexpr int DEPTH = S::DEPTH;
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
     const int kw = P.kw, tg = W4_WARPS / kw, C = P.ctas_k;
-    const int rank = blockIdx.x % C, grp = blockIdx.x / C;
+    const int rank = blockIdx.x % C, grp0 = blockIdx.x / C;
     const int row0 = blockIdx.y * (4 * NT), rows = min(4 * NT, P.n_rows - row0);
     const int rt = NT == 1 ? rows : 4;                      // rows of a column tile that are there at all
     const int x_lanes = 8 * rt;
-    float *sums = (float *)smem;                            // [8][SUMS]
-    float *parts = sums + W4_WARPS * S::SUMS;               // [C][tg][SUMS], first CTA
-    float4 *xrow = (float4 *)(parts + (C > 1 ? C * tg * S::SUMS : 0));   // [kw][xq][NT * 4]
+    const int entries = tg * S::SUMS, share = entries / C;  // sums of the CTA; those it finishes
+    float *sums = (float *)smem;                            // [buffers][8][SUMS]
+    float *parts = sums + P.buffers * W4_WARPS * S::SUMS;   // [buffers][C][share]
+    float4 *xrow = (float4 *)(parts + (C > 1 ? P.buffers * entries : 0));   // [kw][xq][NT * 4]
     uint4 *zeros = (uint4 *)(xrow + kw * P.xq * NT * 4);    // 32 bytes
     uint4 *xf = zeros + 2;                                  // [kw][xq][NT][x_lanes][2]
 
     mx::pdl_trigger();
     if (C > 1) mx::cluster_arrive_relaxed();   // waited for before the first store to another CTA's memory
     if (tid < 2) zeros[tid] = make_uint4(0, 0, 0, 0);
+
+    // this warp's slice: tiles k0 .. k1, len of them, and steps, a multiple of DEPTH
+    const int ws = warp % kw, slice = rank * kw + ws, n_slices = C * kw;
+    const int k0 = (int)((long long)P.k_tiles * slice / n_slices), k1 = (int)((long long)P.k_tiles * (slice + 1) / n_slices);
+    const int len = k1 - k0, steps = (len + DEPTH - 1) / DEPTH * DEPTH;
+    auto first_tile = [&](int grp) { return (grp * tg + warp / kw) * T; };
+    // this warp's part of a group of output tiles into L2, from where the loads to registers are short enough (lane t of T)
+    const int per_group = G32 ? 1 : P.group / W4_K;
+    const int sz0 = G32 ? 2 * k0 : k0 / per_group, sz_len = (G32 ? min(2 * k1, P.groups) : (k1 - 1) / per_group + 1) - sz0;
+    auto prefetch = [&](int grp) {
+        const int t = first_tile(grp) + lane;
+        if (lane < T && t < P.n_tiles) {
+            prefetch_bulk(P.codes + ((size_t)t * P.k_tiles + k0) * 32, len * 512);
+            prefetch_bulk(P.sz + ((size_t)t * P.groups + sz0) * 16, sz_len * 64);
+        }
+    };
+    prefetch(grp0);   // under the previous kernel's tail
     mx::pdl_wait();
 
-    // this warp's slice and output tiles
-    const int ws = warp % kw, slice = rank * kw + ws, n_slices = C * kw;
-    const int t_first = (grp * tg + warp / kw) * T;
-    const int k0 = (int)((long long)P.k_tiles * slice / n_slices), k1 = (int)((long long)P.k_tiles * (slice + 1) / n_slices);
-    // what is requested next: tile kq, with its group gq of which left_q tiles are still to come
-    const bool any = t_first < P.n_tiles;
-    const int per_group = G32 ? 1 : P.group / W4_K;
+    // what is requested next: step q of group q_grp; its (s, z), of which left_q tiles are still to come
     const uint4 *code_q[T];
     const uint32_t *sz_q[T];
+    const int left_0 = G32 ? 1 : per_group - k0 % per_group;
+    int q_grp = grp0, q = 0, left_q = 0;
+    bool q_any = false;
+    auto aim = [&]() {
+        const int first = first_tile(q_grp);
+        q_any = first < P.n_tiles;
+        left_q = left_0;
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-        const int nt = min(t_first + t, P.n_tiles - 1);
-        code_q[t] = P.codes + ((size_t)nt * P.k_tiles + k0) * 32 + lane;
-        sz_q[t] = P.sz + ((size_t)nt * P.groups + (G32 ? 2 * k0 : k0 / per_group)) * 16 + g;
-    }
-    int kq = k0, left_q = G32 ? 1 : per_group - k0 % per_group;
+        for (int t = 0; t < T; ++t) {
+            const int nt = min(first + t, P.n_tiles - 1);
+            code_q[t] = P.codes + ((size_t)nt * P.k_tiles + k0) * 32 + lane;
+            sz_q[t] = P.sz + ((size_t)nt * P.groups + sz0) * 16 + g;
+        }
+    };
     uint4 codes[DEPTH][T];
     uint32_t sz[DEPTH][T][G32 ? 4 : 2];
     auto request = [&](int d) {
-        if (any && kq < k1) {
+        if (q_any && q < len) {
 #pragma unroll
             for (int t = 0; t < T; ++t) {
                 codes[d][t] = ld_stream(code_q[t]);
                 sz[d][t][0] = __ldg(sz_q[t]), sz[d][t][1] = __ldg(sz_q[t] + 8);
                 if (G32) {   // (a second group behind the last one: the padding of the inputs, whatever it is multiplied by is 0)
-                    const int more = 2 * kq + 1 < P.groups ? 16 : 0;
+                    const int more = 2 * (k0 + q) + 1 < P.groups ? 16 : 0;
                     sz[d][t][2] = __ldg(sz_q[t] + more), sz[d][t][3] = __ldg(sz_q[t] + more + 8);
                 }
                 code_q[t] += 32;
             }
-            ++kq;
             if (--left_q == 0) {
                 left_q = per_group;
 #pragma unroll
                 for (int t = 0; t < T; ++t) sz_q[t] += G32 ? 32 : 16;
             }
         }
+        if (++q == steps) q = 0, q_grp += P.n_clusters, aim();
     };
+    aim();
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
 #pragma unroll
@@ -200,17 +225,10 @@ __global__ void __launch_bounds__(W4_THREADS) gemv_int4_kernel(const Int4Params 
         request(d);
     }
 
-    float total[T][NT][2];
-#pragma unroll
-    for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) total[t][n][0] = total[t][n][1] = 0.0f;
-
     const int most = (P.k_tiles + n_slices - 1) / n_slices;   // tiles of the longest slice
-    for (int c0 = 0; c0 < most; c0 += P.xq) {
-        if (c0) __syncthreads();
-        // ---- rows of the next xq tiles of every slice: scaled, split, in the order of B's fragments ----
-        // a thread takes the 16 inputs (8j .. , 32 + 8j ..) of a (slice, tile, row); the four of a row follow one another
+    // rows of the next xq tiles of every slice: scaled, split, in the order of B's fragments.  A thread takes the 16 inputs (8j .. ,
+    // 32 + 8j ..) of a (slice, tile, row); the four of a row follow one another
+    auto stage_rows = [&](int c0) {
         const int rr = NT == 1 ? rt : 4 * NT, n_x = kw * P.xq * rr * 4;
         for (int i0 = tid & ~31; i0 < n_x; i0 += W4_THREADS) {   // (whole warps, for the shuffles)
             const int i = min(i0 + lane, n_x - 1);
@@ -267,99 +285,123 @@ __global__ void __launch_bounds__(W4_THREADS) gemv_int4_kernel(const Int4Params 
             dst[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]), dst[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
             dst[8] = make_uint4(lo[0], lo[1], lo[2], lo[3]), dst[9] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
         }
+    };
+    const bool has_x = lane < x_lanes;                        // columns of rows that are not there: zeros
+    const int x_step = has_x ? x_lanes * 2 : 0;
+    if (P.xq >= most) {
+        stage_rows(0);
         __syncthreads();
-        // ---- this warp's tiles ----
-        const int end = min(k1 - k0, c0 + P.xq);
-        const bool has_x = lane < x_lanes;                    // columns of rows that are not there: zeros
-        const uint4 *xp = has_x ? xf + ((size_t)ws * P.xq * NT * x_lanes + lane) * 2 : zeros;
-        const float4 *rp = xrow + ws * P.xq * (NT * 4) + (NT == 1 ? min(j, rt - 1) : j);   // the row whose sums this lane gets
-        const int x_step = has_x ? x_lanes * 2 : 0;
-        for (int k_ = c0; k_ < end; k_ += DEPTH)               // (xq is a multiple of DEPTH, or all)
+    }
+    if (C > 1) mx::cluster_wait();
+    int buf = 0;
+    for (int grp = grp0; grp < P.n_groups; grp += P.n_clusters) {
+        const bool any = first_tile(grp) < P.n_tiles;
+        float total[T][NT][2];
 #pragma unroll
-            for (int d = 0; d < DEPTH; ++d) {
-                if (k_ + d >= end) break;
-                uint4 b[NT][2];
-                float4 xr[NT];
+        for (int t = 0; t < T; ++t)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    b[n][0] = xp[0], b[n][1] = xp[1];
-                    xp += x_step;
-                    xr[n] = rp[n * 4];
-                }
-                rp += NT * 4;
+            for (int n = 0; n < NT; ++n) total[t][n][0] = total[t][n][1] = 0.0f;
+        for (int c0 = 0; c0 < most; c0 += P.xq) {
+            if (P.xq < most) {
+                __syncthreads();
+                stage_rows(c0);
+                __syncthreads();
+            }
+            const int end = c0 + P.xq >= len ? steps : c0 + P.xq;   // (xq is a multiple of DEPTH, or all)
+            const uint4 *xp = has_x ? xf + ((size_t)ws * P.xq * NT * x_lanes + lane) * 2 : zeros;
+            const float4 *rp = xrow + ws * P.xq * (NT * 4) + (NT == 1 ? min(j, rt - 1) : j);   // the row whose sums this lane gets
+            for (int k_ = c0; k_ < end; k_ += DEPTH)
 #pragma unroll
-                for (int t = 0; t < T; ++t) {
-                    const uint4 w = codes[d][t];
-                    float acc[NT][4];
-#pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {
-                        uint32_t a0[4], a1[4];
-                        pairs8(hf ? w.y : w.x, a0);
-                        pairs8(hf ? w.w : w.z, a1);
+                for (int d = 0; d < DEPTH; ++d) {
+                    if (any && k_ + d < len) {
+                        uint4 b[NT][2];
+                        float4 xr[NT];
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            if (G32 || hf == 0) mma_f16_first(acc[n], a0[0], a1[0], a0[1], a1[1], b[n][hf].x, b[n][hf].y);
-                            else mma_f16(acc[n], a0[0], a1[0], a0[1], a1[1], b[n][hf].x, b[n][hf].y);
-                            mma_f16(acc[n], a0[2], a1[2], a0[3], a1[3], b[n][hf].z, b[n][hf].w);
+                            b[n][0] = xp[0], b[n][1] = xp[1];
+                            xp += x_step;
+                            xr[n] = rp[n * 4];
                         }
-                        if (G32 || hf == 1) {
-                            const float2 s0 = __half22float2(u_h2(sz[d][t][G32 ? 2 * hf : 0])), s1 = __half22float2(u_h2(sz[d][t][G32 ? 2 * hf + 1 : 1]));
-                            const float m0 = s0.x * 0x1p24f, m1 = s1.x * 0x1p24f;
+                        rp += NT * 4;
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) {
-                                const float xs = G32 && hf ? xr[n].z : xr[n].y;
-                                total[t][n][0] = fmaf(m0, fmaf(-s0.y, xs, acc[n][0] + acc[n][1]) * xr[n].x, total[t][n][0]);
-                                total[t][n][1] = fmaf(m1, fmaf(-s1.y, xs, acc[n][2] + acc[n][3]) * xr[n].x, total[t][n][1]);
+                        for (int t = 0; t < T; ++t) {
+                            const uint4 w = codes[d][t];
+                            float acc[NT][4];
+#pragma unroll
+                            for (int hf = 0; hf < 2; ++hf) {
+                                uint32_t a0[4], a1[4];
+                                pairs8(hf ? w.y : w.x, a0);
+                                pairs8(hf ? w.w : w.z, a1);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    if (G32 || hf == 0) mma_f16_first(acc[n], a0[0], a1[0], a0[1], a1[1], b[n][hf].x, b[n][hf].y);
+                                    else mma_f16(acc[n], a0[0], a1[0], a0[1], a1[1], b[n][hf].x, b[n][hf].y);
+                                    mma_f16(acc[n], a0[2], a1[2], a0[3], a1[3], b[n][hf].z, b[n][hf].w);
+                                }
+                                if (G32 || hf == 1) {
+                                    const float2 s0 = __half22float2(u_h2(sz[d][t][G32 ? 2 * hf : 0])), s1 = __half22float2(u_h2(sz[d][t][G32 ? 2 * hf + 1 : 1]));
+                                    const float m0 = s0.x * 0x1p24f, m1 = s1.x * 0x1p24f;
+#pragma unroll
+                                    for (int n = 0; n < NT; ++n) {
+                                        const float xs = G32 && hf ? xr[n].z : xr[n].y;
+                                        total[t][n][0] = fmaf(m0, fmaf(-s0.y, xs, acc[n][0] + acc[n][1]) * xr[n].x, total[t][n][0]);
+                                        total[t][n][1] = fmaf(m1, fmaf(-s1.y, xs, acc[n][2] + acc[n][3]) * xr[n].x, total[t][n][1]);
+                                    }
+                                }
                             }
                         }
                     }
+                    request(d);
                 }
-                request(d);
+        }
+        // ---- slices of the CTA, then of the cluster, pairwise; each CTA of it finishes a share ----
+        float *mine = sums + buf * W4_WARPS * S::SUMS;
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) mine[warp * S::SUMS + ((t * NT + n) * 2 + e) * 32 + lane] = total[t][n][e];
+        __syncthreads();
+        float *theirs = parts + buf * entries;
+        if (C > 1) {
+            for (int i = tid; i < entries; i += W4_THREADS) {
+                const int gi = i / S::SUMS, e = i - gi * S::SUMS, to = i / share;
+                const float v = tree_sum(mine + gi * kw * S::SUMS + e, kw, S::SUMS);
+                const uint32_t dst = mx::cluster_map(mx::smem_u32(theirs + rank * share + i - to * share), to);
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(v) : "memory");
             }
-    }
-    // ---- slices of the CTA, then of the cluster, pairwise ----
-#pragma unroll
-    for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) sums[warp * S::SUMS + ((t * NT + n) * 2 + e) * 32 + lane] = total[t][n][e];
-    __syncthreads();
-    if (C > 1) {
-        mx::cluster_wait();
-        for (int i = tid; i < tg * S::SUMS; i += W4_THREADS) {
-            const int gi = i / S::SUMS, e = i - gi * S::SUMS;
-            const float v = tree_sum(sums + gi * kw * S::SUMS + e, kw, S::SUMS);
-            const uint32_t dst = mx::cluster_map(mx::smem_u32(parts + rank * tg * S::SUMS + i), 0);
-            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(v) : "memory");
+            mx::cluster_sync();
         }
-        mx::cluster_sync();
-        if (rank != 0) return;
-    }
-    for (int i = tid; i < tg * S::SUMS; i += W4_THREADS) {
-        const int gi = i / S::SUMS, e = i - gi * S::SUMS, l = e & 31, hf = (e >> 5) & 1, n = (e >> 6) % NT, t = (e >> 6) / NT;
-        const float v = C > 1 ? tree_sum(parts + i, C, tg * S::SUMS) : tree_sum(sums + gi * kw * S::SUMS + e, kw, S::SUMS);
-        const int o = ((grp * tg + gi) * T + t) * W4_N + (l >> 2) + 8 * hf, r = n * 4 + (l & 3);
-        if (o < P.n_out && r < rows) {
-            float out = P.bias ? v + P.bias[o] : v;
-            if (P.add) out = P.add[(long long)(row0 + r) * P.add_stride + o] + out;
-            P.y[(long long)(row0 + r) * P.y_stride + o] = out;
+        for (int i = rank * share + tid; i < (rank + 1) * share; i += W4_THREADS) {
+            const int gi = i / S::SUMS, e = i - gi * S::SUMS, l = e & 31, hf = (e >> 5) & 1, n = (e >> 6) % NT, t = (e >> 6) / NT;
+            const float v = C > 1 ? tree_sum(theirs + i - rank * share, C, share) : tree_sum(mine + gi * kw * S::SUMS + e, kw, S::SUMS);
+            const int o = ((grp * tg + gi) * T + t) * W4_N + (l >> 2) + 8 * hf, r = n * 4 + (l & 3);
+            if (o < P.n_out && r < rows) {
+                float out = P.bias ? v + P.bias[o] : v;
+                if (P.add) out = P.add[(long long)(row0 + r) * P.add_stride + o] + out;
+                P.y[(long long)(row0 + r) * P.y_stride + o] = out;
+            }
         }
+        // (the sums of the group before last are read by nobody any more: its barrier is behind all of them)
+        buf ^= P.buffers - 1;
     }
 }
 
 template <int NT, int T, bool G32>
-int launch_int4(mx230_handle *h, cudaStream_t st, Int4Params P) {
-    using S = Int4Smem<NT, T, G32>;
+int launch_int4(mx230_handle *h, cudaStream_t st, Int4Params P, int x_tile) {
+    using S = Int4Form<NT, T, G32>;
     const int tg = W4_WARPS / P.kw, C = P.ctas_k, n_slices = P.kw * C;
-    const int most = (P.k_tiles + n_slices - 1) / n_slices;
-    const int per_tile = P.kw * NT * (32 * (NT == 1 ? 8 * (P.n_rows < 4 ? P.n_rows : 4) : 32) + 64);
+    const int most = (P.k_tiles + n_slices - 1) / n_slices, per_tile = P.kw * x_tile;
     P.xq = W4_X_BYTES / per_tile;
-    P.xq = P.xq >= most ? most : P.xq < DEPTH ? DEPTH : P.xq / DEPTH * DEPTH;
-    const size_t sm = (size_t)(W4_WARPS + (C > 1 ? C * tg : 0)) * S::SUMS * 4 + 32 + (size_t)P.xq * per_tile;
+    P.xq = P.xq >= most ? most : P.xq < S::DEPTH ? S::DEPTH : P.xq / S::DEPTH * S::DEPTH;
+    P.n_groups = (int)((P.n_tiles + (long long)tg * T - 1) / ((long long)tg * T));
+    P.n_clusters = 2 * h->sm_count / C;
+    if (P.n_clusters > P.n_groups) P.n_clusters = P.n_groups;
+    P.buffers = P.n_groups > P.n_clusters ? 2 : 1;
+    const size_t sm = (size_t)P.buffers * (W4_WARPS + (C > 1 ? tg : 0)) * S::SUMS * 4 + 32 + (size_t)P.xq * per_tile;
     MX_SMEM_ATTR_ONCE(h->device, (gemv_int4_kernel<NT, T, G32>), 227 * 1024);
-    const long long groups_n = (P.n_tiles + (long long)tg * T - 1) / ((long long)tg * T);
-    const dim3 grid((unsigned)(groups_n * C), (unsigned)((P.n_rows + 4 * NT - 1) / (4 * NT)));
+    const dim3 grid((unsigned)(P.n_clusters * C), (unsigned)((P.n_rows + 4 * NT - 1) / (4 * NT)));
     MX_LAUNCH(h, st, MX230_K_GEMV_INT4, mx_launch(gemv_int4_kernel<NT, T, G32>, grid, W4_THREADS, sm, st, C, true, P));
     return MX230_OK;
 }
@@ -422,20 +464,28 @@ extern "C" int mx230_gemv_int4(mx230_handle *h, void *stream, float *y, const fl
     P.n_tiles = (int)((n_out + (long long)W4_N - 1) / W4_N), P.k_tiles = (int)((n_in + (long long)W4_K - 1) / W4_K);
     P.x_stride = x_stride, P.y_stride = y_stride, P.add_stride = add_stride;
     P.x_vec = ((uintptr_t)x & 15) == 0 && (n_rows < 2 || x_stride % 4 == 0);
-    // Slices of the inputs: enough warps for sixteen per SM, as far as there are tiles.  This fixes the order of the sums.
+    // Slices of the inputs: a CTA's eight warps, and more where there are few output tiles, each with two tiles at least.  This fixes the
+    // order of the sums.
     int n_slices = 1;
-    while (n_slices < W4_WARPS * W4_CLUSTER && 2 * n_slices <= P.k_tiles && (long long)P.n_tiles * n_slices < SLICE_WARPS * h->sm_count) n_slices *= 2;
-    const bool two = (long long)P.n_tiles * n_slices >= TWO_WARPS * h->sm_count;
-    P.kw = n_slices < KW_MOST ? n_slices : KW_MOST;
-    while (n_slices / P.kw > W4_CLUSTER) P.kw *= 2;
-    P.ctas_k = n_slices / P.kw;
+    while (n_slices < W4_WARPS && 2 * n_slices <= P.k_tiles) n_slices *= 2;
+    while (n_slices < W4_WARPS * W4_CLUSTER && 4 * n_slices <= P.k_tiles && (long long)P.n_tiles * n_slices < 16ll * h->sm_count) n_slices *= 2;
+    // CTAs of a cluster: so many that a CTA's part of the rows stays in shared memory.
+    const int nt = n_rows <= 4 ? 1 : 2, x_tile = nt * (32 * (nt == 1 ? 8 * n_rows : 32) + 64);
+    P.ctas_k = n_slices <= W4_WARPS ? 1 : n_slices / W4_WARPS;
+    while (2 * P.ctas_k <= n_slices && P.ctas_k < W4_CLUSTER && (long long)(P.k_tiles + P.ctas_k - 1) / P.ctas_k * x_tile > W4_X_BYTES) P.ctas_k *= 2;
+    P.kw = n_slices / P.ctas_k;
+    // Output tiles of a warp: as many as still leave work for nearly all CTAs that the SMs hold.
+    const int tg = W4_WARPS / P.kw, places = 2 * h->sm_count / P.ctas_k;
+    int t = nt == 1 ? 4 : 2;
+    while (t > 1 && P.n_tiles / (tg * t) < places * 3 / 4) t /= 2;
     mx230_device_guard guard(h->device);
     cudaStream_t st = (cudaStream_t)stream;
     const bool g32 = group == 32;
-    if (n_rows <= 4) {
-        if (two) return g32 ? launch_int4<1, 2, true>(h, st, P) : launch_int4<1, 2, false>(h, st, P);
-        return g32 ? launch_int4<1, 1, true>(h, st, P) : launch_int4<1, 1, false>(h, st, P);
+    if (nt == 1) {
+        if (t == 4) return g32 ? launch_int4<1, 4, true>(h, st, P, x_tile) : launch_int4<1, 4, false>(h, st, P, x_tile);
+        if (t == 2) return g32 ? launch_int4<1, 2, true>(h, st, P, x_tile) : launch_int4<1, 2, false>(h, st, P, x_tile);
+        return g32 ? launch_int4<1, 1, true>(h, st, P, x_tile) : launch_int4<1, 1, false>(h, st, P, x_tile);
     }
-    if (two) return g32 ? launch_int4<2, 2, true>(h, st, P) : launch_int4<2, 2, false>(h, st, P);
-    return g32 ? launch_int4<2, 1, true>(h, st, P) : launch_int4<2, 1, false>(h, st, P);
+    if (t == 2) return g32 ? launch_int4<2, 2, true>(h, st, P, x_tile) : launch_int4<2, 2, false>(h, st, P, x_tile);
+    return g32 ? launch_int4<2, 1, true>(h, st, P, x_tile) : launch_int4<2, 1, false>(h, st, P, x_tile);
 }
