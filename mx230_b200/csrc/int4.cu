@@ -19,8 +19,14 @@
 // 4p, input 2p + 1 at bits 16 + 4p.  (Which input a k index of the MMA stands for is free, as long as A and B agree.)  Tiles of an
 // output row follow one another along the inputs; behind all tiles, per (16 outputs, group), 16 words (s, z) of fp16.
 //
-// Order of the sums: the inputs are cut into S slices (a power of two that depends on n_in and n_out alone), each summed by one warp
-// in index order, and the slices are added pairwise.  So a row has the same bits whatever rows are computed with it.
+// Weights come by bulk copies, a lane's for a CTA of sixteen warps, into a ring of stages (some output tiles, up to 32 tiles of their
+// inputs each: 16 KB in a row and their (s, z)).  Loads to registers, two to four tiles ahead, kept too few bytes on their way with
+// the warps that fit beside them (16 of them read 5.5 TB/s with nothing else to do, 32 read 6.1), and took four instructions a
+// tile; a ring by cp.async of every lane took as many; bulk copies by the warp, of a KB, were bound by their number.
+//
+// Order of the sums: the inputs are cut over the CTAs of a cluster and there by turns over sixteen warps (a tile each), by n_in and n_out
+// alone; a warp sums in index order, then the warps' and the CTAs' sums are added pairwise.  So a row has the same bits whatever
+// rows are computed with it.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -29,10 +35,12 @@ namespace {
 
 constexpr int W4_K = 64;          // inputs of a tile
 constexpr int W4_N = 16;          // outputs of a tile
-constexpr int W4_WARPS = 8;
-constexpr int W4_THREADS = W4_WARPS * 32;
+constexpr int W4_WARPS = 16;         // that compute
+constexpr int W4_THREADS = W4_WARPS * 32, W4_PRODUCER = 32;
 constexpr int W4_CLUSTER = 8;     // most CTAs whose sums are added through shared memory
-constexpr int W4_X_BYTES = 80 * 1024;   // of shared memory for rows, about: an SM holds two CTAs
+constexpr int W4_K_CTA = 64;      // tiles of the inputs of a CTA, up to eight CTAs; then twice that
+constexpr int W4_STAGES = 6;      // most
+constexpr int W4_SMEM = 222 * 1024;
 
 struct Int4Params {
     float *y;
@@ -42,11 +50,13 @@ struct Int4Params {
     const float *bias, *add;
     int n_rows, n_in, n_out, group, groups;
     int n_tiles, k_tiles;
-    int kw, ctas_k;          // warps of a CTA along the inputs, CTAs of a cluster; kw * ctas_k slices
+    int ctas_k;              // CTAs of a cluster, each with a part of the inputs
     int n_groups, n_clusters;   // of output tiles that a cluster computes at a time; clusters, each with every n_clusters-th of them
-    int buffers;             // of sums: two where a cluster has more than one of them
-    int xq;                  // tiles of a slice whose rows are in shared memory at a time
+    int stages, stage_k;     // of the ring; tiles of the inputs in one
+    int k_cta;               // tiles of the inputs of a CTA, at most
+    uint32_t group_magic;    // 2^32 over the tiles of a group of inputs, rounded up; 0: one
     int x_vec;               // rows are 16-byte aligned
+    int *status;             // where a wait that ran out is recorded
     long long x_stride, y_stride, add_stride;
 };
 
@@ -83,16 +93,6 @@ __global__ void pack_int4_kernel(uint4 *codes_out, uint32_t *sz_out, const uint8
     }
 }
 
-// weights: read once, past the first cache
-__device__ __forceinline__ uint4 ld_stream(const uint4 *p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-
-__device__ __forceinline__ void prefetch_bulk(const void *src, uint32_t bytes) {
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ uint32_t h2_u(__half2 v) { return *(uint32_t *)&v; }
 __device__ __forceinline__ __half2 u_h2(uint32_t v) { return *(__half2 *)&v; }
 
@@ -114,128 +114,108 @@ __device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
-// pairwise sum of n (a power of two, at most 8) values `step` apart
+// pairwise sum of n (a power of two, at most 16) values `step` apart
 __device__ __forceinline__ float tree_sum(const float *p, int n, int step) {
-    float v[8];
+    float v[16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i * step] : 0.0f;
-    if (n > 1) v[0] += v[1], v[2] += v[3], v[4] += v[5], v[6] += v[7];
-    if (n > 2) v[0] += v[2], v[4] += v[6];
-    return n > 4 ? v[0] + v[4] : v[0];
+    for (int i = 0; i < 16; ++i) v[i] = i < n ? p[i * step] : 0.0f;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1)
+        if (n > o)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2 * o) v[i] += v[i + o];
+    return v[0];
 }
 
 // NT: column tiles of four rows.  T: output tiles of a warp.  G32: groups of 32 inputs (else a multiple of 64).
-// Shared memory: sums [buffers][8 warps][T * NT * 64]; in clusters, this CTA's share of everybody's sums [buffers][C][8 / kw * T * NT *
-// 64 / C]; per (slice, tile, row) {2^-e, 2^(e - 24) sum x, or that of either half}; 32 bytes of zeros; rows [kw][xq][NT][lanes][8 words].
-// A warp has DEPTH tiles of each of its output tiles on their way to its registers, across the end of a group of output tiles too.
+// Shared memory: ring [stages][T][stage_k x 512 of codes, stage_k x 64 (groups of 32: 128) of (s, z)]; sums [2][16 warps][T * NT * 64];
+// in clusters, this CTA's share of everybody's sums [2][C][T * NT * 64 / C]; per (tile, row) {2^-e, 2^(e - 24) sum x, or that
+// of either half}; 32 bytes of zeros; rows [k_cta][NT][lanes][8 words].
 template <int NT, int T, bool G32>
 struct Int4Form {
     static constexpr int SUMS = T * NT * 64;                // floats of a warp
-    static constexpr int DEPTH = T == 4 ? 2 : 4;
+    static constexpr int TILE = 512 + (G32 ? 128 : 64);     // bytes of a tile in a stage
 };
 
 template <int NT, int T, bool G32>
-__global__ void __launch_bounds__(W4_THREADS, 2) gemv_int4_kernel(const Int4Params P) {
+__global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(const Int4Params P) {
     using S = Int4Form<NT, T, G32>;
-    constexpr int DEPTH = S::DEPTH;
     extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ __align__(8) unsigned long long full[W4_STAGES], empty[W4_STAGES];
+    __shared__ int aborted;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
-    const int kw = P.kw, tg = W4_WARPS / kw, C = P.ctas_k;
+    constexpr int KW = W4_WARPS;                            // warps along the inputs, by turns
+    const int C = P.ctas_k;
     const int rank = blockIdx.x % C, grp0 = blockIdx.x / C;
     const int row0 = blockIdx.y * (4 * NT), rows = min(4 * NT, P.n_rows - row0);
     const int rt = NT == 1 ? rows : 4;                      // rows of a column tile that are there at all
     const int x_lanes = 8 * rt;
-    const int entries = tg * S::SUMS, share = entries / C;  // sums of the CTA; those it finishes
-    float *sums = (float *)smem;                            // [buffers][8][SUMS]
-    float *parts = sums + P.buffers * W4_WARPS * S::SUMS;   // [buffers][C][share]
-    float4 *xrow = (float4 *)(parts + (C > 1 ? P.buffers * entries : 0));   // [kw][xq][NT * 4]
-    uint4 *zeros = (uint4 *)(xrow + kw * P.xq * NT * 4);    // 32 bytes
-    uint4 *xf = zeros + 2;                                  // [kw][xq][NT][x_lanes][2]
+    const int share = S::SUMS / C;                          // of the CTA's sums, those that it finishes
+    const int stage_bytes = T * P.stage_k * S::TILE;
+    float *sums = (float *)(smem + P.stages * stage_bytes); // [2][16][SUMS]
+    float *parts = sums + 2 * W4_WARPS * S::SUMS;           // [2][C][share]
+    float4 *xrow = (float4 *)(parts + (C > 1 ? 2 * S::SUMS : 0));   // [k_cta][NT * 4]
+    uint4 *zeros = (uint4 *)(xrow + P.k_cta * NT * 4);      // 32 bytes
+    uint4 *xf = zeros + 2;                                  // [k_cta][NT][x_lanes][2]
+    // this CTA's inputs
+    const int k0 = (int)((long long)P.k_tiles * rank / C), k1 = (int)((long long)P.k_tiles * (rank + 1) / C);
+    // group of a tile: by a product with 2^32 / per_group, exact for the 1024 tiles there can be (0: every tile is one)
+    auto sz_group = [&](int kt) { return G32 ? 2 * kt : P.group_magic ? (int)__umulhi((uint32_t)kt, P.group_magic) : kt; };
 
     mx::pdl_trigger();
     if (C > 1) mx::cluster_arrive_relaxed();   // waited for before the first store to another CTA's memory
     if (tid < 2) zeros[tid] = make_uint4(0, 0, 0, 0);
-
-    // this warp's slice: tiles k0 .. k1, len of them, and steps, a multiple of DEPTH
-    const int ws = warp % kw, slice = rank * kw + ws, n_slices = C * kw;
-    const int k0 = (int)((long long)P.k_tiles * slice / n_slices), k1 = (int)((long long)P.k_tiles * (slice + 1) / n_slices);
-    const int len = k1 - k0, steps = (len + DEPTH - 1) / DEPTH * DEPTH;
-    auto first_tile = [&](int grp) { return (grp * tg + warp / kw) * T; };
-    // this warp's part of a group of output tiles into L2, from where the loads to registers are short enough (lane t of T)
-    const int per_group = G32 ? 1 : P.group / W4_K;
-    const int sz0 = G32 ? 2 * k0 : k0 / per_group, sz_len = (G32 ? min(2 * k1, P.groups) : (k1 - 1) / per_group + 1) - sz0;
-    auto prefetch = [&](int grp) {
-        const int t = first_tile(grp) + lane;
-        if (lane < T && t < P.n_tiles) {
-            prefetch_bulk(P.codes + ((size_t)t * P.k_tiles + k0) * 32, len * 512);
-            prefetch_bulk(P.sz + ((size_t)t * P.groups + sz0) * 16, sz_len * 64);
-        }
-    };
-    prefetch(grp0);   // under the previous kernel's tail
+    if (tid == 0) {
+        aborted = 0;
+        for (int i = 0; i < P.stages; ++i) mx::mbar_init(mx::smem_u32(&full[i]), 1), mx::mbar_init(mx::smem_u32(&empty[i]), W4_WARPS);
+        mx::mbar_fence_init();
+    }
+    __syncthreads();
     mx::pdl_wait();
 
-    // what is requested next: step q of group q_grp; its (s, z), of which left_q tiles are still to come
-    const uint4 *code_q[T];
-    const uint32_t *sz_q[T];
-    const int left_0 = G32 ? 1 : per_group - k0 % per_group;
-    int q_grp = grp0, q = 0, left_q = 0;
-    bool q_any = false;
-    auto aim = [&]() {
-        const int first = first_tile(q_grp);
-        q_any = first < P.n_tiles;
-        left_q = left_0;
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-            const int nt = min(first + t, P.n_tiles - 1);
-            code_q[t] = P.codes + ((size_t)nt * P.k_tiles + k0) * 32 + lane;
-            sz_q[t] = P.sz + ((size_t)nt * P.groups + sz0) * 16 + g;
-        }
-    };
-    uint4 codes[DEPTH][T];
-    uint32_t sz[DEPTH][T][G32 ? 4 : 2];
-    auto request = [&](int d) {
-        if (q_any && q < len) {
-#pragma unroll
-            for (int t = 0; t < T; ++t) {
-                codes[d][t] = ld_stream(code_q[t]);
-                sz[d][t][0] = __ldg(sz_q[t]), sz[d][t][1] = __ldg(sz_q[t] + 8);
-                if (G32) {   // (a second group behind the last one: the padding of the inputs, whatever it is multiplied by is 0)
-                    const int more = 2 * (k0 + q) + 1 < P.groups ? 16 : 0;
-                    sz[d][t][2] = __ldg(sz_q[t] + more), sz[d][t][3] = __ldg(sz_q[t] + more + 8);
+    if (warp == W4_WARPS) {
+        // ---- producer: the tiles of every group, stage by stage (lane 0).  In clusters the warp counts in the barrier at every group's
+        // end: it arrives once the group's stages are requested, and waits for the barrier only before it arrives at the next one ----
+        int stage = 0, parity = 1;
+        bool on = true;
+        for (int grp = grp0; grp < P.n_groups; grp += P.n_clusters) {
+            if (lane == 0 && on)
+                for (int k = k0; k < k1; k += P.stage_k) {
+                    if (!mx::mbar_wait(mx::smem_u32(&empty[stage]), parity, &aborted, P.status)) {
+                        on = false;   // (what was requested is waited for by those who read it)
+                        break;
+                    }
+                    const int n = min(P.stage_k, k1 - k), here = min(T, P.n_tiles - grp * T);
+                    const int g_first = sz_group(k), g_last = G32 ? min(2 * (k + n), P.groups) : sz_group(k + n - 1) + 1;
+                    const uint32_t bar = mx::smem_u32(&full[stage]), sz_bytes = (uint32_t)(g_last - g_first) * 64;
+                    uint32_t dst = mx::smem_u32(smem + stage * stage_bytes);
+                    mx::mbar_expect_tx(bar, here * (n * 512 + sz_bytes));
+                    for (int t = 0; t < here; ++t, dst += P.stage_k * S::TILE) {
+                        const size_t nt = (size_t)grp * T + t;
+                        mx::bulk_load(dst, P.codes + (nt * P.k_tiles + k) * 32, n * 512, bar);
+                        mx::bulk_load(dst + P.stage_k * 512, P.sz + (nt * P.groups + g_first) * 16, sz_bytes, bar);
+                    }
+                    if (++stage == P.stages) stage = 0, parity ^= 1;
                 }
-                code_q[t] += 32;
-            }
-            if (--left_q == 0) {
-                left_q = per_group;
-#pragma unroll
-                for (int t = 0; t < T; ++t) sz_q[t] += G32 ? 32 : 16;
+            __syncwarp();
+            if (C > 1) {
+                mx::cluster_wait();
+                mx::cluster_arrive_release();
             }
         }
-        if (++q == steps) q = 0, q_grp += P.n_clusters, aim();
-    };
-    aim();
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-            codes[d][t] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int e = 0; e < (G32 ? 4 : 2); ++e) sz[d][t][e] = 0;
-        }
-        request(d);
+        if (C > 1) mx::cluster_wait();
+        return;
     }
+    auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(W4_THREADS) : "memory"); };
 
-    const int most = (P.k_tiles + n_slices - 1) / n_slices;   // tiles of the longest slice
-    // rows of the next xq tiles of every slice: scaled, split, in the order of B's fragments.  A thread takes the 16 inputs (8j .. ,
-    // 32 + 8j ..) of a (slice, tile, row); the four of a row follow one another
-    auto stage_rows = [&](int c0) {
-        const int rr = NT == 1 ? rt : 4 * NT, n_x = kw * P.xq * rr * 4;
+    // ---- rows: scaled, split, in the order of B's fragments.  A thread takes the 16 inputs (8j .. , 32 + 8j ..) of a (tile, row); the
+    // four of a row follow one another ----
+    {
+        const int rr = NT == 1 ? rt : 4 * NT, n_x = (k1 - k0) * rr * 4;
         for (int i0 = tid & ~31; i0 < n_x; i0 += W4_THREADS) {   // (whole warps, for the shuffles)
             const int i = min(i0 + lane, n_x - 1);
-            const int jj = i & 3, q = (i >> 2) / rr, r = (i >> 2) - q * rr, sl = q / P.xq, kk = q - sl * P.xq;
-            const int s_ = rank * kw + sl;
-            const int kt = (int)((long long)P.k_tiles * s_ / n_slices) + c0 + kk;
-            const bool in = i0 + lane < n_x && r < rows && c0 + kk < most && kt < P.k_tiles;
+            const int jj = i & 3, q = (i >> 2) / rr, r = (i >> 2) - q * rr, kt = k0 + q;
+            const bool in = i0 + lane < n_x && r < rows;
             float v[16];
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
@@ -285,74 +265,74 @@ __global__ void __launch_bounds__(W4_THREADS, 2) gemv_int4_kernel(const Int4Para
             dst[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]), dst[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
             dst[8] = make_uint4(lo[0], lo[1], lo[2], lo[3]), dst[9] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
         }
-    };
-    const bool has_x = lane < x_lanes;                        // columns of rows that are not there: zeros
-    const int x_step = has_x ? x_lanes * 2 : 0;
-    if (P.xq >= most) {
-        stage_rows(0);
-        __syncthreads();
     }
+    sync();
     if (C > 1) mx::cluster_wait();
-    int buf = 0;
+    const bool has_x = lane < x_lanes;                        // columns of rows that are not there: zeros
+    const int x_n = has_x ? x_lanes * 2 : 0, x_step = KW * NT * x_n, tile_bytes = P.stage_k * S::TILE;
+    int stage = 0, parity = 0, buf = 0;
+    bool late = false;
     for (int grp = grp0; grp < P.n_groups; grp += P.n_clusters) {
-        const bool any = first_tile(grp) < P.n_tiles;
         float total[T][NT][2];
 #pragma unroll
         for (int t = 0; t < T; ++t)
 #pragma unroll
             for (int n = 0; n < NT; ++n) total[t][n][0] = total[t][n][1] = 0.0f;
-        for (int c0 = 0; c0 < most; c0 += P.xq) {
-            if (P.xq < most) {
-                __syncthreads();
-                stage_rows(c0);
-                __syncthreads();
+        const uint4 *xp = has_x ? xf + ((size_t)warp * NT * x_lanes + lane) * 2 : zeros;
+        const float4 *rp = xrow + warp * (NT * 4) + (NT == 1 ? min(j, rt - 1) : j);   // the row whose sums this lane gets
+        for (int k = k0; k < k1; k += P.stage_k) {
+            const uint32_t bar = mx::smem_u32(&full[stage]);
+            if (!mx::mbar_wait(bar, parity, &aborted, P.status)) {
+                // (its copies still land here: it goes on once they have, and its sums do not count)
+                for (const long long since = clock64(); !mx::mbar_try_wait(bar, parity) && clock64() - since < mx::LANDING_CYCLES;) {}
+                late = true;
             }
-            const int end = c0 + P.xq >= len ? steps : c0 + P.xq;   // (xq is a multiple of DEPTH, or all)
-            const uint4 *xp = has_x ? xf + ((size_t)ws * P.xq * NT * x_lanes + lane) * 2 : zeros;
-            const float4 *rp = xrow + ws * P.xq * (NT * 4) + (NT == 1 ? min(j, rt - 1) : j);   // the row whose sums this lane gets
-            for (int k_ = c0; k_ < end; k_ += DEPTH)
+            const unsigned char *base = smem + stage * stage_bytes;
+            const int end = min(k1, k + P.stage_k), g_first = sz_group(k);
+            for (int kt = k + warp; kt < end; kt += KW) {
+                const unsigned char *at = base + (kt - k) * 512;
+                const uint32_t *sz = (const uint32_t *)(base + P.stage_k * 512) + (sz_group(kt) - g_first) * 16 + g;
+                uint4 b[NT][2];
+                float4 xr[NT];
 #pragma unroll
-                for (int d = 0; d < DEPTH; ++d) {
-                    if (any && k_ + d < len) {
-                        uint4 b[NT][2];
-                        float4 xr[NT];
+                for (int n = 0; n < NT; ++n) {
+                    b[n][0] = xp[n * x_n], b[n][1] = xp[n * x_n + 1];
+                    xr[n] = rp[n * 4];
+                }
+                xp += x_step, rp += KW * NT * 4;
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    const uint4 w = *(const uint4 *)(at + t * tile_bytes + lane * 16);
+                    float acc[NT][4];
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        uint32_t a0[4], a1[4];
+                        pairs8(hf ? w.y : w.x, a0);
+                        pairs8(hf ? w.w : w.z, a1);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            b[n][0] = xp[0], b[n][1] = xp[1];
-                            xp += x_step;
-                            xr[n] = rp[n * 4];
+                            if (G32 || hf == 0) mma_f16_first(acc[n], a0[0], a1[0], a0[1], a1[1], b[n][hf].x, b[n][hf].y);
+                            else mma_f16(acc[n], a0[0], a1[0], a0[1], a1[1], b[n][hf].x, b[n][hf].y);
+                            mma_f16(acc[n], a0[2], a1[2], a0[3], a1[3], b[n][hf].z, b[n][hf].w);
                         }
-                        rp += NT * 4;
+                        if (G32 || hf == 1) {
+                            // (a second group of 32 that is not there belongs to inputs that are not there either: s = z = 0)
+                            const bool there = !G32 || hf == 0 || 2 * kt + 1 < P.groups;
+                            const uint32_t *z = sz + t * (tile_bytes / 4) + (G32 ? hf * 16 : 0);
+                            const float2 s0 = __half22float2(u_h2(there ? z[0] : 0)), s1 = __half22float2(u_h2(there ? z[8] : 0));
 #pragma unroll
-                        for (int t = 0; t < T; ++t) {
-                            const uint4 w = codes[d][t];
-                            float acc[NT][4];
-#pragma unroll
-                            for (int hf = 0; hf < 2; ++hf) {
-                                uint32_t a0[4], a1[4];
-                                pairs8(hf ? w.y : w.x, a0);
-                                pairs8(hf ? w.w : w.z, a1);
-#pragma unroll
-                                for (int n = 0; n < NT; ++n) {
-                                    if (G32 || hf == 0) mma_f16_first(acc[n], a0[0], a1[0], a0[1], a1[1], b[n][hf].x, b[n][hf].y);
-                                    else mma_f16(acc[n], a0[0], a1[0], a0[1], a1[1], b[n][hf].x, b[n][hf].y);
-                                    mma_f16(acc[n], a0[2], a1[2], a0[3], a1[3], b[n][hf].z, b[n][hf].w);
-                                }
-                                if (G32 || hf == 1) {
-                                    const float2 s0 = __half22float2(u_h2(sz[d][t][G32 ? 2 * hf : 0])), s1 = __half22float2(u_h2(sz[d][t][G32 ? 2 * hf + 1 : 1]));
-                                    const float m0 = s0.x * 0x1p24f, m1 = s1.x * 0x1p24f;
-#pragma unroll
-                                    for (int n = 0; n < NT; ++n) {
-                                        const float xs = G32 && hf ? xr[n].z : xr[n].y;
-                                        total[t][n][0] = fmaf(m0, fmaf(-s0.y, xs, acc[n][0] + acc[n][1]) * xr[n].x, total[t][n][0]);
-                                        total[t][n][1] = fmaf(m1, fmaf(-s1.y, xs, acc[n][2] + acc[n][3]) * xr[n].x, total[t][n][1]);
-                                    }
-                                }
+                            for (int n = 0; n < NT; ++n) {
+                                const float xs = G32 && hf ? xr[n].z : xr[n].y;
+                                total[t][n][0] = fmaf(s0.x, fmaf(-s0.y, xs, acc[n][0] + acc[n][1]) * xr[n].x, total[t][n][0]);
+                                total[t][n][1] = fmaf(s1.x, fmaf(-s1.y, xs, acc[n][2] + acc[n][3]) * xr[n].x, total[t][n][1]);
                             }
                         }
                     }
-                    request(d);
                 }
+            }
+            __syncwarp();
+            if (lane == 0) mx::mbar_arrive(mx::smem_u32(&empty[stage]));
+            if (++stage == P.stages) stage = 0, parity ^= 1;
         }
         // ---- slices of the CTA, then of the cluster, pairwise; each CTA of it finishes a share ----
         float *mine = sums + buf * W4_WARPS * S::SUMS;
@@ -361,48 +341,70 @@ __global__ void __launch_bounds__(W4_THREADS, 2) gemv_int4_kernel(const Int4Para
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) mine[warp * S::SUMS + ((t * NT + n) * 2 + e) * 32 + lane] = total[t][n][e];
-        __syncthreads();
-        float *theirs = parts + buf * entries;
+                for (int e = 0; e < 2; ++e) mine[warp * S::SUMS + ((t * NT + n) * 2 + e) * 32 + lane] = late ? NAN : total[t][n][e];
+        sync();
+        float *theirs = parts + buf * S::SUMS;
         if (C > 1) {
-            for (int i = tid; i < entries; i += W4_THREADS) {
-                const int gi = i / S::SUMS, e = i - gi * S::SUMS, to = i / share;
-                const float v = tree_sum(mine + gi * kw * S::SUMS + e, kw, S::SUMS);
+            for (int i = tid; i < S::SUMS; i += W4_THREADS) {
+                const float v = tree_sum(mine + i, KW, S::SUMS);
+                const int to = i / share;
                 const uint32_t dst = mx::cluster_map(mx::smem_u32(theirs + rank * share + i - to * share), to);
                 asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(v) : "memory");
             }
             mx::cluster_sync();
         }
         for (int i = rank * share + tid; i < (rank + 1) * share; i += W4_THREADS) {
-            const int gi = i / S::SUMS, e = i - gi * S::SUMS, l = e & 31, hf = (e >> 5) & 1, n = (e >> 6) % NT, t = (e >> 6) / NT;
-            const float v = C > 1 ? tree_sum(theirs + i - rank * share, C, share) : tree_sum(mine + gi * kw * S::SUMS + e, kw, S::SUMS);
-            const int o = ((grp * tg + gi) * T + t) * W4_N + (l >> 2) + 8 * hf, r = n * 4 + (l & 3);
+            const int l = i & 31, hf = (i >> 5) & 1, n = (i >> 6) % NT, t = (i >> 6) / NT;
+            float v = C > 1 ? tree_sum(theirs + i - rank * share, C, share) : tree_sum(mine + i, KW, S::SUMS);
+            const int o = (grp * T + t) * W4_N + (l >> 2) + 8 * hf, r = n * 4 + (l & 3);
             if (o < P.n_out && r < rows) {
+                v *= 0x1p24f;   // (sums of q 2^-24)
                 float out = P.bias ? v + P.bias[o] : v;
                 if (P.add) out = P.add[(long long)(row0 + r) * P.add_stride + o] + out;
                 P.y[(long long)(row0 + r) * P.y_stride + o] = out;
             }
         }
         // (the sums of the group before last are read by nobody any more: its barrier is behind all of them)
-        buf ^= P.buffers - 1;
+        buf ^= 1;
     }
 }
 
 template <int NT, int T, bool G32>
 int launch_int4(mx230_handle *h, cudaStream_t st, Int4Params P, int x_tile) {
     using S = Int4Form<NT, T, G32>;
-    const int tg = W4_WARPS / P.kw, C = P.ctas_k, n_slices = P.kw * C;
-    const int most = (P.k_tiles + n_slices - 1) / n_slices, per_tile = P.kw * x_tile;
-    P.xq = W4_X_BYTES / per_tile;
-    P.xq = P.xq >= most ? most : P.xq < S::DEPTH ? S::DEPTH : P.xq / S::DEPTH * S::DEPTH;
-    P.n_groups = (int)((P.n_tiles + (long long)tg * T - 1) / ((long long)tg * T));
-    P.n_clusters = 2 * h->sm_count / C;
-    if (P.n_clusters > P.n_groups) P.n_clusters = P.n_groups;
-    P.buffers = P.n_groups > P.n_clusters ? 2 : 1;
-    const size_t sm = (size_t)P.buffers * (W4_WARPS + (C > 1 ? tg : 0)) * S::SUMS * 4 + 32 + (size_t)P.xq * per_tile;
-    MX_SMEM_ATTR_ONCE(h->device, (gemv_int4_kernel<NT, T, G32>), 227 * 1024);
+    const int C = P.ctas_k;
+    P.n_groups = (P.n_tiles + T - 1) / T;
+    // Shared memory: rows and sums, and what is left for stages, of four tiles a warp where three of them fit, or two, or one (a whole
+    // number of turns; 4096 x 128000, one row: 64 us with two, 57 with four).
+    const size_t fixed = (size_t)2 * (W4_WARPS + (C > 1 ? 1 : 0)) * S::SUMS * 4 + 32 + (size_t)P.k_cta * x_tile;
+    P.stage_k = 4 * W4_WARPS;
+    while (P.stage_k > W4_WARPS && fixed + (size_t)(P.stage_k == 2 * W4_WARPS ? 2 : 3) * T * P.stage_k * S::TILE > W4_SMEM) P.stage_k /= 2;
+    if (P.stage_k > P.k_cta) P.stage_k = P.k_cta;
+    const size_t stage = (size_t)T * P.stage_k * S::TILE;
+    MX_REQUIRE(fixed + 2 * stage <= W4_SMEM, MX230_ERR_UNSUPPORTED, "gemv_int4: %d inputs a CTA and two stages do not fit shared memory", P.k_cta * W4_K);
+    P.stages = (int)((W4_SMEM - fixed) / stage);
+    if (P.stages > W4_STAGES) P.stages = W4_STAGES;
+    const size_t sm = fixed + P.stages * stage;
+    MX_SMEM_ATTR_ONCE(h->device, (gemv_int4_kernel<NT, T, G32>), W4_SMEM);
+    // clusters that the device holds at once, of CTAs that fill an SM (asked once per size)
+    static int fit[64][4];
+    const int size = C == 1 ? 0 : C == 2 ? 1 : C == 4 ? 2 : 3;
+    int held = h->sm_count;
+    if (C > 1) {
+        if (h->device >= 64 || fit[h->device][size] == 0) {
+            cudaLaunchConfig_t cfg = {};
+            cudaLaunchAttribute at;
+            cfg.gridDim = dim3(C), cfg.blockDim = dim3(W4_THREADS + W4_PRODUCER), cfg.dynamicSmemBytes = W4_SMEM, cfg.attrs = &at, cfg.numAttrs = 1;
+            at.id = cudaLaunchAttributeClusterDimension;
+            at.val.clusterDim.x = C, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+            MX_CHECK_CUDA(cudaOccupancyMaxActiveClusters(&held, gemv_int4_kernel<NT, T, G32>, &cfg));
+            if (held < 1) held = 1;
+            if (h->device < 64) fit[h->device][size] = held;
+        } else held = fit[h->device][size];
+    }
+    P.n_clusters = held < P.n_groups ? held : P.n_groups;
     const dim3 grid((unsigned)(P.n_clusters * C), (unsigned)((P.n_rows + 4 * NT - 1) / (4 * NT)));
-    MX_LAUNCH(h, st, MX230_K_GEMV_INT4, mx_launch(gemv_int4_kernel<NT, T, G32>, grid, W4_THREADS, sm, st, C, true, P));
+    MX_LAUNCH(h, st, MX230_K_GEMV_INT4, mx_launch(gemv_int4_kernel<NT, T, G32>, grid, W4_THREADS + W4_PRODUCER, sm, st, C, true, P));
     return MX230_OK;
 }
 
@@ -456,6 +458,7 @@ extern "C" int mx230_gemv_int4(mx230_handle *h, void *stream, float *y, const fl
                "gemv_int4: misaligned pointer");
     MX_REQUIRE(add != y || n_rows < 2 || add_stride == y_stride, MX230_ERR_INVALID_ARG, "gemv_int4: add is y, with another stride");
     MX_REQUIRE(n_rows <= 65535 * 4, MX230_ERR_UNSUPPORTED, "gemv_int4: %d rows", n_rows);
+    MX_REQUIRE(n_in <= 2 * W4_K_CTA * W4_CLUSTER * W4_K, MX230_ERR_UNSUPPORTED, "gemv_int4: n_in %d (at most %d)", n_in, 2 * W4_K_CTA * W4_CLUSTER * W4_K);
     Int4Params P{};
     P.y = y, P.x = x, P.bias = bias, P.add = add;
     P.codes = (const uint4 *)packed, P.sz = (const uint32_t *)((const char *)packed + codes_bytes(n_in, n_out));
@@ -464,20 +467,20 @@ extern "C" int mx230_gemv_int4(mx230_handle *h, void *stream, float *y, const fl
     P.n_tiles = (int)((n_out + (long long)W4_N - 1) / W4_N), P.k_tiles = (int)((n_in + (long long)W4_K - 1) / W4_K);
     P.x_stride = x_stride, P.y_stride = y_stride, P.add_stride = add_stride;
     P.x_vec = ((uintptr_t)x & 15) == 0 && (n_rows < 2 || x_stride % 4 == 0);
-    // Slices of the inputs: a CTA's eight warps, and more where there are few output tiles, each with two tiles at least.  This fixes the
-    // order of the sums.
-    int n_slices = 1;
-    while (n_slices < W4_WARPS && 2 * n_slices <= P.k_tiles) n_slices *= 2;
-    while (n_slices < W4_WARPS * W4_CLUSTER && 4 * n_slices <= P.k_tiles && (long long)P.n_tiles * n_slices < 16ll * h->sm_count) n_slices *= 2;
-    // CTAs of a cluster: so many that a CTA's part of the rows stays in shared memory.
-    const int nt = n_rows <= 4 ? 1 : 2, x_tile = nt * (32 * (nt == 1 ? 8 * n_rows : 32) + 64);
-    P.ctas_k = n_slices <= W4_WARPS ? 1 : n_slices / W4_WARPS;
-    while (2 * P.ctas_k <= n_slices && P.ctas_k < W4_CLUSTER && (long long)(P.k_tiles + P.ctas_k - 1) / P.ctas_k * x_tile > W4_X_BYTES) P.ctas_k *= 2;
-    P.kw = n_slices / P.ctas_k;
-    // Output tiles of a warp: as many as still leave work for nearly all CTAs that the SMs hold.
-    const int tg = W4_WARPS / P.kw, places = 2 * h->sm_count / P.ctas_k;
-    int t = nt == 1 ? 4 : 2;
-    while (t > 1 && P.n_tiles / (tg * t) < places * 3 / 4) t /= 2;
+    P.status = h->status_dev;
+    const unsigned long long per_group = group == 32 ? 1 : group / W4_K;
+    P.group_magic = per_group == 1 ? 0 : (uint32_t)(((1ull << 32) + per_group - 1) / per_group);
+    // Inputs over CTAs so that a CTA's rows fit its shared memory, and where there are few output tiles.  This fixes the order of the sums.
+    P.ctas_k = 1;
+    while (P.ctas_k < W4_CLUSTER && (P.k_tiles > W4_K_CTA * P.ctas_k || (P.k_tiles >= 64 * P.ctas_k && (long long)P.n_tiles * P.ctas_k < h->sm_count))) P.ctas_k *= 2;
+    P.k_cta = (P.k_tiles + P.ctas_k - 1) / P.ctas_k;
+    // Rows of a pass: eight, or four where eight do not fit.
+    const int nt = n_rows <= 4 || P.k_cta > W4_K_CTA ? 1 : 2, x_tile = nt * (32 * (nt == 1 ? 8 * (n_rows < 4 ? n_rows : 4) : 32) + 64);
+    // Output tiles of a warp, which share what is read of the rows: two where half the SMs then have a group of them, four (of few rows)
+    // where they have three groups for two SMs (one row, us with one / two / four: 896 x 1152 2.4, 2.7, 3.3; 4096 x 4096 5.5, 4.9, 6.1;
+    // 4096 x 14336 12.6, 11.3, 10.8; 4096 x 128000 80, 58, 56).
+    const long long here = (long long)P.n_tiles * P.ctas_k;
+    const int t = nt == 1 && here * 2 >= 4 * 3ll * h->sm_count * 95 / 100 ? 4 : here >= h->sm_count ? 2 : 1;
     mx230_device_guard guard(h->device);
     cudaStream_t st = (cudaStream_t)stream;
     const bool g32 = group == 32;
