@@ -525,10 +525,11 @@ int mx230_gemv_int8(mx230_handle *h, void *stream, float *y, const float *x, con
 /* The same for up to a few rows over 4-bit weights with group scales (decode tokens of several sequences):
  *     y[r][o] = sum_i x[r][i] scale[i / group][o] (code[i][o] - zero[i / group][o]) + bias[o] + add[r][o]
  * x, y, bias, add fp32, rows x_stride, y_stride, add_stride elements apart; bias and add may be null, add may be y (with its
- * stride).  Any n_in, n_out and number of rows; built for 1 to 16 rows, more go in turns over the weights.  A row's bits do not depend on the
- * rows computed with it.  `packed` (mx230_int4_bytes, 16-byte aligned) is made once by mx230_pack_int4 from codes [n_in][n_out] (the
+ * stride).  n_in up to 65536, any n_out and number of rows (eight at a time go over the weights, so it is built for a few).  A row's
+ * bits do not depend on the rows computed with it.  `packed` (mx230_int4_bytes, 16-byte aligned) is made once by mx230_pack_int4 from codes [n_in][n_out] (the
  * low four bits of a byte), fp16 scales and zeros [ceil(n_in / group)][n_out] (zeros null: 8); group 32 or a multiple of 64.
- * Weights and both parts of x (22 bits of it, relative to the largest of 64) are exact on the tensor cores; sums are fp32.
+ * x goes in as two fp16 parts relative to the largest of 64 (off by half an ulp of fp32, or 2^-39 of that largest one), codes as they
+ * are; sums are fp32, of x code and of x apart (zeros are meant to be 0 to 15; larger ones are taken, at the cost of digits).
  * No workspace. */
 size_t mx230_int4_bytes(int n_in, int n_out, int group);
 int mx230_pack_int4(mx230_handle *h, void *stream, void *packed, const uint8_t *codes, const void *scales_fp16,

@@ -4,13 +4,15 @@
 // Bounded by HBM on the weights: half a byte each, read once, and 4 bytes of scale and zero point per group.  At that rate an SM
 // takes 46 weights a cycle, so a weight may cost about two instructions of a lane; multiply-adds on CUDA cores, with the
 // conversion from 4 bits in front, would take more for a single row and that many times more for several.  Hence warp-level
-// tensor-core tiles (m16n8k16) with the weights as A: 16 outputs x 16 inputs.  Four bits in the lowest places of an fp16 are the
-// number q 2^-24 (a subnormal, which the tensor cores take as it is), in the next four places 16 q 2^-24, so a pair of weights costs
-// one "and", and half the inputs carry a factor of 1/16 against it.  The rows are the eight columns of B, two columns a row:
+// tensor-core tiles (m16n8k16) with the weights as A: 16 outputs x 16 inputs.  Four bits at places 4 to 7 of an fp16 are the number
+// q 2^-20 (a subnormal, which the tensor cores take as it is), so a pair of weights costs an "and" and three quarters of a shift.  (At
+// places 0 to 3 they are q 2^-24, one shift less a pair, but the products of a step are added with the digits that the largest possible
+// number of a subnormal's exponent leaves, ten bits above q: 1.3e-6 of the result over 4096 inputs, 0.3e-6 so.)  The rows are the eight
+// columns of B, two columns a row:
 //   x 2^e = hi + lo, both fp16, e such that the largest of the 64 values of a tile lies in [2^14, 2^15):
-// |x 2^e - hi - lo| <= 2^-24 |x 2^e|, as exact as x itself (but for values 2^-13 times the tile's largest and less, which keep an
-// absolute error of 2^-35 of that).  Products are then exact in fp32; sums are fp32, per tile of 64 inputs (32, if groups are of
-// 32).  The zero point meets the sum of the tile's x: the row's total gets s 2^(24 - e) (sum x q - z sum x), whose error goes by
+// |x 2^e - hi - lo| <= 2^-24 |x 2^e|, as exact as x itself (but for values 2^-17 times the tile's largest and less, which keep an
+// absolute error of 2^-39 of that).  Products are then exact in fp32; sums are fp32, per tile of 64 inputs (32, if groups are of
+// 32).  The zero point meets the sum of the tile's x: the row's total gets s 2^(20 - e) (sum x q - z sum x), whose error goes by
 // sum |x| (q + z) instead of sum |x (q - z)|, about four times that, and saves the subtraction per weight (161 instructions a
 // warp and tile with it, of which 36 for the conversion; the kernel was bound by them: 37 us for 4096 x 14336, one row).
 //
@@ -96,10 +98,10 @@ __global__ void pack_int4_kernel(uint4 *codes_out, uint32_t *sz_out, const uint8
 __device__ __forceinline__ uint32_t h2_u(__half2 v) { return *(uint32_t *)&v; }
 __device__ __forceinline__ __half2 u_h2(uint32_t v) { return *(__half2 *)&v; }
 
-// eight codes -> four pairs (inputs 2p, 2p + 1) of q 2^-24 (p even) or 16 q 2^-24 (p odd)
+// eight codes -> four pairs (inputs 2p, 2p + 1) of q 2^-20
 __device__ __forceinline__ void pairs8(uint32_t w, uint32_t (&a)[4]) {
-    const uint32_t v = w >> 8;
-    a[0] = w & 0x000F000Fu, a[1] = w & 0x00F000F0u, a[2] = v & 0x000F000Fu, a[3] = v & 0x00F000F0u;
+    constexpr uint32_t PLACE = 0x00F000F0u;
+    a[0] = (w << 4) & PLACE, a[1] = w & PLACE, a[2] = (w >> 4) & PLACE, a[3] = (w >> 8) & PLACE;
 }
 
 // c = a b + c, or a b
@@ -129,7 +131,7 @@ __device__ __forceinline__ float tree_sum(const float *p, int n, int step) {
 
 // NT: column tiles of four rows.  T: output tiles of a warp.  G32: groups of 32 inputs (else a multiple of 64).
 // Shared memory: ring [stages][T][stage_k x 512 of codes, stage_k x 64 (groups of 32: 128) of (s, z)]; sums [2][16 warps][T * NT * 64];
-// in clusters, this CTA's share of everybody's sums [2][C][T * NT * 64 / C]; per (tile, row) {2^-e, 2^(e - 24) sum x, or that
+// in clusters, this CTA's share of everybody's sums [2][C][T * NT * 64 / C]; per (tile, row) {2^-e, 2^(e - 20) sum x, or that
 // of either half}; 32 bytes of zeros; rows [k_cta][NT][lanes][8 words].
 template <int NT, int T, bool G32>
 struct Int4Form {
@@ -251,11 +253,11 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
                 if (G32) sum[1] += __shfl_xor_sync(0xFFFFFFFFu, sum[1], o);
             }
             if (i0 + lane >= n_x) continue;
-            if (jj == 0) xrow[q * (NT * 4) + r] = make_float4(down, sum[0] * 0x1p-24f, sum[1] * 0x1p-24f, 0.0f);
+            if (jj == 0) xrow[q * (NT * 4) + r] = make_float4(down, sum[0] * 0x1p-20f, sum[1] * 0x1p-20f, 0.0f);
             uint32_t hi[8], lo[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float f = (e & 1) ? 0.0625f : 1.0f, a = v[2 * e] * f, b = v[2 * e + 1] * f;
+                const float a = v[2 * e], b = v[2 * e + 1];
                 const __half2 h = __floats2half2_rn(a, b);
                 const float2 back = __half22float2(h);
                 hi[e] = h2_u(h), lo[e] = h2_u(__floats2half2_rn(a - back.x, b - back.y));
@@ -358,7 +360,7 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
             float v = C > 1 ? tree_sum(theirs + i - rank * share, C, share) : tree_sum(mine + i, KW, S::SUMS);
             const int o = (grp * T + t) * W4_N + (l >> 2) + 8 * hf, r = n * 4 + (l & 3);
             if (o < P.n_out && r < rows) {
-                v *= 0x1p24f;   // (sums of q 2^-24)
+                v *= 0x1p20f;   // (sums of q 2^-20)
                 float out = P.bias ? v + P.bias[o] : v;
                 if (P.add) out = P.add[(long long)(row0 + r) * P.add_stride + o] + out;
                 P.y[(long long)(row0 + r) * P.y_stride + o] = out;

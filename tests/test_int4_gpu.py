@@ -1,10 +1,10 @@
 """Products with 4-bit weights against the same sums in 64 bits.
 
 Tolerance, against M = sum |x| s (q + z), as the sums of x q and of x are taken apart.  Codes and both parts of x are exact in fp16; x is off by
-2^-24 |x|, or by 2^-35 of the largest of its 64.  The tensor core adds the 16 products of a step with at most 17 truncations of 2^-24 M:
-2^-20 M with the steps of a tile.  A tile's sum of x: 19 rounded additions, 2^-20 M.  The difference, its scale and the
-addition round: 2^-22 M a tile, for at most the tiles of a slice, and six pairwise sums.  Then the bias and what is added, half a
-step each.
+2^-24 |x|, or by 2^-39 of the largest of its 64.  The 16 products of a step are added by the tensor core, taken as 17 truncations of 2^-24 M
+(what it keeps is not documented): 2^-20 M a step, and no step has more than its share of M.  A tile's sum of x: 19 rounded
+additions, 2^-20 M.  The difference, its scale and the addition round: 2^-22 M a tile, for at most the tiles of a slice, and
+seven pairwise sums.  Then the bias and what is added, half a step each.
 """
 import math
 
@@ -81,6 +81,19 @@ def test_a_row_does_not_depend_on_the_others(handle, n_in, n_out, group):
         y = torch.empty(n, n_out, device="cuda")
         la.gemv_int4(handle, y, x[:n], w)
         assert torch.equal(y, alone[:n]), n
+
+
+@pytest.mark.parametrize("n_in,n_out,rows,group", [(65536, 40, 5, 128), (32769, 100, 2, 32), (40000, 33, 9, 192), (4096, 2400, 3, 1 << 20), (700, 300, 4, 704)])
+def test_long_rows_and_wide_groups(handle, n_in, n_out, rows, group):
+    """Up to eight CTAs along the inputs, more rows than fit beside them, groups that end inside a stage or never."""
+    codes, scales, z = weights(n_in, n_out, group, True, n_in)
+    w = la.pack_int4(handle, codes, scales, z, group=group)
+    x = torch.randn(rows, n_in, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    y, d = torch.empty(rows, n_out, device="cuda"), Dense(codes, scales, z, group)
+    la.gemv_int4(handle, y, x, w)
+    want = x.double() @ d.w
+    check(y, want, d.limit(x, want), (n_in, group))
+    handle.check_status()
 
 
 @pytest.mark.parametrize("scale", [1e-30, 1e-12, 1.0, 1e20])
@@ -203,6 +216,10 @@ def test_refusals(handle):
         with pytest.raises(_lib.Mx230Error) as e:
             call()
         assert e.value.code == _lib.ERR_INVALID_ARG
+    long = la.pack_int4(handle, torch.zeros(65537, 4, dtype=torch.uint8, device="cuda"), torch.zeros(513, 4, dtype=torch.float16, device="cuda"), group=128)
+    with pytest.raises(_lib.Mx230Error) as e:
+        la.gemv_int4(handle, torch.zeros(1, 4, device="cuda"), torch.zeros(1, 65537, device="cuda"), long)
+    assert e.value.code == _lib.ERR_UNSUPPORTED
     with pytest.raises(_lib.Mx230Error) as e:
         la.pack_int4(handle, codes, torch.zeros(6, 48, dtype=torch.float16, device="cuda"), group=48)
     assert e.value.code == _lib.ERR_UNSUPPORTED

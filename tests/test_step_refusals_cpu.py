@@ -60,6 +60,7 @@ def test_int4_refuses(L):
     for g in (0, -64, 16, 48, 96, 31):
         assert L.mx230_gemv_int4(*{**ok, "group": g}.values()) == _lib.ERR_UNSUPPORTED, g
     assert L.mx230_gemv_int4(*{**ok, "rows": 1 << 30}.values()) == _lib.ERR_UNSUPPORTED
+    assert L.mx230_gemv_int4(*{**ok, "n_in": 65537, "xs": 65537}.values()) == _lib.ERR_UNSUPPORTED
     assert L.mx230_gemv_int4(*{**ok, "rows": 0}.values()) == 0
     pk = dict(h=H, st=None, packed=P, codes=P, scales=P, zeros=None, n_in=256, n_out=64, group=64)
     for c in [dict(h=None), dict(packed=None), dict(codes=None), dict(scales=None), dict(packed=P + 4), dict(scales=P + 1), dict(n_in=0), dict(n_out=-1)]:
