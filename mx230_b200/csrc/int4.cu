@@ -132,7 +132,7 @@ __device__ __forceinline__ float tree_sum(const float *p, int n, int step) {
 // NT: column tiles of four rows.  T: output tiles of a warp.  G32: groups of 32 inputs (else a multiple of 64).
 // Shared memory: ring [stages][T][stage_k x 512 of codes, stage_k x 64 (groups of 32: 128) of (s, z)]; sums [2][16 warps][T * NT * 64];
 // in clusters, this CTA's share of everybody's sums [2][C][T * NT * 64 / C]; per (tile, row) {2^-e, 2^(e - 20) sum x, or that
-// of either half}; 32 bytes of zeros; rows [k_cta][NT][lanes][8 words].
+// of either half, 2^-e of the second half}; 32 bytes of zeros; rows [k_cta][NT][lanes][8 words].
 template <int NT, int T, bool G32>
 struct Int4Form {
     static constexpr int SUMS = T * NT * 64;                // floats of a warp
@@ -237,11 +237,19 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
             for (int o = 1; o < 4; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
             // e = 14 - exponent of amax; 2^e and 2^-e by their bits
             const int eb = max((int)(__float_as_uint(amax) >> 23), 15);
-            float up = __uint_as_float((uint32_t)(268 - eb) << 23), down = __uint_as_float((uint32_t)(eb - 14) << 23);
-            if (amax == INFINITY) {   // infinite values alone count: as 1, and the tile's sum times infinity
-                up = 1.0f, down = INFINITY;
+            float up = __uint_as_float((uint32_t)(268 - eb) << 23), down = __uint_as_float((uint32_t)(eb - 14) << 23), down2 = down;
+            if (amax == INFINITY) {   // infinite values alone count: as 1, and the sum of those with their scale times infinity
+                unsigned there = 0;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) v[e] = isinf(v[e]) ? copysignf(1.0f, v[e]) : v[e] == v[e] ? 0.0f : v[e];
+                for (int e = 0; e < 16; ++e) {
+                    if (isinf(v[e])) there |= G32 ? 1u << (e >> 3) : 1u;
+                    v[e] = isinf(v[e]) ? copysignf(1.0f, v[e]) : v[e] == v[e] ? 0.0f : v[e];
+                }
+                if (G32) {   // (of the row's four lanes, which are all here)
+                    there |= __shfl_xor_sync(0xFu << (lane & 28), there, 1);
+                    there |= __shfl_xor_sync(0xFu << (lane & 28), there, 2);
+                }
+                up = 1.0f, down = !G32 || (there & 1) ? INFINITY : 1.0f, down2 = there & 2 ? INFINITY : 1.0f;
             }
             float sum[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -253,7 +261,7 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
                 if (G32) sum[1] += __shfl_xor_sync(0xFFFFFFFFu, sum[1], o);
             }
             if (i0 + lane >= n_x) continue;
-            if (jj == 0) xrow[q * (NT * 4) + r] = make_float4(down, sum[0] * 0x1p-20f, sum[1] * 0x1p-20f, 0.0f);
+            if (jj == 0) xrow[q * (NT * 4) + r] = make_float4(down, sum[0] * 0x1p-20f, sum[1] * 0x1p-20f, down2);
             uint32_t hi[8], lo[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -324,9 +332,9 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
                             const float2 s0 = __half22float2(u_h2(there ? z[0] : 0)), s1 = __half22float2(u_h2(there ? z[8] : 0));
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
-                                const float xs = G32 && hf ? xr[n].z : xr[n].y;
-                                total[t][n][0] = fmaf(s0.x, fmaf(-s0.y, xs, acc[n][0] + acc[n][1]) * xr[n].x, total[t][n][0]);
-                                total[t][n][1] = fmaf(s1.x, fmaf(-s1.y, xs, acc[n][2] + acc[n][3]) * xr[n].x, total[t][n][1]);
+                                const float xs = G32 && hf ? xr[n].z : xr[n].y, back = G32 && hf ? xr[n].w : xr[n].x;
+                                total[t][n][0] = fmaf(s0.x, fmaf(-s0.y, xs, acc[n][0] + acc[n][1]) * back, total[t][n][0]);
+                                total[t][n][1] = fmaf(s1.x, fmaf(-s1.y, xs, acc[n][2] + acc[n][3]) * back, total[t][n][1]);
                             }
                         }
                     }

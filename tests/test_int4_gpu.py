@@ -134,6 +134,28 @@ def test_infinities_and_nan_stay_in_their_row(handle):
         assert torch.equal(torch.isnan(want), torch.isnan(y[r])) and torch.equal(want[~torch.isnan(want)], y[r].double()[~torch.isnan(want)])
 
 
+@pytest.mark.parametrize("n_in,group", [(256, 32), (250, 32), (97, 32), (160, 32), (64, 32), (256, 128), (130, 64)])
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+def test_one_infinity_gives_its_weight_the_sign(handle, n_in, group, value):
+    """In either half of a tile, in the last one too, whose other half may be nothing: inf s (q - z), NaN where that is 0."""
+    codes, scales, z = weights(n_in, 48, group, True, 4)
+    w = la.pack_int4(handle, codes, scales, z, group=group)
+    d = Dense(codes, scales, z, group)
+    for rows in (1, 6):
+        x = torch.randn(rows, n_in, device="cuda", generator=torch.Generator(device="cuda").manual_seed(8))
+        for k in (0, 33, n_in // 2, n_in - 1):
+            if k >= n_in:
+                continue
+            at = x.clone()
+            at[rows - 1, k] = value
+            y = torch.empty(rows, 48, device="cuda")
+            la.gemv_int4(handle, y, at, w)
+            want = value * d.w[k]
+            nan = torch.isnan(want)
+            assert torch.equal(nan, torch.isnan(y[-1])) and torch.equal(want[~nan], y[-1].double()[~nan]), (rows, k)
+            assert torch.isfinite(y[:-1]).all()
+
+
 def test_strides_and_what_lies_beside(handle):
     n_in, n_out, rows = 200, 50, 6
     codes, scales, z = weights(n_in, n_out, 64, True, 3)
