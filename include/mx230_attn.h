@@ -78,7 +78,9 @@ enum {
                                     merges by thread-block clusters CTA `value` of the first decode group (the first 64
                                     columns of a projection) waits for sums that nobody sends, so that the bounded wait
                                     of their consumer runs out and the abort path executes: the heads that lack sums
-                                    become NaN, the columns of a projection are not written */
+                                    become NaN, the columns of a projection are not written.  In products with
+                                    4-bit weights CTA 0 requests none of its stages from the value-th on, and the
+                                    outputs that lack them become NaN */
 };
 
 /* kernel ids of the profiling interface */

@@ -59,6 +59,7 @@ struct Int4Params {
     uint32_t group_magic;    // 2^32 over the tiles of a group of inputs, rounded up; 0: one
     int x_vec;               // rows are 16-byte aligned
     int *status;             // where a wait that ran out is recorded
+    int test_drop_tile;      // test hook: stage from which on CTA 0's producer requests nothing; -1 = off
     long long x_stride, y_stride, add_stride;
 };
 
@@ -145,6 +146,7 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(8) unsigned long long full[W4_STAGES], empty[W4_STAGES];
     __shared__ int aborted;
+    __shared__ volatile int stop_grp, stop_k;               // first stage that the producer, having given up, does not request
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
     constexpr int KW = W4_WARPS;                            // warps along the inputs, by turns
     const int C = P.ctas_k;
@@ -168,7 +170,7 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
     if (C > 1) mx::cluster_arrive_relaxed();   // waited for before the first store to another CTA's memory
     if (tid < 2) zeros[tid] = make_uint4(0, 0, 0, 0);
     if (tid == 0) {
-        aborted = 0;
+        aborted = 0, stop_grp = 0x7FFFFFFF;
         for (int i = 0; i < P.stages; ++i) mx::mbar_init(mx::smem_u32(&full[i]), 1), mx::mbar_init(mx::smem_u32(&empty[i]), W4_WARPS);
         mx::mbar_fence_init();
     }
@@ -178,15 +180,20 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
     if (warp == W4_WARPS) {
         // ---- producer: the tiles of every group, stage by stage (lane 0).  In clusters the warp counts in the barrier at every group's
         // end: it arrives once the group's stages are requested, and waits for the barrier only before it arrives at the next one ----
-        int stage = 0, parity = 1;
+        int stage = 0, parity = 1, count = 0;
         bool on = true;
         for (int grp = grp0; grp < P.n_groups; grp += P.n_clusters) {
             if (lane == 0 && on)
                 for (int k = k0; k < k1; k += P.stage_k) {
-                    if (!mx::mbar_wait(mx::smem_u32(&empty[stage]), parity, &aborted, P.status)) {
+                    if ((count == P.test_drop_tile && blockIdx.x == 0 && blockIdx.y == 0) ||
+                        !mx::mbar_wait(mx::smem_u32(&empty[stage]), parity, &aborted, P.status)) {
                         on = false;   // (what was requested is waited for by those who read it)
+                        stop_k = k;
+                        __threadfence_block();
+                        stop_grp = grp;
                         break;
                     }
+                    ++count;
                     const int n = min(P.stage_k, k1 - k), here = min(T, P.n_tiles - grp * T);
                     const int g_first = sz_group(k), g_last = G32 ? min(2 * (k + n), P.groups) : sz_group(k + n - 1) + 1;
                     const uint32_t bar = mx::smem_u32(&full[stage]), sz_bytes = (uint32_t)(g_last - g_first) * 64;
@@ -237,19 +244,20 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
             for (int o = 1; o < 4; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
             // e = 14 - exponent of amax; 2^e and 2^-e by their bits
             const int eb = max((int)(__float_as_uint(amax) >> 23), 15);
-            float up = __uint_as_float((uint32_t)(268 - eb) << 23), down = __uint_as_float((uint32_t)(eb - 14) << 23), down2 = down;
+            float up = __uint_as_float((uint32_t)(268 - eb) << 23), down = __uint_as_float((uint32_t)(eb - 14) << 23), down2 = G32 ? down : 0.0f;
             if (amax == INFINITY) {   // infinite values alone count: as 1, and the sum of those with their scale times infinity
-                unsigned there = 0;
+                unsigned there = G32 ? 0 : 1;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    if (isinf(v[e])) there |= G32 ? 1u << (e >> 3) : 1u;
+                    if (G32 && isinf(v[e])) there |= 1u << (e >> 3);
                     v[e] = isinf(v[e]) ? copysignf(1.0f, v[e]) : v[e] == v[e] ? 0.0f : v[e];
                 }
                 if (G32) {   // (of the row's four lanes, which are all here)
                     there |= __shfl_xor_sync(0xFu << (lane & 28), there, 1);
                     there |= __shfl_xor_sync(0xFu << (lane & 28), there, 2);
                 }
-                up = 1.0f, down = !G32 || (there & 1) ? INFINITY : 1.0f, down2 = there & 2 ? INFINITY : 1.0f;
+                up = 1.0f, down = there & 1 ? INFINITY : 1.0f;
+                if (G32) down2 = there & 2 ? INFINITY : 1.0f;
             }
             float sum[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -293,8 +301,9 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
         for (int k = k0; k < k1; k += P.stage_k) {
             const uint32_t bar = mx::smem_u32(&full[stage]);
             if (!mx::mbar_wait(bar, parity, &aborted, P.status)) {
-                // (its copies still land here: it goes on once they have, and its sums do not count)
-                for (const long long since = clock64(); !mx::mbar_try_wait(bar, parity) && clock64() - since < mx::LANDING_CYCLES;) {}
+                // (its copies, if they are requested, still land here: it goes on once they have, and its sums do not count)
+                for (const long long since = clock64(); !mx::mbar_try_wait(bar, parity) && clock64() - since < mx::LANDING_CYCLES;)
+                    if (stop_grp < grp || (stop_grp == grp && stop_k <= k)) break;
                 late = true;
             }
             const unsigned char *base = smem + stage * stage_bytes;
@@ -477,7 +486,7 @@ extern "C" int mx230_gemv_int4(mx230_handle *h, void *stream, float *y, const fl
     P.n_tiles = (int)((n_out + (long long)W4_N - 1) / W4_N), P.k_tiles = (int)((n_in + (long long)W4_K - 1) / W4_K);
     P.x_stride = x_stride, P.y_stride = y_stride, P.add_stride = add_stride;
     P.x_vec = ((uintptr_t)x & 15) == 0 && (n_rows < 2 || x_stride % 4 == 0);
-    P.status = h->status_dev;
+    P.status = h->status_dev, P.test_drop_tile = h->test_drop_tile;
     const unsigned long long per_group = group == 32 ? 1 : group / W4_K;
     P.group_magic = per_group == 1 ? 0 : (uint32_t)(((1ull << 32) + per_group - 1) / per_group);
     // Inputs over CTAs so that a CTA's rows fit its shared memory, and where there are few output tiles.  This fixes the order of the sums.

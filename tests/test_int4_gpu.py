@@ -194,6 +194,32 @@ def test_high_bits_of_codes_and_large_zeros(handle):
     check(a, want, d.limit(x, want), "zeros of 255")
 
 
+@pytest.mark.parametrize("n_in,n_out,rows,stage", [(896, 20000, 2, 0), (896, 20000, 6, 2), (14336, 4096, 8, 3), (4096, 40000, 1, 1), (4096, 40000, 1, 2)])
+def test_weights_that_never_arrive(handle, n_in, n_out, rows, stage):
+    """The wait for them ends, the outputs without them are NaN and the others right; the next call is right again."""
+    codes, scales, z = weights(n_in, n_out, 64, True, 12)
+    w = la.pack_int4(handle, codes, scales, z)
+    x = torch.randn(rows, n_in, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    y, again = torch.empty(rows, n_out, device="cuda"), torch.zeros(rows, n_out, device="cuda")
+    la.gemv_int4(handle, y, x, w)
+    handle.check_status()
+    try:
+        handle.set_option(_lib.OPT_WAIT_LIMIT, 2000)   # 2e6 SM cycles, about 1 ms
+        handle.set_option(_lib.OPT_TEST_DROP_TILE, stage)
+        la.gemv_int4(handle, again, x, w)
+        with pytest.raises(_lib.Mx230Error) as e:
+            handle.check_status()
+        assert e.value.code == _lib.ERR_DEVICE_STATUS
+    finally:
+        handle.set_option(_lib.OPT_TEST_DROP_TILE, -1)
+        handle.set_option(_lib.OPT_WAIT_LIMIT, 4000000)
+    lost = torch.isnan(again)
+    assert lost.any() and not lost.all() and torch.equal(again[~lost], y[~lost])
+    la.gemv_int4(handle, again, x, w)
+    handle.check_status()
+    assert torch.equal(again, y)
+
+
 def test_captured_replayed_and_on_another_stream(handle):
     n_in, n_out = 4864, 896
     codes, scales, z = weights(n_in, n_out, 64, True, 7)
