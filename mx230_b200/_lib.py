@@ -97,6 +97,13 @@ def require(cond, msg) -> None:
         raise Mx230Error(ERR_INVALID_ARG, msg if isinstance(msg, str) else msg())
 
 
+def require_int32(what: str, *values) -> None:
+    """Whole numbers that go into the library as int, which ctypes would cut to 32 bits."""
+    for v in values:
+        if not -0x80000000 <= v <= 0x7FFFFFFF:
+            raise Mx230Error(ERR_INVALID_ARG, f"{what}: {v} is not a number of 32 bits")
+
+
 def ptr(t) -> C.c_void_p | None:
     """Device (or host) address of a torch tensor / numpy array / int / None."""
     if t is None:

@@ -475,6 +475,7 @@ extern "C" int mx230_gemv_int4(mx230_handle *h, void *stream, float *y, const fl
                "gemv_int4: rows of y share memory, or a stride is negative (x %lld, y %lld, add %lld)", x_stride, y_stride, add_stride);
     MX_REQUIRE(((uintptr_t)packed & 15) == 0 && (((uintptr_t)x | (uintptr_t)y | (uintptr_t)bias | (uintptr_t)add) & 3) == 0, MX230_ERR_INVALID_ARG,
                "gemv_int4: misaligned pointer");
+    MX_REQUIRE(x != y && bias != y, MX230_ERR_INVALID_ARG, "gemv_int4: y is x or the bias, which other blocks still read");
     MX_REQUIRE(add != y || n_rows < 2 || add_stride == y_stride, MX230_ERR_INVALID_ARG, "gemv_int4: add is y, with another stride");
     MX_REQUIRE(n_rows <= 65535 * 4, MX230_ERR_UNSUPPORTED, "gemv_int4: %d rows", n_rows);
     MX_REQUIRE(n_in <= 2 * W4_K_CTA * W4_CLUSTER * W4_K, MX230_ERR_UNSUPPORTED, "gemv_int4: n_in %d (at most %d)", n_in, 2 * W4_K_CTA * W4_CLUSTER * W4_K);

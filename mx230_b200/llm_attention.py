@@ -12,7 +12,7 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._lib import addr, check, lib, ptr, require
+from ._lib import addr, check, lib, ptr, require, require_int32
 from .common import Handle, raw_stream, stream_ptr
 
 KV_BLOCK = 16  # 03-llm-engine/src/gpu.rs:209
@@ -107,6 +107,7 @@ class Rotary:
         given = {} if scaling is None else {k: v for k, v in scaling.items() if k != "kind"}
         require(set(given) == ({"factor", *names} if kind else set()), f"Rotary: scaling {scaling!r} needs factor {' '.join(names)}")
         low, high, length = [given[n] for n in names] or (0.0, 0.0, 0)
+        require_int32("Rotary", rot_dim, length)
         table, factor = (C.c_uint64 * max(1, rot_dim // 2))(), C.c_float()
         check(lib().mx230_rotary_table(table, C.byref(factor), rot_dim, theta, kind, given.get("factor", 1.0), low, high, length))
         self.rot_dim, self.interleaved, self.factor = rot_dim, int(interleaved), factor.value
@@ -131,6 +132,7 @@ def rotary(h: Handle, out, x, pos, plan: Rotary, inverse=False, stream=None):
         on_device(h, "rotary: pos", pos, torch.int32)
         require(pos.shape == (n,) and (n < 2 or pos.stride(0) == 1), lambda: f"rotary: positions {tuple(pos.shape)} for {n} rows")
         at, first = pos.data_ptr(), 0
+    require_int32("rotary", n, heads, dim, first)
     check(lib().mx230_rotary(h._h, raw_stream(stream, dev), out.data_ptr(), x.data_ptr(), _DTYPES[dtype], at, first, plan._addr, plan.factor,
                              n, heads, dim, plan.rot_dim, plan.interleaved, inverse, xr, xh, outr, outh))
 
@@ -463,6 +465,7 @@ def pack_int4(h: Handle, codes, scales, zeros=None, group: int | None = None, st
         require(len(fits) == 1, lambda: f"pack_int4: {groups} groups of {n_in} inputs: give the group")
         group = fits[0]
     require(group > 0 and -(-n_in // group) == groups, lambda: f"pack_int4: {groups} groups of {group} for {n_in} inputs")
+    require_int32("pack_int4", n_in, n_out, group)
     on_device(h, "pack_int4: codes", codes, torch.uint8), on_device(h, "pack_int4: scales", scales, torch.float16)
     require(codes.is_contiguous() and scales.is_contiguous(), "pack_int4: codes and scales must be contiguous")
     if zeros is not None:
@@ -493,7 +496,9 @@ def gemv_int4(h: Handle, y, x, w: Int4Weights, b=None, add=None, stream=None):
         on_device(h, "gemv_int4: add", add, f32)
         ad, plus = add.stride(), add.data_ptr()
         require(add.shape == ys and (n_out == 1 or ad[-1] == 1), "gemv_int4: add must have the shape of y, its rows contiguous")
-    check(lib().mx230_gemv_int4(h._h, raw_stream(stream, dev), y.data_ptr(), x.data_ptr(), w._addr, bias, plus, rows[0] if rows else 1, w.n_in,
+    n = rows[0] if rows else 1
+    require_int32("gemv_int4", n)
+    check(lib().mx230_gemv_int4(h._h, raw_stream(stream, dev), y.data_ptr(), x.data_ptr(), w._addr, bias, plus, n, w.n_in,
                                 n_out, w.group, xd[0], yd[0], ad[0]))
 
 

@@ -20,7 +20,7 @@ import numpy as np
 
 import torch
 
-from ._lib import check, lib, require
+from ._lib import check, lib, require, require_int32
 from .common import Handle, raw_stream
 from .llm_attention import _DTYPES, on_device
 from .paging import KvPool
@@ -124,6 +124,7 @@ def sample(h: Handle, token, logits, u, temperature=1.0, top_k=0, top_p=1.0, min
     k, ks = (0, vector("sample: top_k", top_k, torch.int32)) if isinstance(top_k, torch.Tensor) else (top_k, None)
     p, ps = (0.0, vector("sample: top_p", top_p, torch.float32)) if isinstance(top_p, torch.Tensor) else (top_p, None)
     m, ms = (0.0, vector("sample: min_p", min_p, torch.float32)) if isinstance(min_p, torch.Tensor) else (min_p, None)
+    require_int32("sample", n, vocab, k)
     check(lib().mx230_sample(h._h, raw_stream(stream, dev), vector("sample: token", token, torch.int32),
                              None if prob is None else vector("sample: prob", prob, torch.float32), logits.data_ptr(), dtype, n, vocab, row,
                              vector("sample: u", u, torch.float32), t, ts, k, ks, p, ps, m, ms))
@@ -134,6 +135,7 @@ class Sampler:
     request's tokens do not depend on what is served beside it."""
 
     def __init__(self, h: Handle, seed: int = 0):
+        require(0 <= seed < 1 << 128, f"Sampler: seed {seed} (0 to 2^128 - 1)")
         self.h, self.seed = h, seed
 
     def uniform(self, request: int, step: int) -> float:

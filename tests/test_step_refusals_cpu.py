@@ -5,8 +5,10 @@ import math
 
 import numpy as np
 import pytest
+import torch
 
-from mx230_b200 import _lib
+from mx230_b200 import _lib, serving
+from mx230_b200 import llm_attention as la
 
 
 @pytest.fixture(scope="module")
@@ -52,9 +54,10 @@ def test_rotary_table(L):
 
 
 def test_int4_refuses(L):
-    ok = dict(h=H, st=None, y=P, x=P, packed=P, bias=None, add=None, rows=4, n_in=256, n_out=64, group=64, xs=256, ys=64, adds=0)
+    ok = dict(h=H, st=None, y=P, x=P + 65536, packed=P, bias=None, add=None, rows=4, n_in=256, n_out=64, group=64, xs=256, ys=64, adds=0)
     cases = [dict(h=None), dict(y=None), dict(x=None), dict(packed=None), dict(rows=-1), dict(n_in=0), dict(n_out=0), dict(n_in=-5), dict(xs=-1),
-             dict(ys=63), dict(ys=-64), dict(add=P + 64, adds=-1), dict(add=P, adds=0), dict(packed=P + 8), dict(y=P + 2), dict(x=P + 1), dict(bias=P + 2)]
+             dict(ys=63), dict(ys=-64), dict(add=P + 64, adds=-1), dict(add=P, adds=0), dict(packed=P + 8), dict(y=P + 2), dict(x=P + 1), dict(bias=P + 2), dict(x=P), dict(bias=P),
+             dict(rows=1, x=P)]
     for c in cases:
         assert L.mx230_gemv_int4(*{**ok, **c}.values()) == _lib.ERR_INVALID_ARG, c
     for g in (0, -64, 16, 48, 96, 31):
@@ -82,3 +85,66 @@ def test_sample_refuses(L):
     assert L.mx230_sample(*{**ok, "vocab": (1 << 22) + 1}.values()) == _lib.ERR_UNSUPPORTED
     assert L.mx230_sample(*{**ok, "rows": 1 << 28}.values()) == _lib.ERR_UNSUPPORTED
     assert L.mx230_sample(*{**ok, "rows": 0}.values()) == 0
+
+
+class _Lib:
+    """In the library's place: a call of it fails the test."""
+
+    def __getattr__(self, name):
+        raise AssertionError(f"{name} was called")
+
+
+class _Handle:
+    device, _h = 0, H
+
+
+class _Tensor(torch.Tensor):
+    """A tensor of the CPU that says that it lies on device 0."""
+
+    def get_device(self):
+        return 0
+
+
+def t(*shape, dtype=torch.float32):
+    return torch.empty(*shape, dtype=dtype).as_subclass(_Tensor)
+
+
+@pytest.mark.parametrize("big", [1 << 31, (1 << 32) + 1, -(1 << 31) - 1, -(1 << 40)])
+def test_numbers_beyond_32_bits(monkeypatch, big):
+    """An int argument would lose its upper bits on the way into the library."""
+    monkeypatch.setattr(_lib, "_lib", _Lib())
+    h, x = _Handle(), t(3, 2, 8)
+    plan = la.Rotary.__new__(la.Rotary)
+    plan.rot_dim, plan.interleaved, plan.factor, plan._addr, plan._device = 8, 0, 1.0, P, 0
+    refused = []
+    for call in (lambda: la.rotary(h, x, x, big, plan, stream=0), lambda: la.Rotary(big, 1e4, device="cpu"),
+                 lambda: la.Rotary(8, 1e4, {"kind": "yarn", "factor": 2.0, "slow": 1.0, "fast": 32.0, "length": big}, device="cpu"),
+                 lambda: la.pack_int4(h, t(40, 8, dtype=torch.uint8), t(1, 8, dtype=torch.float16), group=big, stream=0),
+                 lambda: serving.sample(h, t(3, dtype=torch.int32), t(3, 10), t(3), top_k=big, stream=0)):
+        with pytest.raises(_lib.Mx230Error) as e:
+            call()
+        refused.append(e.value.code)
+    assert refused == [_lib.ERR_INVALID_ARG] * 5
+
+
+def test_lengths_beyond_32_bits(monkeypatch):
+    monkeypatch.setattr(_lib, "_lib", _Lib())
+    h, n = _Handle(), (1 << 32) + 1
+    plan = la.Rotary.__new__(la.Rotary)
+    plan.rot_dim, plan.interleaved, plan.factor, plan._addr, plan._device = 2, 0, 1.0, P, 0
+    one = lambda dtype=torch.float32: t(1, dtype=dtype)  # noqa: E731
+    many = lambda *shape, dtype=torch.float32: one(dtype).expand(*shape)  # noqa: E731
+    w = la.Int4Weights.__new__(la.Int4Weights)
+    w.packed, w.n_in, w.n_out, w.group, w._addr, w._device = None, 1, 1, 64, P, 0
+    for call in (lambda: la.rotary(h, many(n, 1, 1), many(n, 1, 1), 0, plan, stream=0),
+                 lambda: la.gemv_int4(h, many(n, 1), many(n, 1), w, stream=0),
+                 lambda: serving.sample(h, many(n, dtype=torch.int32), many(n, 1), many(n), stream=0)):
+        with pytest.raises(_lib.Mx230Error):
+            call()
+
+
+def test_seeds():
+    for seed in (-1, 1 << 128):
+        with pytest.raises(_lib.Mx230Error):
+            serving.Sampler(_Handle(), seed)
+    assert 0.0 <= serving.Sampler(_Handle(), (1 << 128) - 1).uniform(0, 0) < 1.0
