@@ -2,12 +2,17 @@
 each head, the KV write and attention over a paged cache, 4-bit logits, and tokens drawn by each request's settings inside
 `run_continuous`.  Served together and one at a time the tokens are the same, and the logits are those of the same
 layer in 64 bits."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
 
 from mx230_b200 import _lib
 from mx230_b200 import llm_attention as la
+from mx230_b200 import serving
 from mx230_b200.paging import KvPool
 from mx230_b200.serving import Request, Sampler, run_continuous
 from tests.conftest import assert_close
@@ -129,3 +134,77 @@ def test_a_masked_row_is_an_error(handle):
     sampler = Sampler(handle)
     with pytest.raises(_lib.Mx230Error):
         sampler.draw(torch.full((1, 50), float("-inf"), device="cuda"), [(3, 0, Request([1], 1))])
+
+
+FIRST_CALLS = """
+import torch
+from mx230_b200 import llm_attention as la, serving
+from mx230_b200.common import Handle
+torch.cuda.set_device(0)
+h = Handle(0, 16 << 20)
+g = torch.Generator(device="cuda").manual_seed(0)
+plan = la.Rotary(64, 1e4, device="cuda")
+made = []
+for n_in, n_out, rows in ((896, 300, 1), (4864, 896, 6), (14336, 512, 3)):
+    codes = torch.randint(0, 16, (n_in, n_out), device="cuda", dtype=torch.uint8, generator=g)
+    w = la.pack_int4(h, codes, torch.rand(-(-n_in // 64), n_out, device="cuda", generator=g).half(), group=64)
+    made.append((torch.empty(rows, n_out, device="cuda"), torch.randn(rows, n_in, device="cuda", generator=g), w))
+x = torch.randn(5, 4, 64, device="cuda", generator=g)
+out = torch.empty_like(x)
+logits, u = torch.randn(3, 70000, device="cuda", generator=g), torch.rand(3, device="cuda", generator=g)
+token = torch.empty(3, dtype=torch.int32, device="cuda")
+def calls():
+    for y, a, w in made:
+        la.gemv_int4(h, y, a, w)
+    la.rotary(h, out, x, 7, plan)
+    serving.sample(h, token, logits, u, top_p=0.9)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    calls()
+graph.replay()
+torch.cuda.synchronize()
+results = [y for y, *_ in made] + [out, token]
+captured = [r.clone() for r in results]
+for r in results:
+    r.zero_()
+calls()
+assert all(torch.equal(a, b) for a, b in zip(results, captured))
+h.check_status()
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    """What the host asks and sets once (attributes, clusters that fit) it may do while a stream is captured."""
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS], capture_output=True, text=True, timeout=300,
+                          cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_two_streams_at_once(handle):
+    """No call has a workspace: two of a kind on two streams, over and over, with the results of one after the other."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    codes = torch.randint(0, 16, (14336, 1024), device="cuda", dtype=torch.uint8, generator=g)
+    w = la.pack_int4(handle, codes, torch.rand(224, 1024, device="cuda", generator=g).half(), group=64)
+    xs = [torch.randn(n, 14336, device="cuda", generator=g) for n in (3, 8)]
+    logits = [torch.randn(n, 128000, device="cuda", generator=g) * 3 for n in (2, 40)]
+    us = [torch.rand(l.shape[0], device="cuda", generator=g) for l in logits]
+    ys = [torch.empty(x.shape[0], 1024, device="cuda") for x in xs]
+    tokens = [torch.empty(l.shape[0], dtype=torch.int32, device="cuda") for l in logits]
+
+    def calls(i, **kw):
+        la.gemv_int4(handle, ys[i], xs[i], w, **kw)
+        serving.sample(handle, tokens[i], logits[i], us[i], top_p=0.95, **kw)
+
+    calls(0), calls(1)
+    want = [t.clone() for t in ys + tokens]
+    torch.cuda.synchronize()
+    for t in ys + tokens:
+        t.zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        calls(0, stream=streams[0]), calls(1, stream=streams[1])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(ys + tokens, want))
+    handle.check_status()
