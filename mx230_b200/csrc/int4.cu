@@ -388,14 +388,38 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
     }
 }
 
+// Clusters of C CTAs that the device holds at once, each of which fills an SM (asked once per size, of any form of the kernel).
+int clusters_held(mx230_handle *h, int C, int *held) {
+    static int fit[64][4];
+    const int size = C == 2 ? 1 : C == 4 ? 2 : 3;
+    *held = h->sm_count;
+    if (C == 1) return MX230_OK;
+    if (h->device >= 64 || fit[h->device][size] == 0) {
+        MX_SMEM_ATTR_ONCE(h->device, (gemv_int4_kernel<1, 1, false>), W4_SMEM);
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute at;
+        cfg.gridDim = dim3(C), cfg.blockDim = dim3(W4_THREADS + W4_PRODUCER), cfg.dynamicSmemBytes = W4_SMEM, cfg.attrs = &at, cfg.numAttrs = 1;
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = C, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+        MX_CHECK_CUDA(cudaOccupancyMaxActiveClusters(held, gemv_int4_kernel<1, 1, false>, &cfg));
+        if (*held < 1) *held = 1;
+        if (h->device < 64) fit[h->device][size] = *held;
+    } else *held = fit[h->device][size];
+    return MX230_OK;
+}
+
+// What comes before the ring in shared memory: rows and sums.
+size_t fixed_bytes(const Int4Params &P, int x_tile, int sums) {
+    return (size_t)2 * (W4_WARPS + (P.ctas_k > 1 ? 1 : 0)) * sums * 4 + 32 + (size_t)P.k_cta * x_tile;
+}
+
 template <int NT, int T, bool G32>
-int launch_int4(mx230_handle *h, cudaStream_t st, Int4Params P, int x_tile) {
+int launch_int4(mx230_handle *h, cudaStream_t st, Int4Params P, int x_tile, int held) {
     using S = Int4Form<NT, T, G32>;
-    const int C = P.ctas_k;
     P.n_groups = (P.n_tiles + T - 1) / T;
     // Shared memory: rows and sums, and what is left for stages, of four tiles a warp where three of them fit, or two, or one (a whole
     // number of turns; 4096 x 128000, one row: 64 us with two, 57 with four).
-    const size_t fixed = (size_t)2 * (W4_WARPS + (C > 1 ? 1 : 0)) * S::SUMS * 4 + 32 + (size_t)P.k_cta * x_tile;
+    const size_t fixed = fixed_bytes(P, x_tile, S::SUMS);
     P.stage_k = 4 * W4_WARPS;
     while (P.stage_k > W4_WARPS && fixed + (size_t)(P.stage_k == 2 * W4_WARPS ? 2 : 3) * T * P.stage_k * S::TILE > W4_SMEM) P.stage_k /= 2;
     if (P.stage_k > P.k_cta) P.stage_k = P.k_cta;
@@ -405,25 +429,9 @@ int launch_int4(mx230_handle *h, cudaStream_t st, Int4Params P, int x_tile) {
     if (P.stages > W4_STAGES) P.stages = W4_STAGES;
     const size_t sm = fixed + P.stages * stage;
     MX_SMEM_ATTR_ONCE(h->device, (gemv_int4_kernel<NT, T, G32>), W4_SMEM);
-    // clusters that the device holds at once, of CTAs that fill an SM (asked once per size)
-    static int fit[64][4];
-    const int size = C == 1 ? 0 : C == 2 ? 1 : C == 4 ? 2 : 3;
-    int held = h->sm_count;
-    if (C > 1) {
-        if (h->device >= 64 || fit[h->device][size] == 0) {
-            cudaLaunchConfig_t cfg = {};
-            cudaLaunchAttribute at;
-            cfg.gridDim = dim3(C), cfg.blockDim = dim3(W4_THREADS + W4_PRODUCER), cfg.dynamicSmemBytes = W4_SMEM, cfg.attrs = &at, cfg.numAttrs = 1;
-            at.id = cudaLaunchAttributeClusterDimension;
-            at.val.clusterDim.x = C, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
-            MX_CHECK_CUDA(cudaOccupancyMaxActiveClusters(&held, gemv_int4_kernel<NT, T, G32>, &cfg));
-            if (held < 1) held = 1;
-            if (h->device < 64) fit[h->device][size] = held;
-        } else held = fit[h->device][size];
-    }
     P.n_clusters = held < P.n_groups ? held : P.n_groups;
-    const dim3 grid((unsigned)(P.n_clusters * C), (unsigned)((P.n_rows + 4 * NT - 1) / (4 * NT)));
-    MX_LAUNCH(h, st, MX230_K_GEMV_INT4, mx_launch(gemv_int4_kernel<NT, T, G32>, grid, W4_THREADS + W4_PRODUCER, sm, st, C, true, P));
+    const dim3 grid((unsigned)(P.n_clusters * P.ctas_k), (unsigned)((P.n_rows + 4 * NT - 1) / (4 * NT)));
+    MX_LAUNCH(h, st, MX230_K_GEMV_INT4, mx_launch(gemv_int4_kernel<NT, T, G32>, grid, W4_THREADS + W4_PRODUCER, sm, st, P.ctas_k, true, P));
     return MX230_OK;
 }
 
@@ -496,19 +504,33 @@ extern "C" int mx230_gemv_int4(mx230_handle *h, void *stream, float *y, const fl
     P.k_cta = (P.k_tiles + P.ctas_k - 1) / P.ctas_k;
     // Rows of a pass: eight, or four where eight do not fit.
     const int nt = n_rows <= 4 || P.k_cta > W4_K_CTA ? 1 : 2, x_tile = nt * (32 * (nt == 1 ? 8 * (n_rows < 4 ? n_rows : 4) : 32) + 64);
-    // Output tiles of a warp, which share what is read of the rows: two where half the SMs then have a group of them, four (of few rows)
-    // where they have three groups for two SMs (one row, us with one / two / four: 896 x 1152 2.4, 2.7, 3.3; 4096 x 4096 5.5, 4.9, 6.1;
-    // 4096 x 14336 12.6, 11.3, 10.8; 4096 x 128000 80, 58, 56).
-    const long long here = (long long)P.n_tiles * P.ctas_k;
-    const int t = nt == 1 && here * 2 >= 4 * 3ll * h->sm_count * 95 / 100 ? 4 : here >= h->sm_count ? 2 : 1;
     mx230_device_guard guard(h->device);
-    cudaStream_t st = (cudaStream_t)stream;
+    int held;
+    rc = clusters_held(h, P.ctas_k, &held);
+    if (rc) return rc;
     const bool g32 = group == 32;
+    // Output tiles of a warp, which share what is read of the rows.  Four rows: one, two or four, whichever needs least time, taken as
+    // rounds of the clusters times 3, 5 or 9 (three rows and more: 10).  One row, us with one / two / four: 896 x 1152 2.3, 2.7, 3.5;
+    // 4096 x 4096 5.3, 5.0, 6.5; 4096 x 14336 12.1, 11.8, 11.5; 4096 x 128000 78, 67, 59 (four rows 83, 69, 72).  Eight rows: two where there
+    // is a round of them and three stages fit beside the rows (14336 x 4096 25.1, 22.4; 4096 x 14336, where two stages would, 18.9, 21.3).
+    int t = 1;
     if (nt == 1) {
-        if (t == 4) return g32 ? launch_int4<1, 4, true>(h, st, P, x_tile) : launch_int4<1, 4, false>(h, st, P, x_tile);
-        if (t == 2) return g32 ? launch_int4<1, 2, true>(h, st, P, x_tile) : launch_int4<1, 2, false>(h, st, P, x_tile);
-        return g32 ? launch_int4<1, 1, true>(h, st, P, x_tile) : launch_int4<1, 1, false>(h, st, P, x_tile);
+        const int cost[3] = {30, 50, n_rows < 3 ? 89 : 101};
+        long long best = 0;
+        for (int i = 0; i < 3; ++i) {
+            const long long groups = (P.n_tiles + (1 << i) - 1) >> i, time = (groups + held - 1) / held * cost[i];
+            if (i == 0 || time < best) best = time, t = 1 << i;
+        }
+    } else if (P.n_tiles > held) {
+        const size_t stage = (size_t)2 * W4_WARPS * (g32 ? Int4Form<2, 2, true>::TILE : Int4Form<2, 2, false>::TILE);
+        if (fixed_bytes(P, x_tile, Int4Form<2, 2, false>::SUMS) + 3 * stage <= W4_SMEM) t = 2;
     }
-    if (t == 2) return g32 ? launch_int4<2, 2, true>(h, st, P, x_tile) : launch_int4<2, 2, false>(h, st, P, x_tile);
-    return g32 ? launch_int4<2, 1, true>(h, st, P, x_tile) : launch_int4<2, 1, false>(h, st, P, x_tile);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (nt == 1) {
+        if (t == 4) return g32 ? launch_int4<1, 4, true>(h, st, P, x_tile, held) : launch_int4<1, 4, false>(h, st, P, x_tile, held);
+        if (t == 2) return g32 ? launch_int4<1, 2, true>(h, st, P, x_tile, held) : launch_int4<1, 2, false>(h, st, P, x_tile, held);
+        return g32 ? launch_int4<1, 1, true>(h, st, P, x_tile, held) : launch_int4<1, 1, false>(h, st, P, x_tile, held);
+    }
+    if (t == 2) return g32 ? launch_int4<2, 2, true>(h, st, P, x_tile, held) : launch_int4<2, 2, false>(h, st, P, x_tile, held);
+    return g32 ? launch_int4<2, 1, true>(h, st, P, x_tile, held) : launch_int4<2, 1, false>(h, st, P, x_tile, held);
 }
