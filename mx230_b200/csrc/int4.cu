@@ -7,14 +7,15 @@
 // tensor-core tiles (m16n8k16) with the weights as A: 16 outputs x 16 inputs.  Four bits at places 4 to 7 of an fp16 are the number
 // q 2^-20 (a subnormal, which the tensor cores take as it is), so a pair of weights costs an "and" and three quarters of a shift.  (At
 // places 0 to 3 they are q 2^-24, one shift less a pair, but the products of a step are added with the digits that the largest possible
-// number of a subnormal's exponent leaves, ten bits above q: 1.3e-6 of the result over 4096 inputs, 0.3e-6 so.)  The rows are the eight
+// number of a subnormal's exponent leaves, ten bits above q: 1.3e-6 of the result over 4096 inputs, 0.2e-6 so.)  The rows are the eight
 // columns of B, two columns a row:
 //   x 2^e = hi + lo, both fp16, e such that the largest of the 64 values of a tile lies in [2^14, 2^15):
 // |x 2^e - hi - lo| <= 2^-24 |x 2^e|, as exact as x itself (but for values 2^-17 times the tile's largest and less, which keep an
 // absolute error of 2^-39 of that).  Products are then exact in fp32; sums are fp32, per tile of 64 inputs (32, if groups are of
 // 32).  The zero point meets the sum of the tile's x: the row's total gets s 2^(20 - e) (sum x q - z sum x), whose error goes by
 // sum |x| (q + z) instead of sum |x (q - z)|, about four times that, and saves the subtraction per weight (161 instructions a
-// warp and tile with it, of which 36 for the conversion; the kernel was bound by them: 37 us for 4096 x 14336, one row).
+// warp and tile with it, of which 36 for the conversion; about 80 without: of 4096 x 14336, one row, 11.5 us are left, 71 of 4096 x 128000
+// for four, where HBM would need 4.7 and 42).
 //
 // Layout, made once by mx230_pack_int4: tiles of 16 outputs x 64 inputs, 512 bytes, of which lane (g = lane / 4, j = lane % 4) has 16:
 // words [row g: inputs 8j .. 8j+7][row g: inputs 32 + 8j ..][row g + 8: 8j ..][row g + 8: 32 + 8j ..], input 2p of eight at bits
@@ -23,7 +24,7 @@
 //
 // Weights come by bulk copies, a lane's for a CTA of sixteen warps, into a ring of stages (some output tiles, up to 32 tiles of their
 // inputs each: 16 KB in a row and their (s, z)).  Loads to registers, two to four tiles ahead, kept too few bytes on their way with
-// the warps that fit beside them (16 of them read 5.5 TB/s with nothing else to do, 32 read 6.1), and took four instructions a
+// the warps that fit beside them (16 of them read 5.6 TB/s with nothing else to do, 32 read 6.1), and took four instructions a
 // tile; a ring by cp.async of every lane took as many; bulk copies by the warp, of a KB, were bound by their number.
 //
 // Order of the sums: the inputs are cut over the CTAs of a cluster and there by turns over sixteen warps (a tile each), by n_in and n_out
@@ -418,7 +419,7 @@ int launch_int4(mx230_handle *h, cudaStream_t st, Int4Params P, int x_tile, int 
     using S = Int4Form<NT, T, G32>;
     P.n_groups = (P.n_tiles + T - 1) / T;
     // Shared memory: rows and sums, and what is left for stages, of four tiles a warp where three of them fit, or two, or one (a whole
-    // number of turns; 4096 x 128000, one row: 64 us with two, 57 with four).
+    // number of turns; 4096 x 128000, one row: four take a tenth less than two).
     const size_t fixed = fixed_bytes(P, x_tile, S::SUMS);
     P.stage_k = 4 * W4_WARPS;
     while (P.stage_k > W4_WARPS && fixed + (size_t)(P.stage_k == 2 * W4_WARPS ? 2 : 3) * T * P.stage_k * S::TILE > W4_SMEM) P.stage_k /= 2;

