@@ -176,7 +176,7 @@ __device__ __forceinline__ float finite(float l) {   // infinity is the largest 
 constexpr float SM_INTERVAL = 8388608.0f;
 __device__ __forceinline__ float interval(float l, float m, float scale) { return fmaf(m - l, scale, SM_INTERVAL); }
 
-// running sums of n counts and masses (n <= PER * SM_THREADS), PER a thread, in place; counts may be null
+// running sums of n counts and masses (n <= PER * SM_THREADS), PER a thread, in place; either may be null
 template <int PER>
 __device__ __forceinline__ void running_sums(unsigned *cnt, u64 *mass, int n, Shared &S) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i0 = PER * threadIdx.x;
@@ -184,16 +184,21 @@ __device__ __forceinline__ void running_sums(unsigned *cnt, u64 *mass, int n, Sh
     unsigned cs[PER], c = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        m += i0 + i < n ? mass[i0 + i] : 0, c += cnt && i0 + i < n ? cnt[i0 + i] : 0;
+        m += mass && i0 + i < n ? mass[i0 + i] : 0, c += cnt && i0 + i < n ? cnt[i0 + i] : 0;
         ms[i] = m, cs[i] = c;
     }
     const u64 own_m = m;
     const unsigned own_c = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const u64 mu = __shfl_up_sync(0xFFFFFFFFu, m, o);
-        const unsigned cu = __shfl_up_sync(0xFFFFFFFFu, c, o);
-        if (lane >= o) m += mu, c += cu;
+        if (mass) {
+            const u64 mu = __shfl_up_sync(0xFFFFFFFFu, m, o);
+            if (lane >= o) m += mu;
+        }
+        if (cnt) {
+            const unsigned cu = __shfl_up_sync(0xFFFFFFFFu, c, o);
+            if (lane >= o) c += cu;
+        }
     }
     if (lane == 31) S.scan[warp] = m, S.scan_cnt[warp] = c;
     __syncthreads();
@@ -202,14 +207,14 @@ __device__ __forceinline__ void running_sums(unsigned *cnt, u64 *mass, int n, Sh
     unsigned cb = lane < warp ? S.scan_cnt[lane] : 0;
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) {
-        before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
-        cb += __shfl_xor_sync(0xFFFFFFFFu, cb, o);
+        if (mass) before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
+        if (cnt) cb += __shfl_xor_sync(0xFFFFFFFFu, cb, o);
     }
     before = __shfl_sync(0xFFFFFFFFu, before, 0) + m - own_m, cb = __shfl_sync(0xFFFFFFFFu, cb, 0) + c - own_c;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
         if (i0 + i < n) {
-            mass[i0 + i] = before + ms[i];
+            if (mass) mass[i0 + i] = before + ms[i];
             if (cnt) cnt[i0 + i] = cb + cs[i];
         }
     __syncthreads();
@@ -274,7 +279,18 @@ __device__ __forceinline__ void sort_entries(u64 *v, u64 *other, int n) {
 }
 __device__ __forceinline__ void sort_down(u64 *v, u64 *other, int n) {
     static_assert(SM_LIST == 2 * SM_THREADS, "two entries a thread");
-    if (n <= SM_THREADS) sort_entries<1>(v, other, n);
+    if (n <= SM_THREADS / 4) {   // few: an entry's place is the number of larger ones (no two are equal), counted by four lanes
+        const int i = min((int)threadIdx.x >> 2, max(n - 1, 0));
+        const u64 e = v[i];
+        int place = 0;
+#pragma unroll 4
+        for (int o = threadIdx.x & 3; o < n; o += 4) place += v[o] > e;
+        place += __shfl_xor_sync(0xFFFFFFFFu, place, 1);
+        place += __shfl_xor_sync(0xFFFFFFFFu, place, 2);
+        __syncthreads();
+        if (threadIdx.x < 4 * n && (threadIdx.x & 3) == 0) v[place] = e;
+        __syncthreads();
+    } else if (n <= SM_THREADS) sort_entries<1>(v, other, n);
     else sort_entries<2>(v, other, n);
 }
 
@@ -290,6 +306,10 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
     mx::pdl_trigger();
     __syncwarp();
     mx::cluster_arrive_relaxed();   // waited for before the first store to another CTA's memory
+    auto clear_histogram = [&]() {   // (its three arrays follow one another)
+        for (int i = tid; i < (int)(3 * sizeof(S.cnt) / 16); i += SM_THREADS) ((uint4 *)S.cnt)[i] = make_uint4(0, 0, 0, 0);
+    };
+    clear_histogram();
     mx::pdl_wait();
 
     float T_ = P.temperatures ? P.temperatures[row] : P.temperature;
@@ -412,33 +432,35 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
         if (h) atomicAdd(&S.hi[b], h);
     };
     auto clear = [&]() {
-        for (int b = tid; b < SM_BINS + 32; b += SM_THREADS) S.cnt[b] = S.lo[b] = S.hi[b] = 0;
+        clear_histogram();
         __syncthreads();
     };
     int turn = 0;
     auto answer = [&]() { return &S.found[turn++ & 3]; };
     // the CTAs' histograms, added up by shares of the intervals into the first CTA's arrays, there as running sums
-    auto merge = [&](unsigned *to_cnt, u64 *to_mass, bool counted, auto bins) {
+    auto merge = [&](unsigned *to_cnt, u64 *to_mass, bool counted, bool weighed, auto bins) {
         cluster_sync();
         const int b0 = bins.value / C * rank;
         for (int b = b0 + tid; b < b0 + bins.value / C; b += SM_THREADS) {
             unsigned c = 0;
             u64 ms = 0;
+            if (counted)
 #pragma unroll 8
-            for (int r = 0; r < C; ++r) {
-                c += ld_cluster32(mx::cluster_map(mx::smem_u32(&S.cnt[b]), r));
-                ms += (u64)ld_cluster32(mx::cluster_map(mx::smem_u32(&S.hi[b]), r)) << 32 | ld_cluster32(mx::cluster_map(mx::smem_u32(&S.lo[b]), r));
-            }
+                for (int r = 0; r < C; ++r) c += ld_cluster32(mx::cluster_map(mx::smem_u32(&S.cnt[b]), r));
+            if (weighed)
+#pragma unroll 8
+                for (int r = 0; r < C; ++r)
+                    ms += (u64)ld_cluster32(mx::cluster_map(mx::smem_u32(&S.hi[b]), r)) << 32 | ld_cluster32(mx::cluster_map(mx::smem_u32(&S.lo[b]), r));
             if (!counted) {
                 // at most so many have this mass: none has less than the interval's end (the masses are whole; below 1: any number)
                 const double least_mass = floor(weight(fmax(-(b + 0.51) / (double)scale, -28.75 * (double)T_), log2e_t, P.power) * (SM_MASS * (1 - 1e-6)) - 0.5);
                 c = least_mass >= 1.0 ? (unsigned)fmin((double)ms / least_mass + 1.0, SM_LIST + 1.0) : SM_LIST + 1;
             }
             st_cluster(mx::cluster_map(mx::smem_u32(&to_cnt[b]), 0), c);
-            st_cluster(mx::cluster_map(mx::smem_u32(&to_mass[b]), 0), ms);
+            if (weighed) st_cluster(mx::cluster_map(mx::smem_u32(&to_mass[b]), 0), ms);
         }
         cluster_sync();
-        if (first_cta) running_sums<bins.value / SM_THREADS>(to_cnt, to_mass, bins.value, S);
+        if (first_cta) running_sums<bins.value / SM_THREADS>(to_cnt, weighed ? to_mass : nullptr, bins.value, S);
     };
     // first CTA, by warp 0, of whose lane 0 this is the next window: it goes to all; then it is the one in force
     int wp = 0;
@@ -553,7 +575,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
                 add_to(b, mass(l));
             });
             unsigned *c_run = (unsigned *)S.all;   // (no list is in use)
-            merge(c_run, S.mine, true, std::integral_constant<int, SM_LIST>());
+            merge(c_run, S.mine, true, true, std::integral_constant<int, SM_LIST>());
             if (first_cta) {
                 next = S.w[wp];
                 const u64 left = t - (by_mass ? next.base_mass : next.base_count);
@@ -611,9 +633,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
         }, Weigh());
     };
     u64 z = 0, z_min = 0;   // first CTA: mass of K, then of what is kept; of M
-    for (;;) {
+    for (bool again = false;; again = true) {
         // ---- histogram over max - l ----
-        clear();
+        if (again) clear();
         sum_min = 0;
         if (!with_mass) histogram(std::true_type(), std::false_type());
         else if (with_count) histogram(std::true_type(), std::true_type());
@@ -628,13 +650,13 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
                 st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_b[rank]), 0), sum_min);
             }
         }
-        merge(S.run_cnt, S.run_mass, with_count, std::integral_constant<int, SM_BINS>());
+        merge(S.run_cnt, S.run_mass, with_count, with_mass, std::integral_constant<int, SM_BINS>());
         // ---- what is to be looked at: all that can be kept, if that is a list; else (k = 0) the interval where P ends and those where
         // the token then can be, if they are; else more than that ----
         Window next{};
         if (first_cta) {
             const unsigned there = S.run_cnt[SM_BINS - 1];
-            z = z_min = S.run_mass[SM_BINS - 1];
+            z = z_min = with_mass ? S.run_mass[SM_BINS - 1] : 0;   // (else known from the list)
             int b = SM_BINS - 1;
             if (k) b = first_over(S.run_cnt, SM_BINS, (u64)min((unsigned)k, there) - 1, answer());
             else if (p < 1.0f) b = first_over(S.run_mass, SM_BINS, (u64)ceil((double)p * (double)z) - 1, answer());
@@ -672,7 +694,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
         const Window w = S.w[wp];
         const bool one = w.c1 == w.b1;
         const u64 front = w.c0 ? S.run_mass[w.c0 - 1] : 0;
-        const u64 in_c = S.run_mass[w.c1] - front, between = one ? 0 : S.run_mass[w.b0 - 1] - S.run_mass[w.c1];
+        const u64 in_c = one ? 0 : S.run_mass[w.c1] - front, between = one ? 0 : S.run_mass[w.b0 - 1] - S.run_mass[w.c1];
         if (k) z = S.mine[min(k, total) - 1];
         u64 keep = z;
         if (p < 1.0f) keep = front + between + S.mine[first_over(S.mine, total, (u64)ceil((double)p * (double)z) - 1 - front - between, answer())];
