@@ -12,7 +12,7 @@
 // target known from the one before (the intersection of two prefixes has the smaller of their masses).
 //
 // The logits have to be read once, 4 or 2 bytes each; what bounds the kernel is instructions, about 85 a warp for 32 logits that are
-// weighed (64 rows of 128000 in fp32 with top-p 0.95: 51 us, 5 of them HBM's), and for a few rows latency (one row of 32000: 12 us).
+// weighed (64 rows of 128000 in fp32 with top-p 0.95: 51 us, 5 of them HBM's), and for a few rows latency (one row of 32000: 10 us).
 // A cluster of one to eight CTAs takes a row.  A histogram over 2048 equal intervals of max - l, as far as weights are not 0 (28.7 T), in
 // counts (top-k) or masses says which intervals hold the entries that are sought: all down to P's or K's end, if that is one list, or
 // the interval where P ends and those where the token then can be.  Their entries alone are collected, sorted and summed.  Where

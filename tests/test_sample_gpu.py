@@ -88,6 +88,17 @@ def test_matches_the_definition(handle, vocab, dtype, s):
     check(handle, x, uniforms(n, vocab), **s, what=(vocab, s))
 
 
+@pytest.mark.parametrize("vocab", [2, 3, 31, 33, 127, 128, 129, 130, 511, 512, 513, 1023, 1024, 1025])
+def test_lists_of_every_length(handle, vocab):
+    """Rows that are looked at whole, however long the list: equal logits among them, and the last entry drawn."""
+    x = logits_of(5, vocab, 1.0, vocab)
+    x[1] = x[1].round()
+    x[2] = 0.5
+    x[3, : vocab // 2] = -math.inf
+    for s in (dict(k=vocab - 1), dict(p=0.99), dict(t=2.0, k=vocab // 2 + 1, p=0.8), dict(m=0.1)):
+        check(handle, x, [0.5, 0.97, 0.999, 0.2, 1.0], **s, what=(vocab, s))
+
+
 def test_the_largest_vocabulary(handle):
     x = logits_of(1, 1 << 22, 2.0, 5, torch.float32)
     for s in (dict(p=0.9), dict(k=50), dict(t=50.0, k=100_000, p=0.9)):
