@@ -736,15 +736,25 @@ template <typename T>
 int launch_sample(mx230_handle *h, cudaStream_t st, SampleParams P, int n_rows) {
     constexpr int VE = 16 / (int)sizeof(T);
     const int pieces = P.vocab / VE + 2;
-    // CTAs of a row: up to four while there are no three of them for every SM, eight for a few rows (clusters of eight that fill their
-    // SMs find few places: 16 rows of 128000, kept, 26 us with eight, 19 with four; one row 21 and 28), each with a few thousand logits.
+    // CTAs of a row, each with a few thousand logits: two or four where the clusters (which find no place on some SMs)
+    // then all run at once, two CTAs an SM, four of short rows a little earlier; two also where they need up to three halves of that, unless
+    // short rows are asked for a few entries, where what comes behind the passes counts more; eight for a few rows.  us with one / two / four / eight: 64 rows of 128000, top-p 96, 72, 51, 70; 70 rows with two
+    // and four 71, 55; 100 rows 118, 79, 85; 200 rows 142, 124, 134; of 50257, top-k 40, 148 rows 21, 23, 43, and 222 rows 30, 42, 59; 16 rows of 128000, top-k 50,
+    // kept, 43, 29, 18, 24; one row, top-p, kept, 77, 48, 28, 21.
+    const bool few = P.top_ks == nullptr && P.top_k > 0 && P.top_k <= SM_LIST / 2;
+    const bool short_row = P.vocab <= 65536;
+    auto fits = [&](int to) {
+        const long long all = (long long)n_rows * to;
+        if (to == SM_CLUSTER) return all <= h->sm_count / 2;
+        return all * 10 <= (short_row ? 17ll : 19ll) * h->sm_count || (to == 2 && all <= 3ll * h->sm_count && !(few && short_row));
+    };
     int c = 1;
-    while (c < SM_CLUSTER && (long long)n_rows * 2 * c <= (c < 4 ? 3 * h->sm_count : h->sm_count / 2) && P.vocab / c > 4096) c *= 2;
+    while (c < SM_CLUSTER && P.vocab / c > 4096 && fits(2 * c)) c *= 2;
     const int share = ((pieces + c - 1) / c + 1) * VE;
     P.ctas = c;
     P.power = POWER_OF_TWO;
     const dim3 grid((unsigned)(n_rows * c));
-    // The row stays in shared memory where its CTAs all have their places with that (32 rows of 128000, four CTAs each: 33 us, read
+    // The row stays in shared memory where its CTAs all have their places with that (32 rows of 128000, four CTAs each: 34 us, read
     // again 45); else it is read again (64 rows: 51, kept 62).
     const size_t kept = sizeof(Shared) + (size_t)share * sizeof(float);
     MX_SMEM_ATTR_ONCE(h->device, (sample_kernel<T, true>), SM_ALL);
