@@ -14,7 +14,7 @@
 // absolute error of 2^-39 of that).  Products are then exact in fp32; sums are fp32, per tile of 64 inputs (32, if groups are of
 // 32).  The zero point meets the sum of the tile's x: the row's total gets s 2^(20 - e) (sum x q - z sum x), whose error goes by
 // sum |x| (q + z) instead of sum |x (q - z)|, about four times that, and saves the subtraction per weight (161 instructions a
-// warp and tile with it, of which 36 for the conversion; about 80 without: of 4096 x 14336, one row, 11.5 us are left, 71 of 4096 x 128000
+// warp and tile with it, of which 36 for the conversion; about 80 without: of 4096 x 14336, one row, 11.5 us are left, 69 of 4096 x 128000
 // for four, where HBM would need 4.7 and 42).
 //
 // Layout, made once by mx230_pack_int4: tiles of 16 outputs x 64 inputs, 512 bytes, of which lane (g = lane / 4, j = lane % 4) has 16:
