@@ -235,11 +235,12 @@ def _plain_sample(st):
     total = mass.sum(1, keepdim=True)
     mass = torch.where((p >= 1) | (before.double() < p * total.double()), mass, 0)
     mass = torch.where(w >= m, mass, 0)
-    run = torch.cumsum(mass, 1)
+    kept = torch.zeros_like(mass).scatter_(1, order.indices, mass)   # in the order of the vocabulary
+    run = torch.cumsum(kept, 1)
     total = run[:, -1:]
-    at = (run <= torch.floor(st["u"].double()[:, None] * total.double()).long()).sum(1, keepdim=True)
-    prob = mass.gather(1, at).double() / total.double()
-    return {"token": order.indices.gather(1, at)[:, 0].to(torch.int32), "prob": prob[:, 0].float()}
+    token = (run <= torch.floor(st["u"].double()[:, None] * total.double()).long()).sum(1)
+    prob = kept.gather(1, token[:, None]).double() / total.double()
+    return {"token": token.to(torch.int32), "prob": prob[:, 0].float()}
 
 
 def run(state):
@@ -317,10 +318,10 @@ def _exact_sample(case, st):
                 so_far += mass[keep]
                 keep += 1
             likely, w, mass = likely[:keep], w[:keep], mass[:keep]
-        held = [v for v, x in zip(mass, w) if x >= m[r]]
-        total, at = sum(held), 0
+        held = sorted((int(i), v) for i, v, x in zip(likely, mass, w) if x >= m[r])
+        total, at = sum(v for _, v in held), 0
         limit = math.floor(u[r] * float(total))
-        for v in held:
+        for _, v in held:
             at += v
             if at > limit:
                 prob[r] = v / total
