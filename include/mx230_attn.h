@@ -560,11 +560,12 @@ int mx230_qkv_rope_kvwrite(mx230_handle *h, void *stream, float *qkv, const floa
  *   K        the first top_k of that order (all where top_k <= 0)
  *   P        the shortest prefix of K with at least top_p times K's weight (K where top_p >= 1 or NaN, one entry where <= 0)
  *   M        the entries with w_i >= min_p (all where min_p <= 0 or NaN; above 1 it is 1)
- *   token    the first of the order whose running weight, its own included, exceeds u times that of P and M together
- *   prob     (may be null) its share of that weight
+ *   kept     what is in P and in M
+ *   token    the first kept entry, by index, with which the sum over those so far exceeds u times the sum over all
+ *   prob     (may be null) its share of that sum
  * temperature <= 0 or NaN: the first of the order, prob 1; above 1e30 it is 1e30.  -inf and NaN logits are masked, +inf counts as
  * the largest finite number; a row with nothing left gets token -1, prob 0.  u below 0 or NaN is 0; at 1 and above the last kept
- * entry is drawn.  Sums are over whole numbers: a row gives the same token in any batch.  At most 4194304 logits a row.
+ * entry by index that has weight is drawn.  Sums are over whole numbers: a row gives the same token in any batch.  At most 4194304 logits a row.
  * No workspace. */
 int mx230_sample(mx230_handle *h, void *stream, int *token, float *prob, const void *logits, int dtype, int n_rows, int vocab,
                  long long row_stride, const float *u, float temperature, const float *temperatures, int top_k,

@@ -5,18 +5,21 @@
 //   top-k      K = the first k entries of that order
 //   top-p      P = the shortest prefix of K whose mass is at least p times K's
 //   min-p      M = the entries with w_i >= m, a prefix as well
-//   token      the first entry of the order whose running mass, its own included, exceeds u times the mass of P and M's intersection
+//   kept       what is in P and in M
+//   token      the first kept entry, by index, with which the sum over those so far exceeds u times the sum over all
 //
-// Sums are over whole numbers, so they do not depend on their order, and the same row gives the same token on any grid.  What has
-// to be found is always "the first entry of the order whose running count or mass exceeds t"; three of them at most, each
-// target known from the one before (the intersection of two prefixes has the smaller of their masses).
+// Sums are over whole numbers, so they do not depend on their order, and the same row gives the same token on any grid.  K and P end
+// with "the first entry of the order whose running count or mass exceeds t"; then what is kept is known, and the token is the
+// first one by index whose running mass exceeds t.
 //
-// The logits have to be read once, 4 or 2 bytes each; what bounds the kernel is instructions, about 85 a warp for 32 logits that are
-// weighed (64 rows of 128000 in fp32 with top-p 0.95: 51 us, 5 of them HBM's), and for a few rows latency (one row of 32000: 10 us).
-// A cluster of one to eight CTAs takes a row.  A histogram over 2048 equal intervals of max - l, as far as weights are not 0 (28.7 T), in
-// counts (top-k) or masses says which intervals hold the entries that are sought: all down to P's or K's end, if that is one list, or
-// the interval where P ends and those where the token then can be.  Their entries alone are collected, sorted and summed.  Where
-// that is more than a list, a histogram over the range of their (value, index) takes the interval's place, as often as it takes.
+// The logits have to be read once, 4 or 2 bytes each; what bounds the kernel is what a weight takes (64 rows of
+// 128000 in fp32 with top-p 0.95: 68 us, 5 of them HBM's), and for a few rows latency (one row of 32000: 10 us).
+// A cluster of one to eight CTAs takes a row, each a part of the vocabulary that follows the one before.  A histogram over 2048 equal
+// intervals of max - l, as far as weights are not 0 (28.7 T), in counts (top-k) or masses says in which interval K or P ends.  If all
+// down to there is one list, its entries are collected, sorted and summed, and what is kept of them is sorted again by index.  Else the
+// interval's entries are, and the last one that is kept goes to all CTAs.  (Where the interval is more than a list, a histogram over the
+// range of its (value, index) takes its place, as often as it takes.)  They add up what is kept by pieces of the row of 128 logits or
+// more, so the piece that holds the token is known, and is looked at again.  Without top-k and top-p that is all there is to do.
 // A weight takes fifteen fp64 instructions; rows with a small k take them for the entries of the list only.
 #include <cuda_fp16.h>
 #include <float.h>
@@ -66,13 +69,12 @@ struct SampleParams {
 
 // What the first CTA tells the others (whole words, so that it can be copied as such).
 struct Window {
-    int kind;                // entries of: 0: intervals b0 .. b1 of the histogram over max - l, and c0 .. c1; 1: lo .. hi as well
-    int b0, b1, c0, c1;
+    int kind;                // entries of: 0: intervals b0 .. b1 of the histogram over max - l; 1: and of lo .. hi as well
+    int b0, b1;
     int count;               // entries in it
     u64 lo, hi;
     u64 base_count, base_mass;   // of the entries in front of it
 };
-constexpr int W_EVERYTHING = SM_LIST + 1;   // count of the window that says: more than a list
 
 struct alignas(16) Shared {
     // this CTA's histogram: counts, masses in two words; what has no weight is counted behind them, by lanes
@@ -409,21 +411,17 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
     }
     T_ = fminf(T_, 1e30f);   // (28.7 T stays finite)
     if (k <= 0 || k >= P.vocab) k = 0;
+    const bool cut_p = p < 1.0f;
     const double log2e_t = 1.4426950408889634 / (double)T_, m64 = (double)m;
     // intervals over what has weight (2^-41 and more: 28.42 T) and what there is
     const float range = fminf(28.7f * T_, m - least);
     const float scale = range > 0.0f ? fminf((float)(SM_BINS - 1) / range, FLT_MAX) : 0.0f;
-    // M: w >= min_w, in doubt only close to the logit for which it is equal
-    const double min_w = min_p > 0.0f ? (double)fminf(min_p, 1.0f) : 0.0;
-    const bool has_min = min_w > 0.0;
-    const float m_at = min_w > 0.0 ? m + logf((float)min_w) * T_ : -FLT_MAX, m_slack = 1e-5f * (fabsf(m) + fabsf(m_at) + T_);
-    const float m_low = m_at - m_slack, m_high = m_at + m_slack;
 
     auto entry = [&](int i, float l) {   // (-0 is 0)
         return (u64)order_key(l + 0.0f) << P.idx_bits | (((1u << P.idx_bits) - 1) - (unsigned)(idx0 + i));
     };
     auto entry_logit = [&](u64 e) { return key_float((uint32_t)(e >> P.idx_bits)); };
-    bool with_mass = k == 0 || k > SM_LIST / 2;   // (a small k: only its entries' weights are asked for)
+    bool with_mass = cut_p && (k == 0 || k > SM_LIST / 2);   // (a small k: only its entries' weights are asked for)
     const bool with_count = k != 0;
     auto mass = [&](float l) { return mass_of((double)l - m64, log2e_t, P.power); };
     auto add_to = [&](unsigned b, u64 mass) {   // a 64-bit sum by two words
@@ -482,21 +480,19 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
         const Window w = S.w[wp];
         const bool exact = w.kind == 1;
         // logits of intervals b0 .. b1 lie between these, by more than the interval's own rounding
-        auto above = [&](int b) { return b == 0 ? INFINITY : m - ((float)b - 0.6f) / scale + 1e-6f * (fabsf(m) + (float)b / scale); };
-        auto below = [&](int b) { return m - ((float)b + 0.6f) / scale - 1e-6f * (fabsf(m) + (float)b / scale); };
         const bool flat = !(scale > 0.0f);
-        const float b_hi = flat ? INFINITY : above(w.b0), b_lo = flat ? -INFINITY : below(w.b1);
-        const float c_hi = flat ? INFINITY : above(w.c0), c_lo = flat ? -INFINITY : below(w.c1);
+        const float hi = flat || w.b0 == 0 ? INFINITY : m - ((float)w.b0 - 0.6f) / scale + 1e-6f * (fabsf(m) + (float)w.b0 / scale);
+        const float lo = flat ? -INFINITY : m - ((float)w.b1 + 0.6f) / scale - 1e-6f * (fabsf(m) + (float)w.b1 / scale);
         for_logits([&](int i, const float (&l)[4]) {
             bool in[4];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) in[v] = (l[v] >= b_lo & l[v] <= b_hi) | (l[v] >= c_lo & l[v] <= c_hi);
+            for (int v = 0; v < 4; ++v) in[v] = l[v] >= lo & l[v] <= hi;
             if (in[0] | in[1] | in[2] | in[3])
 #pragma unroll
                 for (int v = 0; v < 4; ++v)
                     if (in[v]) {
                         const float x = finite(l[v]), b = interval(x, m, scale) - SM_INTERVAL;
-                        if (!((b >= w.b0 && b <= w.b1) || (b >= w.c0 && b <= w.c1))) continue;
+                        if (!(b >= w.b0 && b <= w.b1)) continue;
                         if (exact) {
                             const u64 e = entry(i + v, x);
                             if (e < w.lo || e > w.hi) continue;
@@ -505,8 +501,14 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
                     }
         }, Look());
     };
+    // running masses of the n entries of S.all, of which `logit_of` gives the logit, into S.mine
+    auto running_masses = [&](int n, auto logit_of) {
+        for (int i = tid; i < n; i += SM_THREADS) S.mine[i] = mass(logit_of(S.all[i]));
+        __syncthreads();
+        running_sums<SM_LIST / SM_THREADS>(nullptr, S.mine, n, S);
+    };
     // the window's entries, sorted, and their running masses (first CTA: S.all, S.mine); at most SM_LIST
-    auto collect = [&]() {
+    auto collect = [&](bool masses) {
         if (tid == 0) S.n_mine = 0;
         __syncthreads();
         for_window([&](int i, float l) {
@@ -528,9 +530,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
         if (first_cta) {
             total = (int)min(S.n_all, (unsigned)SM_LIST);
             sort_down(S.all, S.mine, total);
-            for (int i = tid; i < total; i += SM_THREADS) S.mine[i] = mass(entry_logit(S.all[i]));
-            __syncthreads();
-            running_sums<SM_LIST / SM_THREADS>(nullptr, S.mine, total, S);
+            if (masses) running_masses(total, entry_logit);
         }
         return total;
     };
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
         Window next{};
         if (first_cta) {
             const int b = by_mass ? first_over(S.run_mass, SM_BINS, t, answer()) : first_over(S.run_cnt, SM_BINS, t, answer());
-            next.b0 = next.b1 = next.c0 = next.c1 = b;
+            next.b0 = next.b1 = b;
             if (b) next.base_count = S.run_cnt[b - 1], next.base_mass = S.run_mass[b - 1];
             next.count = (int)(S.run_cnt[b] - (unsigned)next.base_count);
         }
@@ -589,13 +589,10 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
             }
             tell(next);
         }
-        const int total = collect();
+        const int total = collect(cut_p);
         if (!first_cta) return 0;
         return by_mass ? first_over(S.mine, total, t - S.w[wp].base_mass, answer()) : (int)(t - S.w[wp].base_count);
     };
-    auto share = [&](double of, u64 total) { return (u64)fmin(of * (double)total, (double)total); };   // (cut off, not rounded)
-
-    u64 sum_min = 0;   // mass of M among this thread's logits
     auto histogram = [&](auto counts, auto masses) {
         // (byte address of an interval's sum from its float; what has no weight goes behind the intervals)
         const uint32_t at0 = mx::smem_u32(S.cnt) - 4u * __float_as_uint(SM_INTERVAL), none = mx::smem_u32(&S.cnt[SM_BINS + lane]);
@@ -625,110 +622,146 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
                     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p red.shared.add.u32 [%0], %1;\n\t}" ::"r"(at[v] + TO_HI), "r"(h)
                                  : "memory");
                 }
-                if (has_min)
-#pragma unroll
-                    for (int v = 0; v < 4; ++v)
-                        if (at[v] != none && l[v] >= m_low && (l[v] >= m_high || weight((double)l[v] - m64, log2e_t, P.power) >= min_w)) sum_min += ms[v];
             }
         }, Weigh());
     };
-    u64 z = 0, z_min = 0;   // first CTA: mass of K, then of what is kept; of M
-    for (bool again = false;; again = true) {
-        // ---- histogram over max - l ----
-        if (again) clear();
-        sum_min = 0;
-        if (!with_mass) histogram(std::true_type(), std::false_type());
-        else if (with_count) histogram(std::true_type(), std::true_type());
-        else histogram(std::false_type(), std::true_type());
-        if (with_mass && min_w > 0.0) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum_min += __shfl_xor_sync(0xFFFFFFFFu, sum_min, o);
-            if (lane == 0) S.scan[warp] = sum_min;
+    auto share = [&](u64 total) { return min((u64)((double)u * (double)total), total - 1); };   // u's part of it (cut off, not rounded)
+    // M: w >= min_w, in doubt only close to the logit for which it is equal
+    const double min_w = min_p > 0.0f ? (double)fminf(min_p, 1.0f) : 0.0;
+    auto in_m = [&](float l) { return weight((double)l - m64, log2e_t, P.power) >= min_w; };
+    auto done = [&](int token, u64 mass, u64 of) {
+        P.token[row] = token;
+        if (P.prob) P.prob[row] = (float)((double)mass / (double)of);
+    };
+
+    // ---- the last entry of K and P: it is known, with all in front of it, from a list; or as the least entry that is kept ----
+    u64 least_kept = 0;
+    if (k || cut_p) {
+        u64 z = 0;   // first CTA: mass of K
+        for (bool again = false;; again = true) {
+            if (again) clear();
+            if (!with_mass) histogram(std::true_type(), std::false_type());
+            else if (with_count) histogram(std::true_type(), std::true_type());
+            else histogram(std::false_type(), std::true_type());
+            merge(S.run_cnt, S.run_mass, with_count, with_mass, std::integral_constant<int, SM_BINS>());
+            Window next{};
+            if (first_cta) {
+                if (with_mass) z = S.run_mass[SM_BINS - 1];   // (k = 0)
+                next.b1 = k ? first_over(S.run_cnt, SM_BINS, (u64)min((unsigned)k, S.run_cnt[SM_BINS - 1]) - 1, answer())
+                            : first_over(S.run_mass, SM_BINS, (u64)ceil((double)p * (double)z) - 1, answer());
+                next.count = min((int)S.run_cnt[next.b1], SM_LIST + 1);
+            }
+            tell(next);
+            if (S.w[wp].count <= SM_LIST || with_mass || !cut_p) break;
+            with_mass = true;   // (many equal logits, or many close to the k-th)
+        }
+        if (S.w[wp].count <= SM_LIST) {   // all that can be kept is a list
+            int n = collect(cut_p);
+            if (!first_cta) return;
+            if (k) n = min(k, n);
+            if (cut_p) n = first_over(S.mine, n, (u64)ceil((double)p * (double)(k ? S.mine[n - 1] : z)) - 1, answer()) + 1;
+            if (min_w > 0.0) {
+                int in = 0;
+                for (int i = tid; i < SM_LIST; i += SM_THREADS) in += __syncthreads_count(i < n && in_m(entry_logit(S.all[i])));
+                n = in;
+            }
+            // what is kept, by index
+            for (int i = tid; i < n; i += SM_THREADS) {
+                const u64 e = S.all[i];
+                S.all[i] = (e & ((1ull << P.idx_bits) - 1)) << 32 | e >> P.idx_bits;
+            }
             __syncthreads();
-            if (tid == 0) {
-                for (int w = 1; w < SM_WARPS; ++w) sum_min += S.scan[w];
-                st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_b[rank]), 0), sum_min);
-            }
+            sort_down(S.all, S.mine, n);
+            running_masses(n, [&](u64 e) { return key_float((uint32_t)e); });
+            z = S.mine[n - 1];
+            const int at = first_over(S.mine, n, share(z), answer());
+            if (tid == 0) done((int)(((1u << P.idx_bits) - 1) - (unsigned)(S.all[at] >> 32)), S.mine[at] - (at ? S.mine[at - 1] : 0), z);
+            return;
         }
-        merge(S.run_cnt, S.run_mass, with_count, with_mass, std::integral_constant<int, SM_BINS>());
-        // ---- what is to be looked at: all that can be kept, if that is a list; else (k = 0) the interval where P ends and those where
-        // the token then can be, if they are; else more than that ----
-        Window next{};
-        if (first_cta) {
-            const unsigned there = S.run_cnt[SM_BINS - 1];
-            z = z_min = with_mass ? S.run_mass[SM_BINS - 1] : 0;   // (else known from the list)
-            int b = SM_BINS - 1;
-            if (k) b = first_over(S.run_cnt, SM_BINS, (u64)min((unsigned)k, there) - 1, answer());
-            else if (p < 1.0f) b = first_over(S.run_mass, SM_BINS, (u64)ceil((double)p * (double)z) - 1, answer());
-            if (with_mass && min_w > 0.0) {
-                z_min = 0;
-                for (int c = 0; c < C; ++c) z_min += S.slot_b[c];
-            }
-            next.b1 = next.c1 = b, next.count = (int)S.run_cnt[b];
-            if (next.count > SM_LIST && k == 0) {
-                // the kept mass lies between these, and u's share of it too
-                const u64 z0 = min(z_min, p < 1.0f ? (b ? S.run_mass[b - 1] : 0) : z), z1 = min(z_min, p < 1.0f ? S.run_mass[b] : z);
-                next.c0 = first_over(S.run_mass, SM_BINS, z0 ? min(share((double)u, z0), z0 - 1) : 0, answer());
-                next.c1 = first_over(S.run_mass, SM_BINS, min(share((double)u, z1), z1 - 1), answer());
-                if (p < 1.0f) {
-                    if (next.c1 >= b) next.c1 = b;
-                    next.b0 = next.b1 = b;
-                    if (next.c1 == b) next.b0 = next.c0;   // (next to each other: one range)
-                } else next.b0 = next.c0, next.b1 = next.c1;
-                const unsigned in_b = S.run_cnt[next.b1] - (next.b0 ? S.run_cnt[next.b0 - 1] : 0);
-                const unsigned in_c = S.run_cnt[next.c1] - (next.c0 ? S.run_cnt[next.c0 - 1] : 0);
-                next.count = (int)(next.c1 == next.b1 ? in_b : in_b + in_c);
-            }
-            if (next.count > SM_LIST) next.count = W_EVERYTHING;
-        }
-        tell(next);
-        if (S.w[wp].count <= SM_LIST || with_mass) break;
-        with_mass = true;   // (many equal logits, or many close to the k-th)
-    }
-    int at;
-    if (S.w[wp].count <= SM_LIST) {
-        const int total = collect();
-        if (!first_cta) return;
-        // the list's running masses are those of the whole order less what lies in front of its ranges: of c (or b, if it is one
-        // range), and between c and b
-        const Window w = S.w[wp];
-        const bool one = w.c1 == w.b1;
-        const u64 front = w.c0 ? S.run_mass[w.c0 - 1] : 0;
-        const u64 in_c = one ? 0 : S.run_mass[w.c1] - front, between = one ? 0 : S.run_mass[w.b0 - 1] - S.run_mass[w.c1];
-        if (k) z = S.mine[min(k, total) - 1];
-        u64 keep = z;
-        if (p < 1.0f) keep = front + between + S.mine[first_over(S.mine, total, (u64)ceil((double)p * (double)z) - 1 - front - between, answer())];
-        if (min_w > 0.0) {
-            if (with_mass) keep = min(keep, z_min);
-            else {   // the last entry of M among the list's; M beyond the list keeps all that P keeps
-                if (tid == 0) S.low = 0;
-                __syncthreads();
-                for (int i = tid; i < total; i += SM_THREADS)
-                    if (weight((double)entry_logit(S.all[i]) - m64, log2e_t, P.power) >= min_w) atomicMax(&S.low, S.mine[i]);
-                __syncthreads();
-                keep = min(keep, S.low);
-            }
-        }
-        z = keep;
-        const u64 t = min(share((double)u, z), z - 1) - front;
-        at = first_over(S.mine, total, one || t < in_c ? t : t - between, answer());   // (else behind c, in b)
-    } else {
         if (k) {
             const int i = search(first_cta ? (u64)min((unsigned)k, S.run_cnt[SM_BINS - 1]) - 1 : 0, false);
-            if (first_cta) z = S.w[wp].base_mass + S.mine[i];
+            if (first_cta) least_kept = S.all[i], z = cut_p ? S.w[wp].base_mass + S.mine[i] : 0;
         }
-        if (p < 1.0f) {
+        if (cut_p) {
             const int i = search(first_cta ? (u64)ceil((double)p * (double)z) - 1 : 0, true);
-            if (first_cta) z = S.w[wp].base_mass + S.mine[i];
+            if (first_cta) least_kept = S.all[i];
         }
-        if (first_cta) z = min(z, z_min);
-        at = search(first_cta ? min(share((double)u, z), z - 1) : 0, true);
-        if (!first_cta) return;
+        if (first_cta && tid < C) st_cluster(mx::cluster_map(mx::smem_u32(&S.low), tid), least_kept);
+        cluster_sync();
+        least_kept = S.low;
+        clear();
     }
-    if (tid == 0) {
-        const u64 e = S.all[at];
-        P.token[row] = (int)(((1u << P.idx_bits) - 1) - (unsigned)(e & ((1ull << P.idx_bits) - 1)));
-        if (P.prob) P.prob[row] = (float)((double)(S.mine[at] - (at ? S.mine[at - 1] : 0)) / (double)z);
+    // ---- masses of what is kept, by pieces of the row that follow one another (a CTA's share is one of them): where u's part of them
+    // is passed ----
+    const float m_at = min_w > 0.0 ? m + logf((float)min_w) * T_ : -FLT_MAX, m_slack = 1e-5f * (fabsf(m) + fabsf(m_at) + T_);
+    float cut = entry_logit(least_kept);
+    int cut_idx = (int)(((1u << P.idx_bits) - 1) - (unsigned)(least_kept & ((1ull << P.idx_bits) - 1)));
+    if (least_kept == 0) cut = fmaxf(least, m - 28.75f * T_), cut_idx = P.vocab;   // (what is below has no weight)
+    const float from = min_w > 0.0 ? fmaxf(cut, m_at - m_slack) : cut, sure = min_w > 0.0 ? m_at + m_slack : -FLT_MAX;
+    auto kept_mass = [&](int i, float raw) -> u64 {
+        if (!(raw >= from)) return 0;
+        const float l = finite(raw);
+        if ((l == cut && idx0 + i > cut_idx) || (l < sure && !in_m(l))) return 0;
+        return mass(l);
+    };
+    constexpr int UNIT = KEEP ? 128 : 32 * VE;   // logits that a warp takes at a time
+    int piece = KEEP || VE == 4 ? 7 : 8;         // of 2^piece logits
+    while ((n - 1) >> piece >= SM_BINS) ++piece;
+    const int n_pieces = ((n - 1) >> piece) + 1;
+    for (int i0 = warp * UNIT; i0 < n; i0 += SM_WARPS * UNIT) {   // (whole warps)
+        u64 sum = 0;
+        if constexpr (KEEP) {
+            const int i = i0 + 4 * lane;
+            if (i < n) {
+                const float4 l = *(const float4 *)(data + i);
+                sum = kept_mass(i, l.x) + kept_mass(i + 1, l.y) + kept_mass(i + 2, l.z) + kept_mass(i + 3, l.w);
+            }
+        } else {
+            const int i = i0 + VE * lane, at = idx0 + i;
+            if (i < n) {
+                const uint4 raw = at >= 0 && at + VE <= P.vocab ? *(const uint4 *)(src + at) : ragged_piece(src, at, P.vocab);
+                const T *e = (const T *)&raw;
+#pragma unroll
+                for (int c = 0; c < VE; ++c) sum += kept_mass(i + c, logit(e[c]));
+            }
+        }
+        if (!__any_sync(0xFFFFFFFFu, sum != 0)) continue;
+        // (at most eight masses a lane, 2^43: in two parts whose sums have 32 bits)
+        const unsigned a = __reduce_add_sync(0xFFFFFFFFu, (unsigned)sum & 0xFFFFFF), b = __reduce_add_sync(0xFFFFFFFFu, (unsigned)(sum >> 24));
+        if (lane == 0) add_to(i0 >> piece, ((u64)b << 24) + a);
+    }
+    __syncthreads();
+    for (int b = tid; b < n_pieces; b += SM_THREADS) S.run_mass[b] = (u64)S.hi[b] << 32 | S.lo[b];
+    __syncthreads();
+    running_sums<SM_BINS / SM_THREADS>(nullptr, S.run_mass, n_pieces, S);
+    const u64 own = S.run_mass[n_pieces - 1];
+    if (tid < C) st_cluster(mx::cluster_map(mx::smem_u32(&S.slot_b[rank]), tid), own);
+    cluster_sync();
+    u64 z = 0, before = 0;
+    for (int c = 0; c < C; ++c) {
+        if (c == rank) before = z;
+        z += S.slot_b[c];
+    }
+    u64 t = share(z);
+    if (t < before || t - before >= own) return;
+    t -= before;
+    const int b = first_over(S.run_mass, n_pieces, t, answer());
+    t -= b ? S.run_mass[b - 1] : 0;
+    const int end = min(n, (b + 1) << piece);
+    for (int i0 = b << piece; i0 < end; i0 += SM_THREADS) {
+        const int i = i0 + tid, at = idx0 + i;
+        u64 own_mass = 0;
+        if (i < end && at >= 0 && at < P.vocab) own_mass = kept_mass(i, KEEP ? data[i] : logit(src[at]));
+        S.mine[tid] = own_mass;
+        __syncthreads();
+        running_sums<1>(nullptr, S.mine, SM_THREADS, S);
+        const u64 all = S.mine[SM_THREADS - 1];
+        if (all > t) {
+            if (S.mine[tid] > t && S.mine[tid] - own_mass <= t) done(at, own_mass, z);
+            return;
+        }
+        t -= all;
+        __syncthreads();
     }
 }
 

@@ -106,9 +106,10 @@ class Scheduler:
 def sample(h: Handle, token, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, prob=None, stream=None):
     """The next token of each row of `logits` [n][vocab] (fp32, fp16 or bf16; the values of a row contiguous) into `token` int32 [n],
     from random numbers `u` fp32 [n] in [0, 1); its probability among what could be drawn into `prob` fp32 [n].  Each setting
-    is a number or a tensor [n] (fp32, top_k int32).  include/mx230_attn.h has the definition at mx230_sample: entries in falling
-    order, the first top_k of them, of those the shortest prefix with top_p of their weight, cut at min_p times the largest
-    weight; the token is where the running weight passes u.  -1 where a row is masked throughout."""
+    is a number or a tensor [n] (fp32, top_k int32).  include/mx230_attn.h has the definition at mx230_sample: of the entries in
+    falling order the first top_k, of those the shortest prefix with top_p of their weight, cut at min_p times the largest
+    weight; among what is kept, in the order of the vocabulary, the token is where the running weight passes u's share.  -1
+    where a row is masked throughout."""
     dev, dtype = h.device, _DTYPES.get(logits.dtype)
     require(logits.dim() == 2 and dtype is not None, lambda: f"sample: logits {tuple(logits.shape)} of {logits.dtype}")
     (n, vocab), (row, one) = logits.shape, logits.stride()
