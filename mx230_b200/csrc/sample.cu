@@ -174,7 +174,7 @@ __device__ __forceinline__ float finite(float l) {   // infinity is the largest 
 }
 
 // Interval of max - l, as the float 2^23 + interval: a difference, and a product and a sum rounded once, so it is monotone in l.
-// Masked logits get infinity or NaN: no interval is larger or smaller than NaN, so "it is below a bound" leaves both out.
+// (Masked logits are not among those that have one.)
 constexpr float SM_INTERVAL = 8388608.0f;
 __device__ __forceinline__ float interval(float l, float m, float scale) { return fmaf(m - l, scale, SM_INTERVAL); }
 
@@ -416,6 +416,10 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
     // intervals over what has weight (2^-41 and more: 28.42 T) and what there is
     const float range = fminf(28.7f * T_, m - least);
     const float scale = range > 0.0f ? fminf((float)(SM_BINS - 1) / range, FLT_MAX) : 0.0f;
+    // The least logit with an interval, 28.7 T below the largest or one step of the floats from there, where they are that far apart.
+    // (The intervals' number alone would not do: where T is subnormal, or nearly, they reach farther, and weights out of what mass_of takes.)
+    float lowest = fmaxf(least, m - 28.7f * T_);
+    if (interval(lowest, m, scale) >= SM_INTERVAL + SM_BINS) lowest = nextafterf(lowest, INFINITY);
 
     auto entry = [&](int i, float l) {   // (-0 is 0)
         return (u64)order_key(l + 0.0f) << P.idx_bits | (((1u << P.idx_bits) - 1) - (unsigned)(idx0 + i));
@@ -482,7 +486,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
         // logits of intervals b0 .. b1 lie between these, by more than the interval's own rounding
         const bool flat = !(scale > 0.0f);
         const float hi = flat || w.b0 == 0 ? INFINITY : m - ((float)w.b0 - 0.6f) / scale + 1e-6f * (fabsf(m) + (float)w.b0 / scale);
-        const float lo = flat ? -INFINITY : m - ((float)w.b1 + 0.6f) / scale - 1e-6f * (fabsf(m) + (float)w.b1 / scale);
+        const float lo = fmaxf(lowest, flat ? -INFINITY : m - ((float)w.b1 + 0.6f) / scale - 1e-6f * (fabsf(m) + (float)w.b1 / scale));
         for_logits([&](int i, const float (&l)[4]) {
             bool in[4];
 #pragma unroll
@@ -603,8 +607,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
                 l[v] = finite(raw[v]);
-                const float x = interval(l[v], m, scale);
-                at[v] = x < SM_INTERVAL + SM_BINS ? at0 + 4u * __float_as_uint(x) : none;
+                at[v] = l[v] >= lowest ? at0 + 4u * __float_as_uint(interval(l[v], m, scale)) : none;
                 if constexpr (decltype(counts)::value) asm volatile("red.shared.add.u32 [%0], 1;" ::"r"(at[v]) : "memory");
             }
             if constexpr (decltype(masses)::value) {
@@ -693,10 +696,10 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleParam
     }
     // ---- masses of what is kept, by pieces of the row that follow one another (a CTA's share is one of them): where u's part of them
     // is passed ----
-    const float m_at = min_w > 0.0 ? m + logf((float)min_w) * T_ : -FLT_MAX, m_slack = 1e-5f * (fabsf(m) + fabsf(m_at) + T_);
+    const float m_at = min_w > 0.0 ? m + logf((float)min_w) * T_ : -FLT_MAX, m_slack = 1e-5f * (fabsf(m) + fabsf(m_at) + T_) + FLT_MIN;
     float cut = entry_logit(least_kept);
     int cut_idx = (int)(((1u << P.idx_bits) - 1) - (unsigned)(least_kept & ((1ull << P.idx_bits) - 1)));
-    if (least_kept == 0) cut = fmaxf(least, m - 28.75f * T_), cut_idx = P.vocab;   // (what is below has no weight)
+    if (least_kept == 0) cut = lowest, cut_idx = P.vocab;   // (what is below has no weight)
     const float from = min_w > 0.0 ? fmaxf(cut, m_at - m_slack) : cut, sure = min_w > 0.0 ? m_at + m_slack : -FLT_MAX;
     auto kept_mass = [&](int i, float raw) -> u64 {
         if (!(raw >= from)) return 0;

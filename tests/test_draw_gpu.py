@@ -171,6 +171,23 @@ def test_masked_rows_infinities_and_zeros(handle):
     check(handle, torch.tensor([[-inf, 6e4, inf, -6e4, 0.0]]).half(), [0.6])
 
 
+@pytest.mark.parametrize("t", [1e-45, 1e-44, 1e-42, 1e-40, 3e-39, 8e-39, 1.2e-38, 1e-37, 1e-36, 1e-30])
+@pytest.mark.parametrize("scale", [1.0, 20.0, 1000.0, 1e5])
+def test_the_smallest_temperatures(handle, t, scale):
+    """Logits as close to each other as such a temperature tells apart, at 0 and where floats are farther apart, and others far below."""
+    t = float(np.float32(t))
+    g = np.random.default_rng(int(scale))
+    x = (g.random((6, 3001)) * -t * scale).astype(np.float32)
+    x[:, 0], x[:, 1], x[:, 2] = 0.0, -1e-37, -2.0
+    x[1] += np.float32(3e-38)
+    x[2] += np.float32(1e-33)
+    x[3, 1700:] = -math.inf
+    x[4] -= np.float32(1e-37)
+    x[5] *= 1e30
+    for s in (dict(), dict(p=0.9), dict(k=2), dict(k=1500), dict(k=1500, p=0.5), dict(m=0.5), dict(p=0.9, m=0.01)):
+        check(handle, torch.from_numpy(x), [0.0, 0.3, 0.5, 0.7, 0.9, 0.99], t=t, **s, what=s)
+
+
 def test_random_numbers_at_and_outside_the_ends(handle):
     u = [0.0, -1.0, math.nan, 1.0, 2.0, math.inf, -math.inf, 1 - 2.0 ** -24]
     for vocab in (3000, 40000):
