@@ -4,23 +4,21 @@
 // Bounded by HBM on the weights: half a byte each, read once, and 4 bytes of scale and zero point per group.  At that rate an SM
 // takes 46 weights a cycle, so a weight may cost about two instructions of a lane; multiply-adds on CUDA cores, with the
 // conversion from 4 bits in front, would take more for a single row and that many times more for several.  Hence warp-level
-// tensor-core tiles (m16n8k16) with the weights as A: 16 outputs x 16 inputs.  Four bits at places 4 to 7 of an fp16 are the number
-// q 2^-20 (a subnormal, which the tensor cores take as it is), so a pair of weights costs an "and" and three quarters of a shift.  (At
-// places 0 to 3 they are q 2^-24, one shift less a pair, but the products of a step are added with the digits that the largest possible
-// number of a subnormal's exponent leaves, ten bits above q: 1.3e-6 of the result over 4096 inputs, 0.2e-6 so.)  The rows are the eight
-// columns of B, two columns a row:
+// tensor-core tiles (m16n8k16) with the weights as A: 16 outputs x 16 inputs.  Four bits at places 0 to 3 or 4 to 7 of an fp16 are the
+// number q 2^-24 or q 2^-20 (a subnormal), so a pair of weights costs an "and", a quarter of a shift and one rounded-once multiply-add
+// that makes it (q - z) 2^-10, exactly: a zero point so has no rounding of its own, and what a weight of 0 meets does not count
+// however large it is.  (Sums of x q and of x apart save the multiply-add, but what is left of their difference goes by
+// sum |x| (q + z): with one x of 10^4 among 4096 whose own weight is 0, 9e-5 of the result.)  The rows are the eight columns of B, two
+// columns a row:
 //   x 2^e = hi + lo, both fp16, e such that the largest of the 64 values of a tile lies in [2^14, 2^15):
 // |x 2^e - hi - lo| <= 2^-24 |x 2^e|, as exact as x itself (but for values 2^-17 times the tile's largest and less, which keep an
 // absolute error of 2^-39 of that).  Products are then exact in fp32; sums are fp32, per tile of 64 inputs (32, if groups are of
-// 32).  The zero point meets the sum of the tile's x: the row's total gets s 2^(20 - e) (sum x q - z sum x), whose error goes by
-// sum |x| (q + z) instead of sum |x (q - z)|, about four times that, and saves the subtraction per weight (161 instructions a
-// warp and tile with it, of which 36 for the conversion; about 80 without: of 4096 x 14336, one row, 11.5 us are left, 69 of 4096 x 128000
-// for four, where HBM would need 4.7 and 42).
+// 32).  The row's total gets s 2^(10 - e) times the tile's sum.
 //
 // Layout, made once by mx230_pack_int4: tiles of 16 outputs x 64 inputs, 512 bytes, of which lane (g = lane / 4, j = lane % 4) has 16:
 // words [row g: inputs 8j .. 8j+7][row g: inputs 32 + 8j ..][row g + 8: 8j ..][row g + 8: 32 + 8j ..], input 2p of eight at bits
 // 4p, input 2p + 1 at bits 16 + 4p.  (Which input a k index of the MMA stands for is free, as long as A and B agree.)  Tiles of an
-// output row follow one another along the inputs; behind all tiles, per (16 outputs, group), 16 words (s, z) of fp16.
+// output row follow one another along the inputs; behind all tiles, per (16 outputs, group), 16 words (s, -z 2^-10) of fp16.
 //
 // Weights come by bulk copies, a lane's for a CTA of sixteen warps, into a ring of stages (some output tiles, up to 32 tiles of their
 // inputs each: 16 KB in a row and their (s, z)).  Loads to registers, two to four tiles ahead, kept too few bytes on their way with
@@ -64,7 +62,7 @@ struct Int4Params {
     long long x_stride, y_stride, add_stride;
 };
 
-// (s, z) and codes of one output tile and input tile; padding: s = 0
+// (s, -z 2^-10) and codes of one output tile and input tile; padding: s = 0
 __global__ void pack_int4_kernel(uint4 *codes_out, uint32_t *sz_out, const uint8_t *codes, const __half *scales, const uint8_t *zeros,
                                  int n_in, int n_out, int group, int n_tiles, int k_tiles, int groups) {
     const long long n_codes = (long long)n_tiles * k_tiles * 32, n_sz = (long long)n_tiles * groups * 16;
@@ -90,9 +88,9 @@ __global__ void pack_int4_kernel(uint4 *codes_out, uint32_t *sz_out, const uint8
             __half sc = __float2half(0.0f), z = __float2half(8.0f);
             if (o < n_out) {
                 sc = scales[(size_t)gr * n_out + o];
-                if (zeros) z = __float2half((float)zeros[(size_t)gr * n_out + o]);
+                if (zeros) z = __float2half((float)zeros[(size_t)gr * n_out + o]);   // (0 to 255: exact, and so is -z 2^-10)
             }
-            sz_out[s] = (uint32_t)__half_as_ushort(sc) | (uint32_t)__half_as_ushort(z) << 16;
+            sz_out[s] = (uint32_t)__half_as_ushort(sc) | (uint32_t)__half_as_ushort(__float2half(-0x1p-10f * __half2float(z))) << 16;
         }
     }
 }
@@ -100,10 +98,12 @@ __global__ void pack_int4_kernel(uint4 *codes_out, uint32_t *sz_out, const uint8
 __device__ __forceinline__ uint32_t h2_u(__half2 v) { return *(uint32_t *)&v; }
 __device__ __forceinline__ __half2 u_h2(uint32_t v) { return *(__half2 *)&v; }
 
-// eight codes -> four pairs (inputs 2p, 2p + 1) of q 2^-20
-__device__ __forceinline__ void pairs8(uint32_t w, uint32_t (&a)[4]) {
-    constexpr uint32_t PLACE = 0x00F000F0u;
-    a[0] = (w << 4) & PLACE, a[1] = w & PLACE, a[2] = (w >> 4) & PLACE, a[3] = (w >> 8) & PLACE;
+// eight codes -> four pairs (inputs 2p, 2p + 1) of (q - z) 2^-10; nz: -z 2^-10, twice
+__device__ __forceinline__ void pairs8(uint32_t w, __half2 nz, uint32_t (&a)[4]) {
+    const __half2 low = __half2half2(__ushort_as_half(0x7400)), high = __half2half2(__ushort_as_half(0x6400));   // 2^14, 2^10
+    const uint32_t v = w >> 8;
+    a[0] = h2_u(__hfma2(u_h2(w & 0x000F000Fu), low, nz)), a[1] = h2_u(__hfma2(u_h2(w & 0x00F000F0u), high, nz));
+    a[2] = h2_u(__hfma2(u_h2(v & 0x000F000Fu), low, nz)), a[3] = h2_u(__hfma2(u_h2(v & 0x00F000F0u), high, nz));
 }
 
 // c = a b + c, or a b
@@ -133,8 +133,8 @@ __device__ __forceinline__ float tree_sum(const float *p, int n, int step) {
 
 // NT: column tiles of four rows.  T: output tiles of a warp.  G32: groups of 32 inputs (else a multiple of 64).
 // Shared memory: ring [stages][T][stage_k x 512 of codes, stage_k x 64 (groups of 32: 128) of (s, z)]; sums [2][16 warps][T * NT * 64];
-// in clusters, this CTA's share of everybody's sums [2][C][T * NT * 64 / C]; per (tile, row) {2^-e, 2^(e - 20) sum x, or that
-// of either half, 2^-e of the second half}; 32 bytes of zeros; rows [k_cta][NT][lanes][8 words].
+// in clusters, this CTA's share of everybody's sums [2][C][T * NT * 64 / C]; per (tile, row) 2^-e of either
+// half; 32 bytes of zeros; rows [k_cta][NT][lanes][8 words].
 template <int NT, int T, bool G32>
 struct Int4Form {
     static constexpr int SUMS = T * NT * 64;                // floats of a warp
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
     const int stage_bytes = T * P.stage_k * S::TILE;
     float *sums = (float *)(smem + P.stages * stage_bytes); // [2][16][SUMS]
     float *parts = sums + 2 * W4_WARPS * S::SUMS;           // [2][C][share]
-    float4 *xrow = (float4 *)(parts + (C > 1 ? 2 * S::SUMS : 0));   // [k_cta][NT * 4]
+    float2 *xrow = (float2 *)(parts + (C > 1 ? 2 * S::SUMS : 0));   // [k_cta][NT * 4]
     uint4 *zeros = (uint4 *)(xrow + P.k_cta * NT * 4);      // 32 bytes
     uint4 *xf = zeros + 2;                                  // [k_cta][NT][x_lanes][2]
     // this CTA's inputs
@@ -260,17 +260,10 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
                 up = 1.0f, down = there & 1 ? INFINITY : 1.0f;
                 if (G32) down2 = there & 2 ? INFINITY : 1.0f;
             }
-            float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] *= up, sum[e >> 3] += v[e];
-            if (!G32) sum[0] += sum[1];
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                sum[0] += __shfl_xor_sync(0xFFFFFFFFu, sum[0], o);
-                if (G32) sum[1] += __shfl_xor_sync(0xFFFFFFFFu, sum[1], o);
-            }
+            for (int e = 0; e < 16; ++e) v[e] *= up;
             if (i0 + lane >= n_x) continue;
-            if (jj == 0) xrow[q * (NT * 4) + r] = make_float4(down, sum[0] * 0x1p-20f, sum[1] * 0x1p-20f, down2);
+            if (jj == 0) xrow[q * (NT * 4) + r] = make_float2(down, down2);
             uint32_t hi[8], lo[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -298,7 +291,7 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
 #pragma unroll
             for (int n = 0; n < NT; ++n) total[t][n][0] = total[t][n][1] = 0.0f;
         const uint4 *xp = has_x ? xf + ((size_t)warp * NT * x_lanes + lane) * 2 : zeros;
-        const float4 *rp = xrow + warp * (NT * 4) + (NT == 1 ? min(j, rt - 1) : j);   // the row whose sums this lane gets
+        const float2 *rp = xrow + warp * (NT * 4) + (NT == 1 ? min(j, rt - 1) : j);   // the row that this lane has
         for (int k = k0; k < k1; k += P.stage_k) {
             const uint32_t bar = mx::smem_u32(&full[stage]);
             if (!mx::mbar_wait(bar, parity, &aborted, P.status)) {
@@ -313,7 +306,7 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
                 const unsigned char *at = base + (kt - k) * 512;
                 const uint32_t *sz = (const uint32_t *)(base + P.stage_k * 512) + (sz_group(kt) - g_first) * 16 + g;
                 uint4 b[NT][2];
-                float4 xr[NT];
+                float2 xr[NT];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     b[n][0] = xp[n * x_n], b[n][1] = xp[n * x_n + 1];
@@ -324,29 +317,33 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
                 for (int t = 0; t < T; ++t) {
                     const uint4 w = *(const uint4 *)(at + t * tile_bytes + lane * 16);
                     float acc[NT][4];
+                    float s0, s1;   // scales of the lane's two outputs
+                    __half2 z0, z1;
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf) {
+                        if (G32 || hf == 0) {
+                            // (a second group of 32 that is not there belongs to inputs that are not there either: s = z = 0)
+                            const bool there = !G32 || hf == 0 || 2 * kt + 1 < P.groups;
+                            const uint32_t *z = sz + t * (tile_bytes / 4) + (G32 ? hf * 16 : 0);
+                            const __half2 w0 = u_h2(there ? z[0] : 0), w1 = u_h2(there ? z[8] : 0);
+                            s0 = __low2float(w0), s1 = __low2float(w1), z0 = __high2half2(w0), z1 = __high2half2(w1);
+                        }
                         uint32_t a0[4], a1[4];
-                        pairs8(hf ? w.y : w.x, a0);
-                        pairs8(hf ? w.w : w.z, a1);
+                        pairs8(hf ? w.y : w.x, z0, a0);
+                        pairs8(hf ? w.w : w.z, z1, a1);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             if (G32 || hf == 0) mma_f16_first(acc[n], a0[0], a1[0], a0[1], a1[1], b[n][hf].x, b[n][hf].y);
                             else mma_f16(acc[n], a0[0], a1[0], a0[1], a1[1], b[n][hf].x, b[n][hf].y);
                             mma_f16(acc[n], a0[2], a1[2], a0[3], a1[3], b[n][hf].z, b[n][hf].w);
                         }
-                        if (G32 || hf == 1) {
-                            // (a second group of 32 that is not there belongs to inputs that are not there either: s = z = 0)
-                            const bool there = !G32 || hf == 0 || 2 * kt + 1 < P.groups;
-                            const uint32_t *z = sz + t * (tile_bytes / 4) + (G32 ? hf * 16 : 0);
-                            const float2 s0 = __half22float2(u_h2(there ? z[0] : 0)), s1 = __half22float2(u_h2(there ? z[8] : 0));
+                        if (G32 || hf == 1)
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
-                                const float xs = G32 && hf ? xr[n].z : xr[n].y, back = G32 && hf ? xr[n].w : xr[n].x;
-                                total[t][n][0] = fmaf(s0.x, fmaf(-s0.y, xs, acc[n][0] + acc[n][1]) * back, total[t][n][0]);
-                                total[t][n][1] = fmaf(s1.x, fmaf(-s1.y, xs, acc[n][2] + acc[n][3]) * back, total[t][n][1]);
+                                const float back = G32 && hf ? xr[n].y : xr[n].x;
+                                total[t][n][0] = fmaf(s0, (acc[n][0] + acc[n][1]) * back, total[t][n][0]);
+                                total[t][n][1] = fmaf(s1, (acc[n][2] + acc[n][3]) * back, total[t][n][1]);
                             }
-                        }
                     }
                 }
             }
@@ -378,7 +375,7 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
             float v = C > 1 ? tree_sum(theirs + i - rank * share, C, share) : tree_sum(mine + i, KW, S::SUMS);
             const int o = (grp * T + t) * W4_N + (l >> 2) + 8 * hf, r = n * 4 + (l & 3);
             if (o < P.n_out && r < rows) {
-                v *= 0x1p20f;   // (sums of q 2^-20)
+                v *= 0x1p10f;   // (sums of (q - z) 2^-10)
                 float out = P.bias ? v + P.bias[o] : v;
                 if (P.add) out = P.add[(long long)(row0 + r) * P.add_stride + o] + out;
                 P.y[(long long)(row0 + r) * P.y_stride + o] = out;
@@ -504,7 +501,7 @@ extern "C" int mx230_gemv_int4(mx230_handle *h, void *stream, float *y, const fl
     while (P.ctas_k < W4_CLUSTER && (P.k_tiles > W4_K_CTA * P.ctas_k || (P.k_tiles >= 64 * P.ctas_k && (long long)P.n_tiles * P.ctas_k < h->sm_count))) P.ctas_k *= 2;
     P.k_cta = (P.k_tiles + P.ctas_k - 1) / P.ctas_k;
     // Rows of a pass: eight, or four where eight do not fit.
-    const int nt = n_rows <= 4 || P.k_cta > W4_K_CTA ? 1 : 2, x_tile = nt * (32 * (nt == 1 ? 8 * (n_rows < 4 ? n_rows : 4) : 32) + 64);
+    const int nt = n_rows <= 4 || P.k_cta > W4_K_CTA ? 1 : 2, x_tile = nt * (32 * (nt == 1 ? 8 * (n_rows < 4 ? n_rows : 4) : 32) + 32);
     mx230_device_guard guard(h->device);
     int held;
     rc = clusters_held(h, P.ctas_k, &held);

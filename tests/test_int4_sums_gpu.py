@@ -1,0 +1,53 @@
+"""Products with 4-bit weights where sums could lose what a 64-bit sum does not: inputs that are far larger than the others.
+
+Tolerance, against M = sum |x| |w|.  Weights are exact, x is off by 2^-23 |x| or by 2^-39 of the largest of its 64.  The 16 products of a
+step are added by the tensor core, taken as 17 truncations of 2^-24 M (what it keeps is not documented): 2^-19 M for all steps with
+the first term.  Scale and addition round: 2^-22 M a tile, for at most the tiles of a slice, and seven pairwise sums.
+"""
+import pytest
+import torch
+
+from mx230_b200 import llm_attention as la
+
+pytestmark = pytest.mark.gpu
+
+
+def weights(n_in, n_out, group, zeros, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    groups = -(-n_in // group)
+    codes = torch.randint(0, 16, (n_in, n_out), device="cuda", generator=g, dtype=torch.uint8)
+    scales = ((0.5 + torch.rand(groups, n_out, device="cuda", generator=g)) * 0.01).half()
+    z = torch.randint(0, 16, (groups, n_out), device="cuda", generator=g, dtype=torch.uint8) if zeros else torch.full((groups, n_out), 8, device="cuda", dtype=torch.uint8)
+    return codes, scales, z
+
+
+def dense(codes, scales, z, group):
+    at = torch.arange(codes.shape[0], device="cuda") // group
+    return (codes.double() - z.double()[at]) * scales.double()[at]
+
+
+def limit(x, w):
+    x, w, n_in = x.double().abs(), w.abs(), w.shape[0]
+    tiles = -(-n_in // 64)
+    out = x @ w * (2.0 ** -19 + (tiles + 8) * 2.0 ** -22) + 1e-30
+    for t in range(0, n_in, 64):
+        out = out + x[:, t:t + 64].amax(1, keepdim=True) * w[t:t + 64].sum(0) * 2.0 ** -39
+    return out
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("n_in,n_out,rows", [(500, 96, 1), (500, 5000, 2), (500, 20000, 1), (900, 3000, 4), (4096, 500, 3), (900, 700, 8), (500, 9000, 6)])
+def test_what_has_weight_zero_does_not_count(handle, n_in, n_out, rows, group, zeros):
+    """A few inputs a million times as large as the others, with codes that are their zero points."""
+    codes, scales, z = weights(n_in, n_out, group, zeros, n_in + rows)
+    x = torch.randn(rows, n_in, device="cuda", generator=torch.Generator(device="cuda").manual_seed(rows))
+    for k in (3, 70, n_in // 2, n_in - 1):
+        codes[k] = z[k // group]
+        x[:, k] *= 1e6
+    w = la.pack_int4(handle, codes, scales, z if zeros else None, group=group)
+    d = dense(codes, scales, z, group)
+    y = torch.empty(rows, n_out, device="cuda")
+    la.gemv_int4(handle, y, x, w)
+    err, lim = (y.double() - x.double() @ d).abs(), limit(x, d)
+    assert (err <= lim).all(), float((err / lim).max())
