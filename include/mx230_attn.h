@@ -532,7 +532,7 @@ int mx230_gemv_int8(mx230_handle *h, void *stream, float *y, const float *x, con
  * low four bits of a byte), fp16 scales and zeros [ceil(n_in / group)][n_out] (zeros null: 8); group 32 or a multiple of 64.
  * x goes in as two fp16 parts relative to the largest of 64 (off by half an ulp of fp32, or 2^-39 of that largest one), codes less
  * zero points (0 to 255) as they are; sums are fp32.
- * A row with infinite x has infinite or NaN y, of the right sign unless several meet in 64 inputs (32 in groups of 32).
+ * A row with infinite x has the infinite or NaN y that the formula gives.
  * No workspace. */
 size_t mx230_int4_bytes(int n_in, int n_out, int group);
 int mx230_pack_int4(mx230_handle *h, void *stream, void *packed, const uint8_t *codes, const void *scales_fp16,

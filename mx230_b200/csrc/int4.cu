@@ -13,7 +13,8 @@
 //   x 2^e = hi + lo, both fp16, e such that the largest of the 64 values of a tile lies in [2^14, 2^15):
 // |x 2^e - hi - lo| <= 2^-24 |x 2^e|, as exact as x itself (but for values 2^-17 times the tile's largest and less, which keep an
 // absolute error of 2^-39 of that).  Products are then exact in fp32; sums are fp32, per tile of 64 inputs (32, if groups are of
-// 32).  The row's total gets s 2^(10 - e) times the tile's sum.
+// 32).  The row's total gets s 2^(10 - e) times the tile's sum.  Infinite x are
+// infinite in hi and 0 in lo, so sums are infinite or NaN as those of x itself.
 //
 // Layout, made once by mx230_pack_int4: tiles of 16 outputs x 64 inputs, 512 bytes, of which lane (g = lane / 4, j = lane % 4) has 16:
 // words [row g: inputs 8j .. 8j+7][row g: inputs 32 + 8j ..][row g + 8: 8j ..][row g + 8: 32 + 8j ..], input 2p of eight at bits
@@ -133,8 +134,8 @@ __device__ __forceinline__ float tree_sum(const float *p, int n, int step) {
 
 // NT: column tiles of four rows.  T: output tiles of a warp.  G32: groups of 32 inputs (else a multiple of 64).
 // Shared memory: ring [stages][T][stage_k x 512 of codes, stage_k x 64 (groups of 32: 128) of (s, z)]; sums [2][16 warps][T * NT * 64];
-// in clusters, this CTA's share of everybody's sums [2][C][T * NT * 64 / C]; per (tile, row) 2^-e of either
-// half; 32 bytes of zeros; rows [k_cta][NT][lanes][8 words].
+// in clusters, this CTA's share of everybody's sums [2][C][T * NT * 64 / C]; per (tile, row) 2^-e; 32
+// bytes of zeros; rows [k_cta][NT][lanes][8 words].
 template <int NT, int T, bool G32>
 struct Int4Form {
     static constexpr int SUMS = T * NT * 64;                // floats of a warp
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
     const int stage_bytes = T * P.stage_k * S::TILE;
     float *sums = (float *)(smem + P.stages * stage_bytes); // [2][16][SUMS]
     float *parts = sums + 2 * W4_WARPS * S::SUMS;           // [2][C][share]
-    float2 *xrow = (float2 *)(parts + (C > 1 ? 2 * S::SUMS : 0));   // [k_cta][NT * 4]
+    float *xrow = parts + (C > 1 ? 2 * S::SUMS : 0);        // [k_cta][NT * 4]
     uint4 *zeros = (uint4 *)(xrow + P.k_cta * NT * 4);      // 32 bytes
     uint4 *xf = zeros + 2;                                  // [k_cta][NT][x_lanes][2]
     // this CTA's inputs
@@ -243,34 +244,30 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
             for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(v[e]));
 #pragma unroll
             for (int o = 1; o < 4; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+            const bool infinite = amax == INFINITY;
+            if (infinite) {   // the largest finite one, of the row's four lanes, which are all here; infinite ones go in as they are
+                amax = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) amax = fmaxf(amax, isinf(v[e]) ? 0.0f : fabsf(v[e]));
+                amax = fmaxf(amax, __shfl_xor_sync(0xFu << (lane & 28), amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xFu << (lane & 28), amax, 2));
+            }
             // e = 14 - exponent of amax; 2^e and 2^-e by their bits
             const int eb = max((int)(__float_as_uint(amax) >> 23), 15);
-            float up = __uint_as_float((uint32_t)(268 - eb) << 23), down = __uint_as_float((uint32_t)(eb - 14) << 23), down2 = G32 ? down : 0.0f;
-            if (amax == INFINITY) {   // infinite values alone count: as 1, and the sum of those with their scale times infinity
-                unsigned there = G32 ? 0 : 1;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    if (G32 && isinf(v[e])) there |= 1u << (e >> 3);
-                    v[e] = isinf(v[e]) ? copysignf(1.0f, v[e]) : v[e] == v[e] ? 0.0f : v[e];
-                }
-                if (G32) {   // (of the row's four lanes, which are all here)
-                    there |= __shfl_xor_sync(0xFu << (lane & 28), there, 1);
-                    there |= __shfl_xor_sync(0xFu << (lane & 28), there, 2);
-                }
-                up = 1.0f, down = there & 1 ? INFINITY : 1.0f;
-                if (G32) down2 = there & 2 ? INFINITY : 1.0f;
-            }
+            const float up = __uint_as_float((uint32_t)(268 - eb) << 23), down = __uint_as_float((uint32_t)(eb - 14) << 23);
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[e] *= up;
             if (i0 + lane >= n_x) continue;
-            if (jj == 0) xrow[q * (NT * 4) + r] = make_float2(down, down2);
+            if (jj == 0) xrow[q * (NT * 4) + r] = down;
             uint32_t hi[8], lo[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float a = v[2 * e], b = v[2 * e + 1];
                 const __half2 h = __floats2half2_rn(a, b);
                 const float2 back = __half22float2(h);
-                hi[e] = h2_u(h), lo[e] = h2_u(__floats2half2_rn(a - back.x, b - back.y));
+                float low_a = a - back.x, low_b = b - back.y;
+                if (infinite) low_a = isinf(a) ? 0.0f : low_a, low_b = isinf(b) ? 0.0f : low_b;
+                hi[e] = h2_u(h), lo[e] = h2_u(__floats2half2_rn(low_a, low_b));
             }
             // lanes of columns 2 (r % 4) and 2 (r % 4) + 1; pairs 0 .. 3 of each half of the tile: MMA steps 2 hf, 2 hf + 1
             uint4 *dst = xf + ((size_t)(q * NT + (r >> 2)) * x_lanes + (r & 3) * 8 + jj) * 2;
@@ -291,7 +288,7 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
 #pragma unroll
             for (int n = 0; n < NT; ++n) total[t][n][0] = total[t][n][1] = 0.0f;
         const uint4 *xp = has_x ? xf + ((size_t)warp * NT * x_lanes + lane) * 2 : zeros;
-        const float2 *rp = xrow + warp * (NT * 4) + (NT == 1 ? min(j, rt - 1) : j);   // the row that this lane has
+        const float *rp = xrow + warp * (NT * 4) + (NT == 1 ? min(j, rt - 1) : j);   // the row that this lane has
         for (int k = k0; k < k1; k += P.stage_k) {
             const uint32_t bar = mx::smem_u32(&full[stage]);
             if (!mx::mbar_wait(bar, parity, &aborted, P.status)) {
@@ -306,11 +303,11 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
                 const unsigned char *at = base + (kt - k) * 512;
                 const uint32_t *sz = (const uint32_t *)(base + P.stage_k * 512) + (sz_group(kt) - g_first) * 16 + g;
                 uint4 b[NT][2];
-                float2 xr[NT];
+                float back[NT];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     b[n][0] = xp[n * x_n], b[n][1] = xp[n * x_n + 1];
-                    xr[n] = rp[n * 4];
+                    back[n] = rp[n * 4];
                 }
                 xp += x_step, rp += KW * NT * 4;
 #pragma unroll
@@ -340,9 +337,8 @@ __global__ void __launch_bounds__(W4_THREADS + W4_PRODUCER, 1) gemv_int4_kernel(
                         if (G32 || hf == 1)
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
-                                const float back = G32 && hf ? xr[n].y : xr[n].x;
-                                total[t][n][0] = fmaf(s0, (acc[n][0] + acc[n][1]) * back, total[t][n][0]);
-                                total[t][n][1] = fmaf(s1, (acc[n][2] + acc[n][3]) * back, total[t][n][1]);
+                                total[t][n][0] = fmaf(s0, (acc[n][0] + acc[n][1]) * back[n], total[t][n][0]);
+                                total[t][n][1] = fmaf(s1, (acc[n][2] + acc[n][3]) * back[n], total[t][n][1]);
                             }
                     }
                 }
@@ -501,7 +497,7 @@ extern "C" int mx230_gemv_int4(mx230_handle *h, void *stream, float *y, const fl
     while (P.ctas_k < W4_CLUSTER && (P.k_tiles > W4_K_CTA * P.ctas_k || (P.k_tiles >= 64 * P.ctas_k && (long long)P.n_tiles * P.ctas_k < h->sm_count))) P.ctas_k *= 2;
     P.k_cta = (P.k_tiles + P.ctas_k - 1) / P.ctas_k;
     // Rows of a pass: eight, or four where eight do not fit.
-    const int nt = n_rows <= 4 || P.k_cta > W4_K_CTA ? 1 : 2, x_tile = nt * (32 * (nt == 1 ? 8 * (n_rows < 4 ? n_rows : 4) : 32) + 32);
+    const int nt = n_rows <= 4 || P.k_cta > W4_K_CTA ? 1 : 2, x_tile = nt * (32 * (nt == 1 ? 8 * (n_rows < 4 ? n_rows : 4) : 32) + 16);
     mx230_device_guard guard(h->device);
     int held;
     rc = clusters_held(h, P.ctas_k, &held);

@@ -1,9 +1,11 @@
-"""Products with 4-bit weights where sums could lose what a 64-bit sum does not: inputs that are far larger than the others.
+"""Products with 4-bit weights where sums could lose what a 64-bit sum does not: inputs that are far larger than the others, or infinite.
 
 Tolerance, against M = sum |x| |w|.  Weights are exact, x is off by 2^-23 |x| or by 2^-39 of the largest of its 64.  The 16 products of a
 step are added by the tensor core, taken as 17 truncations of 2^-24 M (what it keeps is not documented): 2^-19 M for all steps with
 the first term.  Scale and addition round: 2^-22 M a tile, for at most the tiles of a slice, and seven pairwise sums.
 """
+import math
+
 import pytest
 import torch
 
@@ -51,3 +53,23 @@ def test_what_has_weight_zero_does_not_count(handle, n_in, n_out, rows, group, z
     la.gemv_int4(handle, y, x, w)
     err, lim = (y.double() - x.double() @ d).abs(), limit(x, d)
     assert (err <= lim).all(), float((err / lim).max())
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows", [1, 3, 7])
+@pytest.mark.parametrize("first,second", [(5, 9), (5, 40), (5, 70), (130, 249), (64, 127)])
+@pytest.mark.parametrize("signs", [(1, 1), (1, -1), (-1, -1)])
+def test_several_infinities(handle, first, second, signs, rows, group):
+    """Of one sign or of both, in one step, tile or group or not: infinite of the sum's sign, NaN where both meet or a weight is 0."""
+    codes, scales, z = weights(250, 500, group, True, 6)
+    w, d = la.pack_int4(handle, codes, scales, z, group=group), dense(codes, scales, z, group)
+    x = torch.randn(rows, 250, device="cuda", generator=torch.Generator(device="cuda").manual_seed(8))
+    clean, y = torch.empty(rows, 500, device="cuda"), torch.empty(rows, 500, device="cuda")
+    la.gemv_int4(handle, clean, x, w)
+    x[-1, first], x[-1, second] = signs[0] * math.inf, signs[1] * math.inf
+    la.gemv_int4(handle, y, x, w)
+    want = x[-1, first].double() * d[first] + x[-1, second].double() * d[second]
+    nan = torch.isnan(want)
+    assert nan.any() and not nan.all()
+    assert torch.equal(torch.isnan(y[-1]), nan) and torch.equal(y[-1].double()[~nan], want[~nan])
+    assert torch.equal(y[:-1], clean[:-1])
