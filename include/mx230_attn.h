@@ -530,7 +530,7 @@ int mx230_gemv_int8(mx230_handle *h, void *stream, float *y, const float *x, con
  * stride); otherwise y lies apart from what is read.  n_in up to 65536, any n_out and number of rows (eight at a time go over the weights, so it is built for a few).  A row's
  * bits do not depend on the rows computed with it.  `packed` (mx230_int4_bytes, 16-byte aligned) is made once by mx230_pack_int4 from codes [n_in][n_out] (the
  * low four bits of a byte), fp16 scales and zeros [ceil(n_in / group)][n_out] (zeros null: 8); group 32 or a multiple of 64.
- * x goes in as two fp16 parts relative to the largest of 64 (off by half an ulp of fp32, or 2^-39 of that largest one), codes less
+ * x goes in as two fp16 parts relative to the largest of 64 (off by an ulp of fp32, or 2^-39 of that largest one), codes less
  * zero points (0 to 255) as they are; sums are fp32.
  * A row with infinite x has the infinite or NaN y that the formula gives.
  * No workspace. */

@@ -11,7 +11,7 @@
 // sum |x| (q + z): with one x of 10^4 among 4096 whose own weight is 0, 9e-5 of the result.)  The rows are the eight columns of B, two
 // columns a row:
 //   x 2^e = hi + lo, both fp16, e such that the largest of the 64 values of a tile lies in [2^14, 2^15):
-// |x 2^e - hi - lo| <= 2^-24 |x 2^e|, as exact as x itself (but for values 2^-17 times the tile's largest and less, which keep an
+// |x 2^e - hi - lo| <= 2^-23 |x 2^e|, an ulp of fp32 (but for values 2^-17 times the tile's largest and less, which keep an
 // absolute error of 2^-39 of that).  Products are then exact in fp32; sums are fp32, per tile of 64 inputs (32, if groups are of
 // 32).  The row's total gets s 2^(10 - e) times the tile's sum.  Infinite x are
 // infinite in hi and 0 in lo, so sums are infinite or NaN as those of x itself.
