@@ -503,15 +503,16 @@ extern "C" int mx230_gemv_int4(mx230_handle *h, void *stream, float *y, const fl
     rc = clusters_held(h, P.ctas_k, &held);
     if (rc) return rc;
     const bool g32 = group == 32;
-    // Output tiles of a warp, which share what is read of the rows.  Four rows: one, two or four, whichever needs least time, taken as
-    // rounds of the clusters times 3, 5 or 9 (three rows and more: 10).  One row, us with one / two / four: 896 x 1152 2.3, 2.7, 3.5;
-    // 4096 x 4096 5.3, 5.0, 6.5; 4096 x 14336 12.1, 11.8, 11.5; 4096 x 128000 78, 67, 59 (four rows 83, 69, 72).  Eight rows: two where there
-    // is a round of them and three stages fit beside the rows (14336 x 4096 25.1, 22.4; 4096 x 14336, where two stages would, 18.9, 21.3).
+    // Output tiles of a warp, which share what is read of the rows.  Up to two rows: one, two or four, whichever needs least time, taken as
+    // rounds of the clusters times 3, 5 or 9; three and four rows: one or two.  One row, us with one / two / four: 896 x 1152 2.2, 2.4, 3.0;
+    // 4096 x 4096 5.2, 5.0, 6.3; 4096 x 14336 11.9, 11.7, 11.8; 14336 x 4096 17.5, 13.8, 12.2; 4096 x 128000 75, 65, 62 (four rows 78, 67, 73;
+    // 14336 x 4096 18.4, 14.5, 14.0).  Eight rows: two where there is a round of them and three stages fit beside the rows (14336 x 4096
+    // 26.4, 20.0; 4096 x 14336 19.3, 18.7; in groups of 32, where two stages would, 20.5, 21.5).
     int t = 1;
     if (nt == 1) {
-        const int cost[3] = {30, 50, n_rows < 3 ? 89 : 101};
+        const int cost[3] = {30, 50, 89};
         long long best = 0;
-        for (int i = 0; i < 3; ++i) {
+        for (int i = 0; i < (n_rows < 3 ? 3 : 2); ++i) {
             const long long groups = (P.n_tiles + (1 << i) - 1) >> i, time = (groups + held - 1) / held * cost[i];
             if (i == 0 || time < best) best = time, t = 1 << i;
         }

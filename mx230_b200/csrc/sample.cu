@@ -772,17 +772,22 @@ template <typename T>
 int launch_sample(mx230_handle *h, cudaStream_t st, SampleParams P, int n_rows) {
     constexpr int VE = 16 / (int)sizeof(T);
     const int pieces = P.vocab / VE + 2;
-    // CTAs of a row, each with a few thousand logits: two or four where the clusters (which find no place on some SMs)
-    // then all run at once, two CTAs an SM, four of short rows a little earlier; two also where they need up to three halves of that, unless
-    // short rows are asked for a few entries, where what comes behind the passes counts more; eight for a few rows.  us with one / two / four / eight: 64 rows of 128000, top-p 96, 72, 51, 70; 70 rows with two
-    // and four 71, 55; 100 rows 118, 79, 85; 200 rows 142, 124, 134; of 50257, top-k 40, 148 rows 21, 23, 43, and 222 rows 30, 42, 59; 16 rows of 128000, top-k 50,
-    // kept, 43, 29, 18, 24; one row, top-p, kept, 77, 48, 28, 21.
+    // CTAs of a row, each with a few thousand logits, by whether their clusters then all run at once.  us with one / two / four / eight,
+    // in fp32 but for 50257 (bf16), "own" with settings of each row's own:
+    //   eight, which leave room for half as many CTAs as there are SMs: 128000, top-p: 9 rows 137, 80, 41, 28; 16 rows 139, 81, 41, 55;
+    //   four, where two would not keep the row: 128000, top-p: 32 rows 143, 90, 43, 46; 70 rows 166, 108, 68, 112; 74 rows 144, 86, 111, 118.
+    //     Short rows only where four keep it too: 50257, top-p: 33 rows 57, 35, 25, 35; 38 rows 57, 34, 37, 51; top-k 18, 14, 16, 24;
+    //   two, two of them an SM: 148 rows of 50257, top-p 61, 57, 97; 147 rows of it, top-k 25, 22, 42; 148 rows of 128000, top-p 150, 116, 171.
+    //     Up to half as many again, since rows take unequal time: 200 rows of 50257, own, 82, 60, 74; top-p 86, 92, 109; 200 rows of 128000, top-p 210,
+    //     188, 196.  But not short rows of which a few entries are asked for, all alike: 200 rows of 50257, top-k 29, 40, 48.  (Where each row
+    //     has its own k they are taken to be unequal: the host does not see them.)
     const bool few = P.top_ks == nullptr && P.top_k > 0 && P.top_k <= SM_LIST / 2;
     const bool short_row = P.vocab <= 65536;
     auto fits = [&](int to) {
-        const long long all = (long long)n_rows * to;
-        if (to == SM_CLUSTER) return all <= h->sm_count / 2;
-        return all * 10 <= (short_row ? 17ll : 19ll) * h->sm_count || (to == 2 && all <= 3ll * h->sm_count && !(few && short_row));
+        const long long all = (long long)n_rows * to, sms = h->sm_count;
+        if (to == 8) return all * 2 <= sms;
+        if (to == 4) return all * 10 <= (short_row ? 9 : 19) * sms;   // (clusters of four find no place on a tenth of the SMs)
+        return all <= 2 * sms || (all <= 3 * sms && !(few && short_row));
     };
     int c = 1;
     while (c < SM_CLUSTER && P.vocab / c > 4096 && fits(2 * c)) c *= 2;
@@ -790,12 +795,12 @@ int launch_sample(mx230_handle *h, cudaStream_t st, SampleParams P, int n_rows) 
     P.ctas = c;
     P.power = POWER_OF_TWO;
     const dim3 grid((unsigned)(n_rows * c));
-    // The row stays in shared memory where its CTAs all have their places with that (32 rows of 128000, four CTAs each: 34 us, read
-    // again 45); else it is read again (64 rows: 51, kept 62).
+    // The row stays in shared memory where its CTAs all have their places with that (top-p: 33 rows of 128000, four CTAs each: 43 us, read
+    // again 63; 34 rows, which have not, 83 and 64; 64 rows 85 and 67; 64 rows of 50257, two each: 35 and 53).
     const size_t kept = sizeof(Shared) + (size_t)share * sizeof(float);
     MX_SMEM_ATTR_ONCE(h->device, (sample_kernel<T, true>), SM_ALL);
     MX_SMEM_ATTR_ONCE(h->device, (sample_kernel<T, false>), sizeof(Shared));
-    if ((kept <= SM_HALF && (long long)n_rows * c <= 2ll * h->sm_count) || (kept <= SM_ALL && (long long)n_rows * c <= h->sm_count)) MX_LAUNCH(h, st, MX230_K_SAMPLE, mx_launch(sample_kernel<T, true>, grid, SM_THREADS, kept, st, c, true, P));
+    if ((kept <= SM_HALF && (long long)n_rows * c <= 2ll * h->sm_count) || (kept <= SM_ALL && (long long)n_rows * c * 10 <= (c > 2 ? 9ll : 10ll) * h->sm_count)) MX_LAUNCH(h, st, MX230_K_SAMPLE, mx_launch(sample_kernel<T, true>, grid, SM_THREADS, kept, st, c, true, P));
     else MX_LAUNCH(h, st, MX230_K_SAMPLE, mx_launch(sample_kernel<T, false>, grid, SM_THREADS, sizeof(Shared), st, c, true, P));
     return MX230_OK;
 }
