@@ -1,4 +1,5 @@
-"""Products with 4-bit weights where sums could lose what a 64-bit sum does not: inputs that are far larger than the others, or infinite.
+"""Products with 4-bit weights where sums could lose what a 64-bit sum does not: inputs that are far larger than the others, or infinite;
+and groups of 32 with outputs wide enough for two and four output tiles a warp.
 
 Tolerance, against M = sum |x| |w|.  Weights are exact, x is off by 2^-23 |x| or by 2^-39 of the largest of its 64.  The 16 products of a
 step are added by the tensor core, taken as 17 truncations of 2^-24 M (what it keeps is not documented): 2^-19 M for all steps with
@@ -73,3 +74,19 @@ def test_several_infinities(handle, first, second, signs, rows, group):
     assert nan.any() and not nan.all()
     assert torch.equal(torch.isnan(y[-1]), nan) and torch.equal(y[-1].double()[~nan], want[~nan])
     assert torch.equal(y[:-1], clean[:-1])
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("n_in,n_out,rows", [(896, 5001, 1), (4096, 6000, 2), (97, 40001, 1), (2047, 4000, 4), (33, 9007, 2), (700, 30000, 3), (4160, 14336, 1), (31, 20001, 2)])
+def test_wide_products_in_groups_of_32(handle, n_in, n_out, rows, zeros):
+    """An odd number of groups, inputs that end inside one, outputs that end inside a tile or a warp's tiles; a row's bits are those of the row alone."""
+    codes, scales, z = weights(n_in, n_out, 32, zeros, n_in)
+    w, d = la.pack_int4(handle, codes, scales, z if zeros else None, group=32), dense(codes, scales, z, 32)
+    x = torch.randn(8, n_in, device="cuda", generator=torch.Generator(device="cuda").manual_seed(rows))
+    y, other, all8 = (torch.full((n, n_out), math.nan, device="cuda") for n in (rows, 1, 8))
+    la.gemv_int4(handle, y, x[:rows], w)
+    err, lim = (y.double() - x[:rows].double() @ d).abs(), limit(x[:rows], d)
+    assert (err <= lim).all(), float((err / lim).max())
+    la.gemv_int4(handle, other[0], x[rows - 1], w)
+    la.gemv_int4(handle, all8, x, w)
+    assert torch.equal(other[0], y[-1]) and torch.equal(all8[:rows], y)
