@@ -32,6 +32,7 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "pieces.h"
 
 namespace {
 
@@ -477,10 +478,18 @@ extern "C" int mx230_gemv_int4(mx230_handle *h, void *stream, float *y, const fl
                "gemv_int4: rows of y share memory, or a stride is negative (x %lld, y %lld, add %lld)", x_stride, y_stride, add_stride);
     MX_REQUIRE(((uintptr_t)packed & 15) == 0 && (((uintptr_t)x | (uintptr_t)y | (uintptr_t)bias | (uintptr_t)add) & 3) == 0, MX230_ERR_INVALID_ARG,
                "gemv_int4: misaligned pointer");
-    MX_REQUIRE(x != y && bias != y, MX230_ERR_INVALID_ARG, "gemv_int4: y is x or the bias, which other blocks still read");
     MX_REQUIRE(add != y || n_rows < 2 || add_stride == y_stride, MX230_ERR_INVALID_ARG, "gemv_int4: add is y, with another stride");
     MX_REQUIRE(n_rows <= 65535 * 4, MX230_ERR_UNSUPPORTED, "gemv_int4: %d rows", n_rows);
     MX_REQUIRE(n_in <= 2 * W4_K_CTA * W4_CLUSTER * W4_K, MX230_ERR_UNSUPPORTED, "gemv_int4: n_in %d (at most %d)", n_in, 2 * W4_K_CTA * W4_CLUSTER * W4_K);
+    auto rows_of = [&](const void *at, int n, long long stride) {
+        return Pieces{at, (size_t)n * 4, 1, 0, n_rows, n_rows < 2 ? 0 : (long long)((unsigned long long)stride * 4)};
+    };
+    const Pieces out = rows_of(y, n_out, y_stride);
+    MX_REQUIRE(!pieces_overlap(out, rows_of(x, n_in, x_stride)), MX230_ERR_INVALID_ARG, "gemv_int4: y shares memory with x, which other blocks still read");
+    MX_REQUIRE(bias == nullptr || !pieces_overlap(out, {bias, (size_t)n_out * 4, 1, 0, 1, 0}), MX230_ERR_INVALID_ARG, "gemv_int4: y shares memory with the bias");
+    MX_REQUIRE(add == nullptr || add == y || !pieces_overlap(out, rows_of(add, n_out, add_stride)), MX230_ERR_INVALID_ARG,
+               "gemv_int4: add shares memory with y, but is not y");
+    MX_REQUIRE(!pieces_overlap(out, {packed, mx230_int4_bytes(n_in, n_out, group), 1, 0, 1, 0}), MX230_ERR_INVALID_ARG, "gemv_int4: y shares memory with the weights");
     Int4Params P{};
     P.y = y, P.x = x, P.bias = bias, P.add = add;
     P.codes = (const uint4 *)packed, P.sz = (const uint32_t *)((const char *)packed + codes_bytes(n_in, n_out));
