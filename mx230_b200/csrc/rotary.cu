@@ -18,6 +18,7 @@
 #include <math.h>
 
 #include "common.cuh"
+#include "pieces.h"
 
 namespace {
 
@@ -296,8 +297,9 @@ extern "C" int mx230_rotary(mx230_handle *h, void *stream, void *out, const void
     if (n_rows == 0 || n_head == 0) return MX230_OK;
     MX_REQUIRE(out && x && turns, MX230_ERR_INVALID_ARG, "rotary: null argument");
     MX_REQUIRE(x_row >= 0 && x_head >= 0 && out_row >= 0 && out_head >= 0, MX230_ERR_INVALID_ARG, "rotary: negative stride");
-    {   // the outputs lie apart: the smaller stride spans a head, the larger one all that lies under it
-        const bool heads_inside = n_rows < 2 || (n_head >= 2 && out_head <= out_row);
+    // the outputs lie apart: the smaller stride spans a head, the larger one all that lies under it
+    const bool heads_inside = n_rows < 2 || (n_head >= 2 && out_head <= out_row);
+    {
         const long long in_s = heads_inside ? out_head : out_row, out_s = heads_inside ? out_row : out_head;
         const int in_n = heads_inside ? n_head : n_rows, out_n = heads_inside ? n_rows : n_head;
         MX_REQUIRE((in_n < 2 || in_s >= head_dim) && (out_n < 2 || out_s >= (in_n < 2 ? 0 : in_s * (in_n - 1)) + head_dim), MX230_ERR_INVALID_ARG,
@@ -308,6 +310,14 @@ extern "C" int mx230_rotary(mx230_handle *h, void *stream, void *out, const void
     const size_t size = dtype == MX230_F32 ? 4 : 2;
     MX_REQUIRE(((uintptr_t)x | (uintptr_t)out) % size == 0 && (uintptr_t)turns % 8 == 0 && (uintptr_t)pos % 4 == 0, MX230_ERR_INVALID_ARG,
                "rotary: misaligned pointer");
+    if (x != out) {
+        auto heads_of = [&](const void *at, long long row, long long head) {
+            row = (long long)((unsigned long long)row * size), head = (long long)((unsigned long long)head * size);
+            return heads_inside ? Pieces{at, head_dim * size, n_head, head, n_rows, row} : Pieces{at, head_dim * size, n_rows, row, n_head, head};
+        };
+        MX_REQUIRE(!pieces_overlap(heads_of(out, out_row, out_head), heads_of(x, x_row, x_head)), MX230_ERR_INVALID_ARG,
+                   "rotary: out shares memory with x, which other blocks still read, but is not x");
+    }
     RotaryParams P{};
     P.out = out, P.x = x, P.pos = pos, P.pos0 = pos0, P.turns = turns, P.factor = factor;
     P.n_rows = n_rows, P.n_head = n_head, P.head_dim = head_dim, P.half = rot_dim / 2, P.inverse = inverse ? 1 : 0;

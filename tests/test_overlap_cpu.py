@@ -92,3 +92,12 @@ def test_int4(L):
               dict(bias=P), dict(bias=P + 1020), dict(bias=P - 252), dict(add=P + 4), dict(add=P + 4 * 64), dict(add=P - 4 * 64), dict(add=P + 8, adds=0),
               dict(rows=1, add=P + 4), dict(packed=P), dict(packed=P + 1008), dict(packed=P - 4 * 4 * 576 + 16)]:
         assert refused(L, L.mx230_gemv_int4(*{**ok, **c}.values())), c
+
+
+def test_rotary(L):
+    ok = dict(h=H, st=None, out=P, x=P + (1 << 30), dt=0, pos=None, pos0=0, turns=P - (1 << 20), factor=1.0, rows=4, heads=2, dim=64, rot=64, inter=0, inv=0,
+              xr=128, xh=64, outr=128, outh=64)
+    for c in [dict(x=P + 4), dict(x=P - 4), dict(x=P + 256), dict(x=P - 256), dict(x=P + 4 * 511), dict(x=P - 4 * 511), dict(x=P + 2, dt=1), dict(x=P + 2 * 511, dt=2),
+              dict(outr=256, xr=256, x=P + 4 * 64), dict(outr=256, xr=256, x=P + 4 * 127), dict(outr=64, outh=256, x=P + 256), dict(xr=0, xh=0, x=P + 2000),
+              dict(outr=400, outh=64, xr=64, xh=400, x=P + 4 * 300), dict(rows=1, x=P + 252), dict(heads=1, outh=0, xh=0, outr=64, x=P + 1020)]:
+        assert refused(L, L.mx230_rotary(*{**ok, **c}.values())), c
