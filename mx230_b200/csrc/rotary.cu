@@ -220,17 +220,18 @@ int launch_t(mx230_handle *h, cudaStream_t st, RotaryParams P, bool inter) {
     P.slots = P.units >= RT_THREADS ? 1 : RT_THREADS / P.units;
     // Rows and heads of a block: enough for every thread to have its heads in flight twice, unless that left SMs without a block.
     P.heads_per_block = P.n_head;
-    int rows = (2 * RT_UNROLL * P.slots + P.n_head - 1) / P.n_head;
-    const int fill = (P.n_rows + 2 * h->sm_count - 1) / (2 * h->sm_count);
+    auto parts = [](long long n, long long of) { return (n + of - 1) / of; };   // (of numbers up to the largest int)
+    int rows = (int)parts(2 * RT_UNROLL * P.slots, P.n_head);
+    const int fill = (int)parts(P.n_rows, 2 * h->sm_count);
     if (rows > fill) rows = fill;
     const int pairs = n == 1 ? 1 : inter ? n / 2 : n, row_cs = (P.half + pairs - 1) / pairs * pairs;
     if (rows > RT_PAIRS / row_cs) rows = RT_PAIRS / row_cs;
     if (rows < 1) rows = 1;
     P.rows_per_block = rows;
     // few rows: the heads of a row over several blocks
-    while (P.heads_per_block > P.slots && (long long)((P.n_rows + rows - 1) / rows) * ((P.n_head + P.heads_per_block - 1) / P.heads_per_block) < 2 * h->sm_count)
-        P.heads_per_block = (P.heads_per_block + 1) / 2;
-    const dim3 grid((unsigned)((P.n_rows + rows - 1) / rows), (unsigned)((P.n_head + P.heads_per_block - 1) / P.heads_per_block));
+    while (P.heads_per_block > P.slots && parts(P.n_rows, rows) * parts(P.n_head, P.heads_per_block) < 2 * h->sm_count)
+        P.heads_per_block = (int)parts(P.heads_per_block, 2);
+    const dim3 grid((unsigned)parts(P.n_rows, rows), (unsigned)parts(P.n_head, P.heads_per_block));
     MX_REQUIRE(grid.y <= 65535, MX230_ERR_UNSUPPORTED, "rotary: %d heads", P.n_head);
     if constexpr (sizeof(T) == 2)
         if (n == 8) return launch_n<T, 8>(h, st, P, grid, inter);
