@@ -629,6 +629,10 @@ int mx230_sched_admit(mx230_sched *s, int *request, int *table_out);
 int mx230_sched_admitted(mx230_sched *s, int request, uint32_t first_token);
 int mx230_sched_batch(mx230_sched *s, int *n_active, uint32_t *cur, int *pos, int *tables);
 int mx230_sched_step_done(mx230_sched *s, const uint32_t *next_tokens);
+/* Ends a request that awaits its first token or is being decoded, whose result stays as it is (in an open decode step: with
+ * mx230_sched_step_done, which does not take its token); its blocks go back to the pool.  request -1: all of these, at once; an open step is
+ * then over.  The scheduler goes on with the other requests.  mx230_sched_destroy gives no blocks back (it does not look at the pool). */
+int mx230_sched_end(mx230_sched *s, int request);
 int mx230_sched_result(const mx230_sched *s, int request, uint32_t *out, int cap, int *n);
 long long mx230_sched_stat(const mx230_sched *s, int which); /* ServeStats gpu.rs:366: 0 decode_steps, 1 seq_decodes, 2 admitted */
 

@@ -376,6 +376,7 @@ extern "C" {
         s: *mut Mx230Sched, n_active: *mut c_int, cur: *mut u32, pos: *mut c_int, tables: *mut c_int,
     ) -> c_int;
     pub fn mx230_sched_step_done(s: *mut Mx230Sched, next_tokens: *const u32) -> c_int;
+    pub fn mx230_sched_end(s: *mut Mx230Sched, request: c_int) -> c_int;
     pub fn mx230_sched_result(
         s: *const Mx230Sched, request: c_int, out: *mut u32, cap: c_int, n: *mut c_int,
     ) -> c_int;

@@ -24,6 +24,7 @@ struct mx230_sched {
         int pos;                 // position of `cur` (its KV is written by the next step)
         uint32_t cur;
         int target;
+        bool ended = false;      // by mx230_sched_end, in the open decode step
     };
     std::vector<Slot> active;
     std::vector<std::vector<uint32_t>> results;
@@ -145,6 +146,10 @@ extern "C" int mx230_sched_step_done(mx230_sched *s, const uint32_t *next_tokens
     std::vector<mx230_sched::Slot> keep;
     for (size_t i = 0; i < s->active.size(); ++i) {
         mx230_sched::Slot &sl = s->active[i];
+        if (sl.ended) {
+            release(s, sl.table, sl.need);
+            continue;
+        }
         sl.cur = next_tokens[i];
         sl.pos += 1;
         s->results[sl.req].push_back(next_tokens[i]);
@@ -153,6 +158,38 @@ extern "C" int mx230_sched_step_done(mx230_sched *s, const uint32_t *next_tokens
     }
     s->active.swap(keep);
     s->batch_open = false;
+    return MX230_OK;
+}
+
+// Ends a request early: one that was handed out and not confirmed, or one of the active set.
+extern "C" int mx230_sched_end(mx230_sched *s, int request) {
+    MX_REQUIRE(s && request >= -1, MX230_ERR_INVALID_ARG, "sched_end: bad argument");
+    const bool all = request < 0;
+    bool found = all;
+    if (s->pending_req >= 0 && (all || request == s->pending_req)) {
+        release(s, s->pending_table, s->pending_need);
+        s->pending_req = -1;
+        ++s->next_req;
+        found = true;
+    }
+    if (all) s->batch_open = false;
+    std::vector<mx230_sched::Slot> keep;
+    for (mx230_sched::Slot &sl : s->active) {
+        if (!all && sl.req != request) {
+            keep.push_back(sl);
+            continue;
+        }
+        MX_REQUIRE(all || !sl.ended, MX230_ERR_INVALID_ARG, "sched_end: request %d was ended in this step", request);
+        found = true;
+        if (s->batch_open) {
+            sl.ended = true;
+            keep.push_back(sl);
+        } else {
+            release(s, sl.table, sl.need);
+        }
+    }
+    MX_REQUIRE(found, MX230_ERR_INVALID_ARG, "sched_end: request %d is not being served", request);
+    s->active.swap(keep);
     return MX230_OK;
 }
 

@@ -57,7 +57,10 @@ class Scheduler:
         self.n_log = lib().mx230_sched_n_log(self._s)
 
     def close(self):
+        """Requests that are still being served end here; their blocks go back to the pool."""
         if self._s:
+            if self.pool._p:
+                lib().mx230_sched_end(self._s, -1)
             lib().mx230_sched_destroy(self._s)
             self._s = C.c_void_p()
 
@@ -90,6 +93,10 @@ class Scheduler:
     def step_done(self, next_tokens) -> None:
         nt = np.ascontiguousarray(next_tokens, np.uint32)
         check(lib().mx230_sched_step_done(self._s, nt.ctypes.data_as(C.c_void_p)))
+
+    def end(self, request: int) -> None:
+        """Ends a request that awaits its first token or is being decoded (within a step: with `step_done`, which does not take its token)."""
+        check(lib().mx230_sched_end(self._s, request))
 
     def result(self, request: int) -> list[int]:
         n = C.c_int(0)

@@ -1,0 +1,111 @@
+"""Requests that end early, and serving that is left by an error: every block is back in the pool, and the others are served as before
+(no GPU: a pure function in place of the model)."""
+import gc
+
+import pytest
+
+from mx230_b200._lib import Mx230Error
+from mx230_b200.paging import KvPool
+from mx230_b200.serving import Request, Scheduler, run_continuous
+
+BS, N_CTX = 16, 64
+
+
+class Model:
+    def prefill(self, r, prompt, table):
+        return sum(prompt) * 31 % 1000
+
+    def decode_batched(self, cur, pos, tables):
+        return [(int(c) * 131 + int(p) * 17) % 1000 for c, p in zip(cur, pos)]
+
+
+REQUESTS = [Request([1, 2, 3], 9), Request([4] * 20, 1), Request([5] * 10, 30), Request([6] * 33, 12), Request([7], 20)]
+
+
+class Stop(Exception):
+    pass
+
+
+@pytest.mark.parametrize("where", ["prefill", "decode_batched"])
+@pytest.mark.parametrize("calls", [0, 1, 3])
+def test_an_error_of_the_model_gives_the_blocks_back(where, calls):
+    pool, model, left = KvPool(30 * BS, BS), Model(), [calls]
+    plain = getattr(model, where)
+
+    def failing(*a):
+        left[0] -= 1
+        if left[0] < 0:
+            raise Stop
+        return plain(*a)
+
+    setattr(model, where, failing)
+    with pytest.raises(Stop):
+        run_continuous(model, pool, N_CTX, REQUESTS, 3)
+    assert pool.free_blocks == 30
+    pool.audit()
+    setattr(model, where, plain)
+    out, _ = run_continuous(model, pool, N_CTX, REQUESTS, 3)
+    assert [len(o) for o in out] == [r.max_new for r in REQUESTS] and pool.free_blocks == 30
+
+
+def serve(pool, ends=()):
+    """The loop of run_continuous, with requests ended at (request, tokens so far)."""
+    s, m, ended = Scheduler(pool, N_CTX, 3, REQUESTS), Model(), set()
+    while True:
+        while (adm := s.admit()) is not None:
+            r, table = adm
+            if (r, 0) in ends:
+                s.end(r)
+                ended.add(r)
+            else:
+                s.admitted(r, m.prefill(r, REQUESTS[r].prompt, table))
+        cur, pos, tables = s.batch()
+        if not cur.size:
+            break
+        for r in range(len(REQUESTS)):
+            if r not in ended and (r, len(s.result(r))) in ends:
+                s.end(r)
+                ended.add(r)
+                with pytest.raises(Mx230Error):
+                    s.end(r)   # in this step already
+        s.step_done(m.decode_batched(cur, pos, tables))
+    got = [s.result(r) for r in range(len(REQUESTS))]
+    for r in (0, len(REQUESTS) - 1, len(REQUESTS)):
+        with pytest.raises(Mx230Error):
+            s.end(r)   # not being served (any more)
+    s.close()
+    return got
+
+
+def test_requests_that_end_early():
+    pool = KvPool(30 * BS, BS)
+    want = serve(pool)
+    for ends in [{(0, 1)}, {(2, 0)}, {(2, 29), (0, 4)}, {(1, 0), (3, 11), (4, 1)}, {(4, 19), (0, 8)}, {(0, 0), (1, 0), (2, 0), (3, 0), (4, 0)}]:
+        got = serve(pool, ends)
+        cut = dict(ends)
+        assert got == [w[:cut.get(r, len(w))] for r, w in enumerate(want)], ends
+        assert pool.free_blocks == 30
+        pool.audit()
+
+
+def test_a_scheduler_that_is_left_in_the_middle():
+    for step in range(4):
+        pool = KvPool(30 * BS, BS)
+        s = Scheduler(pool, N_CTX, 3, REQUESTS)
+        r, _ = s.admit()
+        if step > 0:
+            s.admitted(r, 7)
+        if step > 1:
+            s.batch()
+        if step > 2:
+            s.end(r)
+        assert pool.free_blocks < 30
+        s.close()
+        assert pool.free_blocks == 30, step
+        pool.audit()
+    s = Scheduler(pool, N_CTX, 3, REQUESTS)
+    s.admit()
+    pool.close()   # the pool first: nothing is given back to it
+    s.close()
+    del s, pool
+    gc.collect()
