@@ -14,13 +14,13 @@ return logits instead (device tensors, [vocab] and [n][vocab]), and the tokens a
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import numpy as np
 
 import torch
 
-from ._lib import check, lib, require, require_int32
+from ._lib import ERR_INVALID_ARG, Mx230Error, check, lib, require, require_int32
 from .common import Handle, raw_stream
 from .llm_attention import _DTYPES, on_device
 from .paging import KvPool
@@ -44,6 +44,7 @@ class ServeStats:
     decode_steps: int = 0
     seq_decodes: int = 0
     admitted: int = 0
+    ended: list = field(default_factory=list)   # requests that ended before their last token (see run_continuous)
 
 
 class Scheduler:
@@ -138,6 +139,14 @@ def sample(h: Handle, token, logits, u, temperature=1.0, top_k=0, top_p=1.0, min
                              vector("sample: u", u, torch.float32), t, ts, k, ks, p, ps, m, ms))
 
 
+class MaskedLogits(Mx230Error):
+    """Every logit of some rows is masked: `tokens` has -1 for those, and the tokens of the others."""
+
+    def __init__(self, tokens, what: str):
+        super().__init__(ERR_INVALID_ARG, what)
+        self.tokens = tokens
+
+
 class Sampler:
     """Draws the tokens of `run_continuous`.  The random number of a request's t-th token depends on (seed, request, t) alone, so a
     request's tokens do not depend on what is served beside it."""
@@ -151,7 +160,7 @@ class Sampler:
         return (int(bits) >> 40) * 2.0 ** -24
 
     def draw(self, logits, rows) -> list[int]:
-        """One token for each of `rows`, (request index, step, Request), from its row of `logits`."""
+        """One token for each of `rows`, (request index, step, Request), from its row of `logits`.  Raises `MaskedLogits` where a row has none."""
         logits = logits.reshape(len(rows), -1)
         dev = lambda a, t: torch.tensor(a, dtype=t, device=logits.device)  # noqa: E731
         token = torch.empty(len(rows), dtype=torch.int32, device=logits.device)
@@ -159,8 +168,8 @@ class Sampler:
                dev([q.temperature for *_, q in rows], torch.float32), dev([q.top_k for *_, q in rows], torch.int32),
                dev([q.top_p for *_, q in rows], torch.float32), dev([q.min_p for *_, q in rows], torch.float32))
         out = token.tolist()
-        for (r, t, _), tok in zip(rows, out):
-            require(tok >= 0, lambda: f"request {r}: every logit of token {t} is masked")
+        if min(out, default=0) < 0:
+            raise MaskedLogits(out, ", ".join(f"request {r}: every logit of token {t} is masked" for (r, t, _), tok in zip(rows, out) if tok < 0))
         return out
 
 
@@ -168,9 +177,24 @@ def run_continuous(model, pool: KvPool, n_ctx: int, requests: list[Request], max
                    sampler: Sampler | None = None):
     """Serves `requests` keeping up to `max_batch` sequences decoding together; returns each
     request's generated tokens (request order) and the occupancy statistics.  `trace`, when given,
-    receives one tuple per event (for tests).  `sampler`: the model returns logits, and it draws the tokens."""
+    receives one tuple per event (for tests).  `sampler`: the model returns logits, and it draws the tokens; a request whose logits are
+    masked throughout ends with the tokens that it has, is named in the statistics, and the others go on."""
     s = Scheduler(pool, n_ctx, max_batch, requests)
     owner = {}   # first block of a running request's table -> the request
+    ended = []   # requests that ended early
+
+    def draw(logits, rows):
+        try:
+            return sampler.draw(logits, rows)
+        except MaskedLogits as e:
+            for (r, t, _), tok in zip(rows, e.tokens):
+                if tok < 0:
+                    s.end(r)
+                    ended.append(r)
+                    if trace is not None:
+                        trace.append(("end", r, t))
+            return [max(tok, 0) for tok in e.tokens]
+
     try:
         while True:
             while (adm := s.admit()) is not None:
@@ -178,7 +202,9 @@ def run_continuous(model, pool: KvPool, n_ctx: int, requests: list[Request], max
                 first = model.prefill(r, requests[r].prompt, table)
                 if sampler is not None:
                     owner[int(table[0])] = r
-                    first = sampler.draw(first, [(r, 0, requests[r])])[0]
+                    first = draw(first, [(r, 0, requests[r])])[0]
+                    if r in ended:
+                        continue
                 if trace is not None:
                     trace.append(("admit", r, table.tolist(), int(first)))
                 s.admitted(r, first)
@@ -188,10 +214,12 @@ def run_continuous(model, pool: KvPool, n_ctx: int, requests: list[Request], max
             nxt = model.decode_batched(cur.copy(), pos.copy(), tables.copy())
             if sampler is not None:
                 rows = [owner[int(t[0])] for t in tables]
-                nxt = sampler.draw(nxt, [(r, int(p) - len(requests[r].prompt) + 1, requests[r]) for r, p in zip(rows, pos)])
+                nxt = draw(nxt, [(r, int(p) - len(requests[r].prompt) + 1, requests[r]) for r, p in zip(rows, pos)])
             if trace is not None:
                 trace.append(("step", cur.tolist(), pos.tolist(), tables.tolist(), [int(x) for x in nxt]))
             s.step_done(nxt)
-        return [s.result(r) for r in range(len(requests))], s.stats()
+        stats = s.stats()
+        stats.ended = sorted(ended)
+        return [s.result(r) for r in range(len(requests))], stats
     finally:
         s.close()

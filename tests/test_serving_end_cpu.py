@@ -6,7 +6,7 @@ import pytest
 
 from mx230_b200._lib import Mx230Error
 from mx230_b200.paging import KvPool
-from mx230_b200.serving import Request, Scheduler, run_continuous
+from mx230_b200.serving import MaskedLogits, Request, Scheduler, run_continuous
 
 BS, N_CTX = 16, 64
 
@@ -109,3 +109,44 @@ def test_a_scheduler_that_is_left_in_the_middle():
     s.close()
     del s, pool
     gc.collect()
+
+
+class Draws:
+    """Tokens from (request, step) alone; none for the ones that are named."""
+
+    def __init__(self, masked=()):
+        self.masked = masked
+
+    def draw(self, logits, rows):
+        out = [-1 if (r, t) in self.masked else (r * 37 + t * 11) % 1000 for r, t, _ in rows]
+        if min(out) < 0:
+            raise MaskedLogits(out, "masked")
+        return out
+
+
+def test_masked_logits_end_their_request_alone():
+    pool = KvPool(30 * BS, BS)
+    want, st = run_continuous(Model(), pool, N_CTX, REQUESTS, 3, sampler=Draws())
+    assert st.ended == [] and [len(w) for w in want] == [r.max_new for r in REQUESTS]
+    for masked in [{(1, 0)}, {(0, 0), (2, 7)}, {(0, 4), (2, 4), (3, 3)}, {(4, 19)}, {(r, 0) for r in range(5)}]:
+        trace = []
+        got, st = run_continuous(Model(), pool, N_CTX, REQUESTS, 3, trace=trace, sampler=Draws(masked))
+        cut = dict(masked)
+        assert got == [w[:cut.get(r, len(w))] for r, w in enumerate(want)], masked
+        assert st.ended == sorted(cut) and sorted(e[1:] for e in trace if e[0] == "end") == sorted(masked)
+        assert pool.free_blocks == 30
+        pool.audit()
+    assert issubclass(MaskedLogits, Mx230Error)
+
+
+def test_another_error_of_the_draw_gives_the_blocks_back():
+    class Failing(Draws):
+        def draw(self, logits, rows):
+            if rows[0][1] == 3:
+                raise Stop
+            return super().draw(logits, rows)
+
+    pool = KvPool(30 * BS, BS)
+    with pytest.raises(Stop):
+        run_continuous(Model(), pool, N_CTX, REQUESTS, 3, sampler=Failing())
+    assert pool.free_blocks == 30
