@@ -628,6 +628,7 @@ int mx230_sched_n_log(const mx230_sched *s);
 int mx230_sched_admit(mx230_sched *s, int *request, int *table_out);
 int mx230_sched_admitted(mx230_sched *s, int request, uint32_t first_token);
 int mx230_sched_batch(mx230_sched *s, int *n_active, uint32_t *cur, int *pos, int *tables);
+int mx230_sched_requests(const mx230_sched *s, int *requests, int cap); /* those of the batch's rows; returns how many there are */
 int mx230_sched_step_done(mx230_sched *s, const uint32_t *next_tokens);
 /* Ends a request that awaits its first token or is being decoded, whose result stays as it is (in an open decode step: with
  * mx230_sched_step_done, which does not take its token); its blocks go back to the pool.  request -1: all of these, at once; an open step is

@@ -375,6 +375,7 @@ extern "C" {
     pub fn mx230_sched_batch(
         s: *mut Mx230Sched, n_active: *mut c_int, cur: *mut u32, pos: *mut c_int, tables: *mut c_int,
     ) -> c_int;
+    pub fn mx230_sched_requests(s: *const Mx230Sched, requests: *mut c_int, cap: c_int) -> c_int;
     pub fn mx230_sched_step_done(s: *mut Mx230Sched, next_tokens: *const u32) -> c_int;
     pub fn mx230_sched_end(s: *mut Mx230Sched, request: c_int) -> c_int;
     pub fn mx230_sched_result(

@@ -138,6 +138,13 @@ extern "C" int mx230_sched_batch(mx230_sched *s, int *n_active, uint32_t *cur, i
     return MX230_OK;
 }
 
+// The requests of the batch's rows, in batch order.
+extern "C" int mx230_sched_requests(const mx230_sched *s, int *requests, int cap) {
+    if (!s || !requests) return -1;
+    for (int i = 0; i < (int)s->active.size() && i < cap; ++i) requests[i] = s->active[i].req;
+    return (int)s->active.size();
+}
+
 // The step's next tokens, in batch order: appended to the results; finished sequences retire.
 extern "C" int mx230_sched_step_done(mx230_sched *s, const uint32_t *next_tokens) {
     MX_REQUIRE(s && next_tokens && s->batch_open, MX230_ERR_INVALID_ARG, "sched_step_done: no open decode step");

@@ -91,6 +91,11 @@ class Scheduler:
                                       pos.ctypes.data_as(C.c_void_p), tables.ctypes.data_as(C.c_void_p)))
         return cur[:n.value], pos[:n.value], tables[:n.value]
 
+    def requests(self) -> list[int]:
+        """The request of each row of the batch."""
+        out = np.empty(self.max_batch, np.int32)
+        return out[:lib().mx230_sched_requests(self._s, out.ctypes.data_as(C.c_void_p), out.size)].tolist()
+
     def step_done(self, next_tokens) -> None:
         nt = np.ascontiguousarray(next_tokens, np.uint32)
         check(lib().mx230_sched_step_done(self._s, nt.ctypes.data_as(C.c_void_p)))
@@ -180,7 +185,6 @@ def run_continuous(model, pool: KvPool, n_ctx: int, requests: list[Request], max
     receives one tuple per event (for tests).  `sampler`: the model returns logits, and it draws the tokens; a request whose logits are
     masked throughout ends with the tokens that it has, is named in the statistics, and the others go on."""
     s = Scheduler(pool, n_ctx, max_batch, requests)
-    owner = {}   # first block of a running request's table -> the request
     ended = []   # requests that ended early
 
     def draw(logits, rows):
@@ -201,7 +205,6 @@ def run_continuous(model, pool: KvPool, n_ctx: int, requests: list[Request], max
                 r, table = adm
                 first = model.prefill(r, requests[r].prompt, table)
                 if sampler is not None:
-                    owner[int(table[0])] = r
                     first = draw(first, [(r, 0, requests[r])])[0]
                     if r in ended:
                         continue
@@ -213,8 +216,7 @@ def run_continuous(model, pool: KvPool, n_ctx: int, requests: list[Request], max
                 break
             nxt = model.decode_batched(cur.copy(), pos.copy(), tables.copy())
             if sampler is not None:
-                rows = [owner[int(t[0])] for t in tables]
-                nxt = draw(nxt, [(r, int(p) - len(requests[r].prompt) + 1, requests[r]) for r, p in zip(rows, pos)])
+                nxt = draw(nxt, [(r, int(p) - len(requests[r].prompt) + 1, requests[r]) for r, p in zip(s.requests(), pos)])
             if trace is not None:
                 trace.append(("step", cur.tolist(), pos.tolist(), tables.tolist(), [int(x) for x in nxt]))
             s.step_done(nxt)

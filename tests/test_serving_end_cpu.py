@@ -150,3 +150,26 @@ def test_another_error_of_the_draw_gives_the_blocks_back():
     with pytest.raises(Stop):
         run_continuous(Model(), pool, N_CTX, REQUESTS, 3, sampler=Failing())
     assert pool.free_blocks == 30
+
+
+def test_the_draw_is_told_the_requests_by_the_scheduler(monkeypatch):
+    """Not by their blocks: a table whose first block is another request's too changes nothing."""
+    asked = []
+
+    class Asking(Draws):
+        def draw(self, logits, rows):
+            asked.append([(r, t, q is REQUESTS[r]) for r, t, q in rows])
+            return super().draw(logits, rows)
+
+    want, _ = run_continuous(Model(), KvPool(30 * BS, BS), N_CTX, REQUESTS, 3, sampler=Asking())
+    plain, batch, admit = asked.copy(), Scheduler.batch, Scheduler.admit
+    asked.clear()
+
+    def first_block(table):
+        table[..., 0] = 5
+        return table
+
+    monkeypatch.setattr(Scheduler, "batch", lambda s: (lambda c, p, t: (c, p, first_block(t)))(*batch(s)))
+    monkeypatch.setattr(Scheduler, "admit", lambda s: (lambda a: None if a is None else (a[0], first_block(a[1])))(admit(s)))
+    got, _ = run_continuous(Model(), KvPool(30 * BS, BS), N_CTX, REQUESTS, 3, sampler=Asking())
+    assert got == want and asked == plain and all(same for rows in asked for *_, same in rows)
