@@ -165,8 +165,11 @@ class Sampler:
         return (int(bits) >> 40) * 2.0 ** -24
 
     def draw(self, logits, rows) -> list[int]:
-        """One token for each of `rows`, (request index, step, Request), from its row of `logits`.  Raises `MaskedLogits` where a row has none."""
-        logits = logits.reshape(len(rows), -1)
+        """One token for each of `rows`, (request index, step, Request), from its row of `logits` [rows][vocab], or [vocab] for one.
+        Raises `MaskedLogits` where a row has none."""
+        if logits.dim() == 1:
+            logits = logits[None]
+        require(logits.dim() == 2 and logits.shape[0] == len(rows), lambda: f"logits {tuple(logits.shape)} for {len(rows)} sequences")
         dev = lambda a, t: torch.tensor(a, dtype=t, device=logits.device)  # noqa: E731
         token = torch.empty(len(rows), dtype=torch.int32, device=logits.device)
         sample(self.h, token, logits, dev([self.uniform(r, t) for r, t, _ in rows], torch.float32),

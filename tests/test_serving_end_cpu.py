@@ -3,10 +3,12 @@
 import gc
 
 import pytest
+import torch
 
+from mx230_b200 import serving
 from mx230_b200._lib import Mx230Error
 from mx230_b200.paging import KvPool
-from mx230_b200.serving import MaskedLogits, Request, Scheduler, run_continuous
+from mx230_b200.serving import MaskedLogits, Request, Sampler, Scheduler, run_continuous
 
 BS, N_CTX = 16, 64
 
@@ -173,3 +175,21 @@ def test_the_draw_is_told_the_requests_by_the_scheduler(monkeypatch):
     monkeypatch.setattr(Scheduler, "admit", lambda s: (lambda a: None if a is None else (a[0], first_block(a[1])))(admit(s)))
     got, _ = run_continuous(Model(), KvPool(30 * BS, BS), N_CTX, REQUESTS, 3, sampler=Asking())
     assert got == want and asked == plain and all(same for rows in asked for *_, same in rows)
+
+
+@pytest.mark.parametrize("shape,n", [((8, 50), 4), ((4, 50), 8), ((100,), 2), ((50,), 0), ((2, 2, 25), 4), ((1, 1, 50), 1), ((), 1), ((3, 50), 1)])
+def test_logits_of_another_number_of_rows(monkeypatch, shape, n):
+    """As of a step that is padded to the largest batch: its rows are not regrouped."""
+    from types import SimpleNamespace
+
+    def drawn(*a, **k):
+        raise AssertionError("drawn")
+
+    monkeypatch.setattr(serving, "sample", drawn)
+    sampler = Sampler(SimpleNamespace(device=0))
+    with pytest.raises(Mx230Error) as e:
+        sampler.draw(torch.zeros(shape), [(r, 0, REQUESTS[0]) for r in range(n)])
+    assert not isinstance(e.value, MaskedLogits)
+    for shape in ((50,), (1, 50)):
+        with pytest.raises(AssertionError, match="drawn"):
+            sampler.draw(torch.zeros(shape), [(0, 0, REQUESTS[0])])
