@@ -18,12 +18,17 @@ from dataclasses import dataclass, field
 
 import numpy as np
 
-import torch
-
 from ._lib import ERR_INVALID_ARG, Mx230Error, check, lib, require, require_int32
 from .common import Handle, raw_stream
-from .llm_attention import _DTYPES, on_device
 from .paging import KvPool
+
+torch = None   # brought in by the first draw: the scheduler runs on hosts without it
+
+
+def _need_torch() -> None:
+    global torch, _DTYPES, on_device
+    import torch
+    from .llm_attention import _DTYPES, on_device
 
 
 @dataclass
@@ -123,6 +128,8 @@ def sample(h: Handle, token, logits, u, temperature=1.0, top_k=0, top_p=1.0, min
     falling order the first top_k, of those the shortest prefix with top_p of their weight, cut at min_p times the largest
     weight; among what is kept, in the order of the vocabulary, the token is where the running weight passes u's share.  -1
     where a row is masked throughout."""
+    if torch is None:
+        _need_torch()
     dev, dtype = h.device, _DTYPES.get(logits.dtype)
     require(logits.dim() == 2 and dtype is not None, lambda: f"sample: logits {tuple(logits.shape)} of {logits.dtype}")
     (n, vocab), (row, one) = logits.shape, logits.stride()
@@ -167,6 +174,8 @@ class Sampler:
     def draw(self, logits, rows) -> list[int]:
         """One token for each of `rows`, (request index, step, Request), from its row of `logits` [rows][vocab], or [vocab] for one.
         Raises `MaskedLogits` where a row has none."""
+        if torch is None:
+            _need_torch()
         if logits.dim() == 1:
             logits = logits[None]
         require(logits.dim() == 2 and logits.shape[0] == len(rows), lambda: f"logits {tuple(logits.shape)} for {len(rows)} sequences")

@@ -1,6 +1,9 @@
 """Requests that end early, and serving that is left by an error: every block is back in the pool, and the others are served as before
 (no GPU: a pure function in place of the model)."""
 import gc
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -193,3 +196,18 @@ def test_logits_of_another_number_of_rows(monkeypatch, shape, n):
     for shape in ((50,), (1, 50)):
         with pytest.raises(AssertionError, match="drawn"):
             sampler.draw(torch.zeros(shape), [(0, 0, REQUESTS[0])])
+
+
+WITHOUT_TORCH = """
+import sys
+sys.modules["torch"] = None
+from mx230_b200.paging import KvPool
+from mx230_b200.serving import Request, Sampler, Scheduler
+s = Scheduler(KvPool(64), 64, 2, [Request([1, 2], 3)])
+assert s.admit()[0] == 0
+"""
+
+
+def test_the_scheduler_needs_no_torch(lib_built):
+    done = subprocess.run([sys.executable, "-c", WITHOUT_TORCH], capture_output=True, text=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert done.returncode == 0, done.stderr[-2000:]
