@@ -456,7 +456,7 @@ class Int4Weights:
 def pack_int4(h: Handle, codes, scales, zeros=None, group: int | None = None, stream=None) -> Int4Weights:
     """Lays out weights scale * (code - zero) once for `gemv_int4`: `codes` uint8 [n_in][n_out] (low four bits), `scales` fp16 and
     `zeros` uint8 [groups][n_out] (None: 8).  A group is 32 inputs or a multiple of 64; `group` may be left out where the
-    number of groups determines it among the powers of two.  Allocates the result: not for the step path."""
+    number of groups determines it among the powers of two.  Allocates the result, on `stream`: not for the step path."""
     require(codes.dim() == 2 and scales.dim() == 2 and scales.shape[1] == codes.shape[1], "pack_int4: codes [n_in][n_out], scales [groups][n_out]")
     n_in, n_out = codes.shape
     groups = scales.shape[0]
@@ -471,8 +471,11 @@ def pack_int4(h: Handle, codes, scales, zeros=None, group: int | None = None, st
     if zeros is not None:
         on_device(h, "pack_int4: zeros", zeros, torch.uint8)
         require(zeros.shape == scales.shape and zeros.is_contiguous(), "pack_int4: zeros must be contiguous, of the scales' shape")
-    packed = torch.empty(lib().mx230_int4_bytes(n_in, n_out, group), dtype=torch.uint8, device=codes.device)
-    check(lib().mx230_pack_int4(h._h, raw_stream(stream, h.device), packed.data_ptr(), addr(codes), addr(scales), addr(zeros), n_in, n_out, group))
+    on = raw_stream(stream, h.device)
+    # (on the stream that writes it: memory that was freed on another one may still be in use there)
+    with torch.cuda.stream(None if stream is None else torch.cuda.ExternalStream(on, device=codes.device)):
+        packed = torch.empty(lib().mx230_int4_bytes(n_in, n_out, group), dtype=torch.uint8, device=codes.device)
+    check(lib().mx230_pack_int4(h._h, on, packed.data_ptr(), addr(codes), addr(scales), addr(zeros), n_in, n_out, group))
     return Int4Weights(packed, n_in, n_out, group)
 
 

@@ -90,3 +90,25 @@ def test_wide_products_in_groups_of_32(handle, n_in, n_out, rows, zeros):
     la.gemv_int4(handle, other[0], x[rows - 1], w)
     la.gemv_int4(handle, all8, x, w)
     assert torch.equal(other[0], y[-1]) and torch.equal(all8[:rows], y)
+
+
+def test_packed_on_another_stream(handle):
+    """Its memory is not what was freed on the current stream, where work may still use it."""
+    codes, scales, z = weights(4096, 2048, 64, True, 3)
+    side = torch.cuda.Stream()
+    x, y, want = torch.randn(2, 4096, device="cuda"), torch.empty(2, 2048, device="cuda"), torch.empty(2, 2048, device="cuda")
+    w = la.pack_int4(handle, codes, scales, z)
+    la.gemv_int4(handle, want, x, w)
+    size, freed = w.nbytes(), w.packed.data_ptr()
+    del w
+    torch.cuda.synchronize()
+    for stream in (side, side.cuda_stream):
+        w = la.pack_int4(handle, codes, scales, z, stream=stream)
+        assert w.nbytes() == size and w.packed.data_ptr() != freed
+        side.synchronize()
+        y.zero_()
+        la.gemv_int4(handle, y, x, w)
+        assert torch.equal(y, want)
+        torch.cuda.synchronize()
+    again = la.pack_int4(handle, codes, scales, z)
+    assert again.packed.data_ptr() == freed   # (the allocator does give that memory to the stream it was freed on)
