@@ -171,6 +171,18 @@ def test_masked_rows_infinities_and_zeros(handle):
     check(handle, torch.tensor([[-inf, 6e4, inf, -6e4, 0.0]]).half(), [0.6])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_more_infinities_than_a_list(handle, dtype):
+    """They count as the largest number, one as much as another: the first ones by index are kept."""
+    x = logits_of(4, 40000, 2.0, 3, dtype)
+    x[0, 100:9000] = math.inf
+    x[1, ::3] = math.inf
+    x[2, 7], x[2, 39999] = math.inf, math.inf
+    x[3, 1::2], x[3, ::2] = math.inf, -math.inf
+    for s in (dict(), dict(k=1500), dict(k=1500, p=0.5), dict(p=0.3), dict(k=3), dict(m=0.5), dict(t=0.0), dict(k=20000, m=1.0)):
+        check(handle, x, [0.0, 0.5, 0.7, 0.9999], **s, what=s)
+
+
 @pytest.mark.parametrize("t", [1e-45, 1e-44, 1e-42, 1e-40, 3e-39, 8e-39, 1.2e-38, 1e-37, 1e-36, 1e-30])
 @pytest.mark.parametrize("scale", [1.0, 20.0, 1000.0, 1e5])
 def test_the_smallest_temperatures(handle, t, scale):
