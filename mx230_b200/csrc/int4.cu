@@ -16,6 +16,9 @@
 // 32).  The row's total gets s 2^(10 - e) times the tile's sum.  Infinite x are
 // infinite in hi and 0 in lo, so sums are infinite or NaN as those of x itself.
 //
+// About 84 instructions a warp and tile at one to four rows.  4096 x 14336, one row: 11.5 us where HBM would need 4.7, bounded by latency
+// (seventeen warps an SM, each scheduler issues in 0.45 of its cycles); 4096 x 128000, four rows: 67 to 71 where it would need 42 (0.61).
+//
 // Layout, made once by mx230_pack_int4: tiles of 16 outputs x 64 inputs, 512 bytes, of which lane (g = lane / 4, j = lane % 4) has 16:
 // words [row g: inputs 8j .. 8j+7][row g: inputs 32 + 8j ..][row g + 8: 8j ..][row g + 8: 32 + 8j ..], input 2p of eight at bits
 // 4p, input 2p + 1 at bits 16 + 4p.  (Which input a k index of the MMA stands for is free, as long as A and B agree.)  Tiles of an

@@ -12,8 +12,9 @@
 // with "the first entry of the order whose running count or mass exceeds t"; then what is kept is known, and the token is the
 // first one by index whose running mass exceeds t.
 //
-// The logits have to be read once, 4 or 2 bytes each; what bounds the kernel is what a weight takes (64 rows of
-// 128000 in fp32 with top-p 0.95: 68 us, 5 of them HBM's), and for a few rows latency (one row of 32000: 10 us).
+// The logits have to be read once, 4 or 2 bytes each; what bounds the kernel is latency: for many rows what a weight takes, a chain
+// of fp64, and barriers (64 rows of 128000 in fp32 with top-p 0.95: 67 us, 5 of them HBM's; half of the cycles issue), for a few rows the
+// cluster's barriers (one row of 32000: 10 us).
 // A cluster of one to eight CTAs takes a row, each a part of the vocabulary that follows the one before.  A histogram over 2048 equal
 // intervals of max - l, as far as weights are not 0 (28.7 T), in counts (top-k) or masses says in which interval K or P ends.  If all
 // down to there is one list, its entries are collected, sorted and summed, and what is kept of them is sorted again by index.  Else the
