@@ -239,3 +239,16 @@ def test_captured_strided_and_on_another_stream(handle):
     serving.sample(handle, token, x, u, 0.8, k, 0.9)
     torch.cuda.synchronize()
     assert torch.equal(other, token)
+
+
+def test_a_masked_row_among_others(handle):
+    """The sampler says which row has no token, and has the others'."""
+    sampler, x = serving.Sampler(handle, 3), logits_of(4, 500, 2.0, 1).cuda()
+    rows = [(r, r + 1, serving.Request([1], 9, 0.8, 40, 0.9)) for r in range(4)]
+    want = sampler.draw(x, rows)
+    x[2] = math.nan
+    with pytest.raises(serving.MaskedLogits, match="request 2") as e:
+        sampler.draw(x, rows)
+    assert e.value.tokens == [*want[:2], -1, want[3]]
+    x[2, 7] = 1.0
+    assert sampler.draw(x, rows) == [*want[:2], 7, want[3]]
